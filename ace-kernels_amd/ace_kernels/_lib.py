@@ -43,6 +43,10 @@ EXPORTS = (
     "ace_forward_noalloc",
     "ace_forward_f64",
     "ace_backward_f64",
+    "ace_vocab_saved_bytes",
+    "ace_vocab_workspace_bytes",
+    "ace_vocab_forward",
+    "ace_vocab_backward",
 )
 
 # ace_forward_noalloc's scratch (ACE_NOALLOC_SCRATCH_BYTES) and its error code
@@ -161,6 +165,25 @@ def lib() -> ctypes.CDLL:
         _i, ctypes.POINTER(AceBwdLevel), _i,
         _i64, _i64, _i, _i, _i, _i, _i,        # B, C, K, binning, include_bg, right, per_class
         _p, _p, _p,                            # bin_table, centre_table, stream
+    ]
+    handle.ace_vocab_saved_bytes.restype = _sz
+    handle.ace_vocab_saved_bytes.argtypes = [_i64]
+    handle.ace_vocab_workspace_bytes.restype = _sz
+    handle.ace_vocab_workspace_bytes.argtypes = [_i, _i64, _i64, _i64, _i]
+    handle.ace_vocab_forward.restype = _i
+    handle.ace_vocab_forward.argtypes = [
+        _p, _p, _i, _p,            # hidden, weight, dtype, labels
+        _i64, _i64, _i64, _i64,    # tokens, hidden_size, vocab, ignore_index
+        _i, _p, _p, _p, _p,        # reduction, saved, loss, confidence, correct
+        _p, _sz, _p,               # workspace, bytes, stream
+    ]
+    handle.ace_vocab_backward.restype = _i
+    handle.ace_vocab_backward.argtypes = [
+        _p, _p, _i,                # hidden, weight, dtype
+        _i64, _i64, _i64,          # tokens, hidden_size, vocab
+        _i, _p, _p, _p,            # reduction, saved, grad_loss, grad_confidence
+        _p, _p,                    # d_hidden, d_weight
+        _p, _sz, _p,               # workspace, bytes, stream
     ]
     handle.ace_set_launch_events.restype = _i
     handle.ace_set_launch_events.argtypes = [_p, _p]

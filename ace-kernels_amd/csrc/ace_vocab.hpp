@@ -1,0 +1,750 @@
+// Softmax cross entropy of hidden states against a vocabulary, with each
+// token's top-label confidence, and its gradients (ace_vocab_forward /
+// ace_vocab_backward, declared in include/ace_hip.h).
+//
+//   s_tv  = h_t . w_v                         never kept: formed tile by tile
+//   lse_t = log sum_v exp s_tv,  nll_t = lse_t - s_t,y
+//   a_t   = argmax_v s_tv,       conf_t = exp(s_t,a - lse_t)
+//   dS_tv = g_t (p_tv - [v = y_t]) + c_t conf_t ([v = a_t] - p_tv)
+//   dh_t  = sum_v dS_tv w_v,     dw_v = sum_t dS_tv h_t
+//
+// with g and c the upstream gradients of nll and conf.  Tokens whose label is
+// not counted are left out at the start: the others' hidden states are copied
+// together (`rows`), so ignored tokens cost nothing and whatever they hold, NaN
+// included, reaches no result.  How many there are is known on the device only;
+// grids are sized for all tokens and the kernels spread the work that there is.
+//
+// Forward: every block forms tiles of vocabulary x tokens (ace_mma.hpp) and
+// folds each into a running maximum and sum per token, held per lane and joined
+// across lanes, waves and blocks at the end.
+// Backward: for each piece of the vocabulary, one kernel forms the tiles again,
+// takes dS from the kept maximum and sum and stores it (in the inputs' type: the
+// matrix cores' operand), one forms the piece's dw, and one adds its part of dh.
+//
+// All sums, the running maxima, the logits and the partial dh are float32.
+#pragma once
+
+#include <float.h>
+#include <hip/hip_ext.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ace_mma.hpp"
+
+namespace ace {
+namespace vocab {
+
+using mma::f32x4;
+using mma::kStep;
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kNone = 0x7fffffff;  // no index
+constexpr int kPrepBlocks = 512;   // most blocks of the kernels that walk tokens
+
+// What a forward leaves for its backward, in one allocation of 4-byte words:
+// the number of counted tokens (`rows`), then n words each of
+struct Saved {
+  int* count;    // [0]: counted tokens
+  int* token;    // row -> token
+  int* row;      // token -> row, -1 if not counted
+  int* label;    // row -> label
+  int* best;     // row -> argmax
+  float* top;    // row -> largest logit
+  float* inv;    // row -> 1 / sum of exp(s - top)
+};
+
+constexpr int kSavedHead = 64;  // words before the arrays
+
+__host__ __device__ inline Saved saved_of(void* p, int64_t n) {
+  int* w = static_cast<int*>(p);
+  int* a = w + kSavedHead;
+  return Saved{w,         a,         a + n, a + 2 * n, a + 3 * n, reinterpret_cast<float*>(a + 4 * n),
+               reinterpret_cast<float*>(a + 5 * n)};
+}
+
+template <typename T>
+struct Four {
+  typedef T type __attribute__((ext_vector_type(4)));
+};
+
+// The first `left` of four neighbouring values at `at`, in T; one store where
+// the row allows it (`vec`: rows are whole aligned groups of four).
+template <typename T>
+__device__ inline void store4(T* at, f32x4 x, int64_t left, bool vec) {
+  const typename Four<T>::type v{(T)x[0], (T)x[1], (T)x[2], (T)x[3]};
+  if (vec && left >= 4) {
+    *reinterpret_cast<typename Four<T>::type*>(at) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (e < left) at[e] = v[e];
+  }
+}
+
+// A block's share of one token's softmax.
+struct Part {
+  float top, sum;
+  int best, pad;
+};
+
+__device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+
+// (top, sum, best) of two disjoint sets of words: the larger logit, the lower
+// index where they are equal.
+__device__ inline void join(float& top, float& sum, int& best, float top2, float sum2, int best2) {
+  const float t = fmaxf(top, top2);
+  best = top2 > top || (top2 == top && best2 < best) ? best2 : best;
+  // a set without a logit has sum 0 and the lowest top: its factor is 0 or 1
+  sum = sum * exp_of(top - t) + sum2 * exp_of(top2 - t);
+  top = t;
+}
+
+// ----------------------------------------------------------- rows of tokens
+
+struct PrepParams {
+  const int64_t* labels;
+  int64_t ignore, vocab;
+  const void* hidden;
+  void* rows;          // [n, width] the counted tokens' hidden states
+  int64_t n;
+  int hidden_size, width;  // width: hidden_size rounded up to 16 bytes
+  int vec;             // rows of `hidden` are whole aligned 16-byte chunks
+  int per_block;       // tokens (forward) or rows (backward) a block handles
+  Saved saved;
+  float* nll;          // outputs of tokens that are not counted: 0 (or null)
+  float* confidence;
+  float* correct;
+  char* zeros;         // 16 zero bytes for the kernels that follow
+  int* ticket;
+};
+
+// Copies the rows `token[0..count)` of `hidden` (LDS list) to rows at..
+template <typename T>
+__device__ inline void copy_rows(const void* hidden, void* rows, int hidden_size, int width,
+                                 int vec, const int* token, int count, int64_t at) {
+  if (vec) {
+    const int chunks = width * (int)sizeof(T) / 16;
+    for (int64_t i = threadIdx.x; i < (int64_t)count * chunks; i += blockDim.x) {
+      const int j = (int)(i / chunks), c = (int)(i % chunks);
+      reinterpret_cast<uint4*>(rows)[(at + j) * chunks + c] =
+          reinterpret_cast<const uint4*>(hidden)[(int64_t)token[j] * chunks + c];
+    }
+  } else {
+    for (int64_t i = threadIdx.x; i < (int64_t)count * width; i += blockDim.x) {
+      const int j = (int)(i / width), c = (int)(i % width);
+      T v{};
+      if (c < hidden_size) v = static_cast<const T*>(hidden)[(int64_t)token[j] * hidden_size + c];
+      static_cast<T*>(rows)[(at + j) * width + c] = v;
+    }
+  }
+}
+
+// Numbers the counted tokens, and copies their labels and hidden states
+// together.  Each block counts the labels before its own by itself: cheaper than
+// another launch, as the labels are few and in the caches.
+template <typename T>
+__global__ __launch_bounds__(256) void prep_kernel(PrepParams p) {
+  __shared__ int s_count[4], s_token[256];
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t first = (int64_t)blockIdx.x * p.per_block;
+  const int64_t last = first + p.per_block < p.n ? first + p.per_block : p.n;
+  auto counted = [&](int64_t t) {
+    const int64_t y = p.labels[t];
+    return y >= 0 && y < p.vocab && y != p.ignore;
+  };
+  if (blockIdx.x == 0 && tid < 4) {
+    reinterpret_cast<int*>(p.zeros)[tid] = 0;
+    if (tid == 0) *p.ticket = 0;
+  }
+  int before = 0;
+  for (int64_t t = tid; t < first; t += 256) before += counted(t);
+  for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
+  if (lane == 0) s_count[wave] = before;
+  __syncthreads();
+  int64_t row = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+  for (int64_t t0 = first; t0 < last; t0 += 256) {
+    __syncthreads();
+    const int64_t t = t0 + tid;
+    const bool in = t < last, yes = in && counted(t);
+    const unsigned long long m = __ballot(yes);
+    if (lane == 0) s_count[wave] = __popcll(m);
+    __syncthreads();
+    int at = __popcll(m & ((1ull << lane) - 1));
+    for (int w = 0; w < wave; ++w) at += s_count[w];
+    const int here = s_count[0] + s_count[1] + s_count[2] + s_count[3];
+    if (yes) {
+      s_token[at] = (int)t;
+      p.saved.token[row + at] = (int)t;
+      p.saved.label[row + at] = (int)p.labels[t];
+      p.saved.row[t] = (int)(row + at);
+    } else if (in) {
+      p.saved.row[t] = -1;
+      if (p.nll) p.nll[t] = 0.f;
+      if (p.confidence) p.confidence[t] = 0.f;
+      if (p.correct) p.correct[t] = 0.f;
+    }
+    __syncthreads();
+    copy_rows<T>(p.hidden, p.rows, p.hidden_size, p.width, p.vec, s_token, here, row);
+    row += here;
+  }
+  if (blockIdx.x == gridDim.x - 1 && tid == 0) *p.saved.count = (int)row;
+}
+
+// Rows of a weight whose rows are not whole aligned 16-byte chunks, padded to
+// `width` with zeros.
+template <typename T>
+__global__ __launch_bounds__(256) void pad_kernel(const T* src, T* dst, int64_t rows, int size,
+                                                  int width) {
+  for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
+    for (int c = (int)threadIdx.x; c < width; c += 256)
+      dst[r * width + c] = c < size ? src[r * size + c] : T{};
+}
+
+// ------------------------------------------------------------------ forward
+
+struct ScoreParams {
+  const char* weight;  // [vocab, width]
+  const char* rows;    // [n, width]
+  int64_t vocab;
+  int hidden_size, width;
+  Saved saved;
+  const char* zeros;
+  // forward
+  Part* part;          // [blocks + token tiles][BN]
+  float* label_logit;  // row -> s_ty
+  // backward
+  int64_t v0;          // first word of this piece
+  int64_t v1;          // end of it
+  int64_t stride;      // elements of a row of ds
+  void* ds;            // [n, stride]
+  const float* g;      // row -> upstream of nll
+  const float* c;      // row -> upstream of conf, times conf; null: none
+  const float* bound;  // float16: blocks' largest |g| + |c|, and how many
+  int bounds;
+  float* scale;        // float16: the power of two that ds is multiplied by (out)
+};
+
+// The tile walk that forward and backward share: this block's units are tiles
+// (token tile, vocabulary tile), vocabulary fastest.  `fold(tt, vt, acc)` takes
+// a finished tile, `enter(tt)` and `leave(tt)` a token tile's run of them.  The
+// first step of the next tile loads while `fold` works.
+template <class TL, class Enter, class Fold, class Leave>
+__device__ inline void walk_tiles(const ScoreParams& p, int64_t v0, int64_t v1, Enter enter,
+                                  Fold fold, Leave leave) {
+  using T = typename TL::T;
+  const int count = *p.saved.count;
+  const int tts = (count + TL::BN - 1) / TL::BN;
+  const int vts = (int)((v1 - v0 + TL::BM - 1) / TL::BM);
+  if (tts == 0) return;
+  const mma::Spread spread{(int64_t)tts * vts, (int)gridDim.x};
+  const int b = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const int64_t u0 = spread.begin(b), u1 = spread.begin(b + 1);
+  if (u0 >= u1) return;
+  char* lds = mma::lds_base();
+  const int64_t row_bytes = (int64_t)p.width * sizeof(T);
+  const int k = p.width;
+  const int steps = (k + kStep<T> - 1) / kStep<T>;
+  typename TL::OpA a;
+  typename TL::OpB bo;
+  typename TL::Source sa, sb;
+  sa.step = sb.step = mma::kStepBytes;
+  int tt = (int)(u0 / vts), vt = (int)(u0 % vts);
+  auto aim = [&](bool tokens) {
+    a.init(row_bytes, v0 + (int64_t)vt * TL::BM, v1);
+    sa.base = p.weight + (v0 + (int64_t)vt * TL::BM) * row_bytes;
+    if (tokens) {
+      bo.init(row_bytes, (int64_t)tt * TL::BN, count);
+      sb.base = p.rows + (int64_t)tt * TL::BN * row_bytes;
+    }
+  };
+  aim(true);
+  TL::load(a, bo, sa, sb, 0, k, lds, p.zeros);
+  int buf = 0;
+  f32x4 acc[TL::MT][TL::NT];
+  enter(tt);
+  for (int64_t u = u0; u < u1; ++u) {
+    const int this_tt = tt, this_vt = vt;
+    const bool more = u + 1 < u1, turn = more && vt + 1 == vts;
+    TL::clear(acc);
+    for (int s = 0; s < steps; ++s) {
+      mma::landed_barrier();
+      if (s + 1 < steps) {
+        TL::load(a, bo, sa, sb, s + 1, k, lds + (buf ^ 1) * TL::kStageBytes, p.zeros);
+      } else if (more) {
+        vt = turn ? 0 : vt + 1;
+        tt += turn;
+        aim(turn);
+        TL::load(a, bo, sa, sb, 0, k, lds + (buf ^ 1) * TL::kStageBytes, p.zeros);
+      }
+      TL::step(lds + buf * TL::kStageBytes, acc);
+      buf ^= 1;
+    }
+    fold(this_tt, this_vt, acc);
+    if (turn || !more) {
+      leave(this_tt);
+      if (turn) enter(tt);
+    }
+  }
+}
+
+template <class TL>
+__global__ __launch_bounds__(TL::kThreads) void score_kernel(ScoreParams p) {
+  constexpr int NT = TL::NT, MT = TL::MT;
+  __shared__ Part s_part[TL::WM][TL::BN];
+  const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int count = *p.saved.count;
+  float top[NT], sum[NT];
+  int best[NT], label[NT];
+  auto enter = [&](int tt) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      top[j] = -FLT_MAX;
+      sum[j] = 0.f;
+      best[j] = kNone;
+      const int r = tt * TL::BN + TL::wave_n() + 16 * j + n;
+      label[j] = r < count ? p.saved.label[r] : -1;
+    }
+  };
+  auto fold = [&](int tt, int vt, f32x4(&acc)[MT][NT]) {
+    const int v_wave = vt * TL::BM + TL::wave_m();  // the wave's first word
+    const int left = (int)(p.vocab - v_wave) - 4 * g;
+    if (p.vocab - v_wave < TL::BM / TL::WM) {  // ragged end: words that do not exist
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (16 * i + e >= left) acc[i][j][e] = -INFINITY;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float t = top[j];
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t = fmaxf(t, acc[i][j][e]);
+      if (__ballot(t > top[j])) {
+        // a new largest logit somewhere in the wave: where it stands.  Words
+        // come in ascending order, so the first place that has it stays.
+        int at = kNone;
+#pragma unroll
+        for (int i = MT - 1; i >= 0; --i)
+#pragma unroll
+          for (int e = 3; e >= 0; --e) at = acc[i][j][e] == t ? v_wave + 16 * i + 4 * g + e : at;
+        if (t > top[j]) best[j] = at;
+      }
+      // the lane's words that the label may be among: v_wave + 4 g + 16 i + e
+      const int y = label[j] - v_wave - 4 * g;
+      if (__ballot(y >= 0 && y < TL::BM / TL::WM && (y & 12) == 0)) {
+        float s = 0.f;
+        bool mine = false;
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (y == 16 * i + e) {
+              s = acc[i][j][e];
+              mine = true;
+            }
+        if (mine) p.label_logit[tt * TL::BN + TL::wave_n() + 16 * j + n] = s;
+      }
+      float l = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) l += exp_of(acc[i][j][e] - t);
+      sum[j] = sum[j] * exp_of(top[j] - t) + l;
+      top[j] = t;
+    }
+  };
+  const int blk = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
+  auto leave = [&](int tt) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int d = 16; d < 64; d *= 2)
+        join(top[j], sum[j], best[j], __shfl_xor(top[j], d), __shfl_xor(sum[j], d),
+             __shfl_xor(best[j], d));
+      if (g == 0)
+        s_part[(int)threadIdx.x / 64 / TL::WN][TL::wave_n() + 16 * j + n] =
+            Part{top[j], sum[j], best[j], 0};
+    }
+    __syncthreads();
+    for (int c = (int)threadIdx.x; c < TL::BN; c += TL::kThreads) {
+      Part q = s_part[0][c];
+#pragma unroll
+      for (int w = 1; w < TL::WM; ++w)
+        join(q.top, q.sum, q.best, s_part[w][c].top, s_part[w][c].sum, s_part[w][c].best);
+      p.part[((int64_t)blk + tt) * TL::BN + c] = q;
+    }
+    __syncthreads();
+  };
+  walk_tiles<TL>(p, 0, p.vocab, enter, fold, leave);
+}
+
+// ----------------------------------------------------------------- backward
+
+struct UpstreamParams {
+  PrepParams copy;
+  int reduction;
+  const float* grad_loss;  // one value, or [n] for none; null: 0
+  const float* grad_conf;  // [n] or null
+  float* g;
+  float* c;
+  float* bound;            // [blocks]
+};
+
+// The rows' upstream gradients, and the counted tokens' hidden states together
+// again (cheaper to copy twice than to keep).
+template <typename T>
+__global__ __launch_bounds__(256) void upstream_kernel(UpstreamParams p) {
+  __shared__ int s_token[256];
+  __shared__ float s_max[4];
+  const PrepParams& q = p.copy;
+  const int tid = (int)threadIdx.x, count = *q.saved.count;
+  if (blockIdx.x == 0 && tid < 4) reinterpret_cast<int*>(q.zeros)[tid] = 0;
+  const int64_t first = (int64_t)blockIdx.x * q.per_block;
+  const int64_t last = first + q.per_block < count ? first + q.per_block : count;
+  float most = 0.f;
+  for (int64_t r0 = first; r0 < last; r0 += 256) {
+    __syncthreads();
+    const int64_t r = r0 + tid;
+    if (r < last) {
+      const int t = q.saved.token[r];
+      s_token[tid] = t;
+      float g = 0.f, c = 0.f;
+      if (p.grad_loss) {
+        g = p.reduction == 2 ? p.grad_loss[t] : p.grad_loss[0];
+        if (p.reduction == 0) g /= (float)count;
+      }
+      if (p.c) p.c[r] = c = p.grad_conf[t] * q.saved.inv[r];
+      p.g[r] = g;
+      most = fmaxf(most, fabsf(g) + fabsf(c));
+    }
+    __syncthreads();
+    if (q.rows)
+      copy_rows<T>(q.hidden, q.rows, q.hidden_size, q.width, q.vec, s_token,
+                   (int)(last - r0 < 256 ? last - r0 : 256), r0);
+  }
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+  if ((tid & 63) == 0) s_max[tid >> 6] = most;
+  __syncthreads();
+  if (tid == 0) p.bound[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+}
+
+// float16 holds dS as dS times a power of two that takes the largest |g| + |c|,
+// dS's bound, to 2^13..2^14: without it the probabilities of a large vocabulary
+// are below float16's smallest numbers.  The other types have float32's range.
+__device__ inline float scale_of(float bound) {
+  if (!(bound > 0.f) || bound > FLT_MAX) return 1.f;
+  int e;
+  frexpf(bound, &e);  // bound < 2^e
+  e = 14 - e;
+  return ldexpf(1.f, e > 100 ? 100 : e < -100 ? -100 : e);
+}
+
+template <class TL>
+__global__ __launch_bounds__(TL::kThreads) void dscore_kernel(ScoreParams p) {
+  using T = typename TL::T;
+  constexpr int NT = TL::NT, MT = TL::MT;
+  const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
+  const int count = *p.saved.count;
+  float scale = 1.f;
+  if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
+    float most = 0.f;  // every wave on its own
+    for (int i = lane; i < p.bounds; i += 64) most = fmaxf(most, p.bound[i]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+    scale = scale_of(most);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *p.scale = scale;
+  }
+  float top[NT], of_p[NT], of_label[NT], of_best[NT];
+  int label[NT], best[NT];
+  auto enter = [&](int tt) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int r = tt * TL::BN + TL::wave_n() + 16 * j + n;
+      const bool in = r < count;
+      const float gr = in ? p.g[r] * scale : 0.f;
+      const float cr = in && p.c ? p.c[r] * scale : 0.f;
+      top[j] = in ? p.saved.top[r] : 0.f;
+      of_p[j] = in ? (gr - cr) * p.saved.inv[r] : 0.f;
+      of_label[j] = gr;
+      of_best[j] = cr;
+      label[j] = in ? p.saved.label[r] : -1;
+      best[j] = in && p.c ? p.saved.best[r] : kNone;
+    }
+  };
+  auto fold = [&](int tt, int vt, f32x4(&acc)[MT][NT]) {
+    const int64_t v_tile = p.v0 + (int64_t)vt * TL::BM;
+    const int v_wave = (int)(v_tile + TL::wave_m() + 4 * g);
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      const int64_t r = (int64_t)tt * TL::BN + TL::wave_n() + 16 * j + n;
+      T* out = static_cast<T*>(p.ds) + r * p.stride + (v_wave - p.v0);
+#pragma unroll
+      for (int i = 0; i < MT; ++i) {
+        f32x4 d;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int v = v_wave + 16 * i + e;
+          float x = of_p[j] * exp_of(acc[i][j][e] - top[j]);
+          if (v == label[j]) x -= of_label[j];
+          if (v == best[j]) x += of_best[j];
+          d[e] = v < p.vocab ? x : 0.f;
+        }
+        if (r < count) store4(out + 16 * i, d, 4, true);
+      }
+    }
+  };
+  walk_tiles<TL>(p, p.v0, p.v1, enter, fold, [](int) {});
+}
+
+struct GradParams {
+  const char* a;        // m contiguous: the weight's piece, or the rows
+  int64_t a_stride;     // bytes
+  const char* b;        // ds
+  int64_t b_stride;
+  const int* count;
+  int64_t m;            // hidden size rounded up to 16 bytes
+  int64_t n;            // words of the piece (dw), unused for dh
+  int64_t k;            // words of the piece (dh), unused for dw
+  int64_t k_map;        // dh: words of a whole piece: every piece is spread alike
+  int accumulate;       // dh: not the first piece
+  float* seg;           // partial tiles [blocks + tiles][BN][BM], or null: store `out`
+  void* out;            // [n, out_stride]
+  int64_t out_stride;   // elements: the hidden size
+  int out_vec;          // rows of `out` are whole aligned groups of four
+  const float* scale;   // float16
+  const char* zeros;
+};
+
+// dh (DW = false): C[h][row] = sum over words of w[v][h] ds[row][v];
+// dw (DW = true):  C[h][v] = sum over rows of rows[row][h] ds[row][v].
+// With `seg`, tiles x steps of k are spread evenly over the blocks, and each
+// block's part of a tile goes to (or is added to) a partial tile of its own,
+// which finish_kernel adds in order.  Without it a block does a whole tile.
+template <class TL, bool DW>
+__global__ __launch_bounds__(TL::kThreads) void grad_kernel(GradParams p) {
+  using T = typename TL::T;
+  constexpr int NT = TL::NT, MT = TL::MT, es = (int)sizeof(T);
+  const int lane = (int)threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  const int count = *p.count;
+  const int64_t nn = DW ? p.n : count;
+  const int k = DW ? count : (int)p.k;
+  const int mts = (int)((p.m + TL::BM - 1) / TL::BM);
+  const int nts = (int)((nn + TL::BN - 1) / TL::BN);
+  const int all = (k + kStep<T> - 1) / kStep<T>;             // steps there are
+  const int ks = DW ? all : (int)((p.k_map + kStep<T> - 1) / kStep<T>);  // steps they are spread as
+  if (nts == 0) return;
+  const int blk = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
+  const mma::Spread spread{(int64_t)mts * nts * ks, (int)gridDim.x};
+  int64_t u = p.seg ? spread.begin(blk) : 0, end = p.seg ? spread.begin(blk + 1) : 1;
+  while (u < end) {
+    int tile, s0, s1;
+    if (p.seg) {
+      tile = (int)(u / ks);
+      s0 = (int)(u % ks);
+      const int64_t upto = end - (int64_t)tile * ks;
+      s1 = upto < ks ? (int)upto : ks;
+    } else {
+      tile = blk;
+      s0 = 0;
+      s1 = ks;
+    }
+    u += s1 - s0 > 0 ? s1 - s0 : 1;
+    if (s1 > all) s1 = all;
+    // tiles in groups of 8 along n: a group's operands are shared in L2
+    constexpr int kGroup = 8;
+    const int group = tile / (kGroup * mts), first = group * kGroup;
+    const int width = nts - first < kGroup ? nts - first : kGroup;
+    const int in_group = tile - first * mts;
+    const int64_t n0 = (int64_t)(first + in_group % width) * TL::BN;
+    const int64_t m0 = (int64_t)(in_group / width) * TL::BM;
+    const int64_t seg = (int64_t)blk + tile;
+    float* part = p.seg ? p.seg + seg * (TL::BM * TL::BN) : nullptr;
+    if (p.seg && p.accumulate && s0 >= s1) continue;
+    typename TL::OpA a;
+    typename TL::OpB b;
+    a.init(p.a_stride, m0, p.m);
+    b.init(p.b_stride, n0, DW ? (nn + 16 / es - 1) / (16 / es) * (16 / es) : nn);
+    const typename TL::Source sa{p.a + m0 * es, kStep<T> * p.a_stride};
+    const typename TL::Source sb{p.b + n0 * (DW ? (int64_t)es : p.b_stride),
+                                 DW ? kStep<T> * p.b_stride : mma::kStepBytes};
+    f32x4 acc[MT][NT];
+    TL::clear(acc);
+    __syncthreads();  // the tile before is done with LDS
+    TL::product(a, b, sa, sb, s0, s1, k, p.zeros, acc);
+    if (p.seg) {
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          f32x4* at = reinterpret_cast<f32x4*>(part + (TL::wave_n() + 16 * j + col) * TL::BM +
+                                               TL::wave_m() + 16 * i + 4 * g);
+          *at = p.accumulate ? *at + acc[i][j] : acc[i][j];
+        }
+    } else {
+      const float inv = p.scale ? 1.f / *p.scale : 1.f;
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        const int64_t n = n0 + TL::wave_n() + 16 * j + col;
+        if (n >= nn) continue;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int64_t m = m0 + TL::wave_m() + 16 * i + 4 * g;
+          store4(static_cast<T*>(p.out) + n * p.out_stride + m, acc[i][j] * inv, p.out_stride - m,
+                 p.out_vec);
+        }
+      }
+    }
+  }
+}
+
+struct FinishParams {
+  const float* seg;
+  const int* count;
+  const int* row;     // dh: token -> row or -1; dw: null (row = index)
+  int64_t out_rows;   // tokens, or words
+  int64_t n;          // dw: words
+  int64_t k_map;      // dh: words of a whole piece
+  int64_t m, hidden_size;
+  int bm, bn, step, grad_blocks;
+  void* out;
+  int out_vec;
+  const float* scale;
+};
+
+// out = the sum of each tile's partial tiles in order, in the output's type.
+template <typename T, bool DW>
+__global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
+  const int count = *p.count;
+  const int64_t nn = DW ? p.n : count;
+  const int k = DW ? count : (int)p.k_map;
+  const int mts = (int)((p.m + p.bm - 1) / p.bm), nts = (int)((nn + p.bn - 1) / p.bn);
+  const int ks = (k + p.step - 1) / p.step;
+  const mma::Spread spread{(int64_t)mts * nts * ks, p.grad_blocks};
+  const float inv = p.scale ? 1.f / *p.scale : 1.f;
+  const int64_t quads = (p.hidden_size + 3) / 4;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.out_rows * quads;
+       i += (int64_t)gridDim.x * 256) {
+    const int64_t o = i / quads, m = i % quads * 4;
+    const int64_t n = DW ? o : p.row[o];
+    f32x4 sum{0.f, 0.f, 0.f, 0.f};
+    if (n >= 0 && ks > 0) {
+      constexpr int kGroup = 8;
+      const int nt = (int)(n / p.bn), mt = (int)(m / p.bm), first = nt / kGroup * kGroup;
+      const int width = nts - first < kGroup ? nts - first : kGroup;
+      const int64_t tile = (int64_t)first * mts + mt * width + (nt - first);
+      const int b0 = spread.owner(tile * ks), b1 = spread.owner((tile + 1) * ks - 1);
+      for (int b = b0; b <= b1; ++b) {
+        if (spread.begin(b) >= spread.begin(b + 1)) continue;
+        sum += *reinterpret_cast<const f32x4*>(p.seg + (b + tile) * p.bm * p.bn +
+                                               (n % p.bn) * p.bm + m % p.bm);
+      }
+    }
+    store4(static_cast<T*>(p.out) + o * p.hidden_size + m, sum * inv, p.hidden_size - m, p.out_vec);
+  }
+}
+
+// ------------------------------------------------------------------ launches
+
+// The tiles that are built: vocabulary (or hidden) x tokens (or vocabulary).
+enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTiles = 4 };
+struct TileShape {
+  int bm, bn, per_cu;  // per_cu: blocks of it whose LDS fits one of the 256 CUs
+};
+constexpr TileShape kShape[kTiles] = {{256, 256, 1}, {128, 128, 2}, {128, 64, 3}, {128, 32, 3}};
+
+// Implemented per element type by ACE_DEFINE_VOCAB in the ace_k_vocab_*.hip
+// units.
+template <typename T>
+struct Launch {
+  static hipError_t prep(const PrepParams&, int blocks, hipStream_t);
+  static hipError_t pad(const void* src, void* dst, int64_t rows, int size, int width, hipStream_t);
+  static hipError_t score(int tile, const ScoreParams&, int blocks, hipStream_t);
+  static hipError_t upstream(const UpstreamParams&, int blocks, hipStream_t);
+  static hipError_t dscore(int tile, const ScoreParams&, int blocks, hipStream_t);
+  static hipError_t grad(int tile, bool dw, const GradParams&, int blocks, hipStream_t);
+  static hipError_t finish(bool dw, const FinishParams&, int blocks, hipStream_t);
+};
+
+template <typename P>
+inline hipError_t launch(void (*kern)(P), int blocks, int threads, size_t lds, hipStream_t s,
+                         const P& p) {
+  if (lds > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
+                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+    if (e != hipSuccess) return e;
+  }
+  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)threads), lds, s, p);
+  return hipGetLastError();
+}
+
+template <typename T, bool AKC, bool BKC, typename F>
+inline hipError_t with_tile(int tile, F f) {
+  switch (tile) {
+    case kTile256: return f(mma::Tile<T, 256, 256, 2, 4, AKC, BKC>{});
+    case kTile128: return f(mma::Tile<T, 128, 128, 2, 2, AKC, BKC>{});
+    case kTile64: return f(mma::Tile<T, 128, 64, 4, 1, AKC, BKC>{});
+    default: return f(mma::Tile<T, 128, 32, 4, 1, AKC, BKC>{});
+  }
+}
+
+#define ACE_DEFINE_VOCAB(T)                                                                      \
+  template <>                                                                                    \
+  hipError_t Launch<T>::prep(const PrepParams& p, int blocks, hipStream_t s) {                   \
+    return launch(prep_kernel<T>, blocks, 256, 0, s, p);                                         \
+  }                                                                                              \
+  template <>                                                                                    \
+  hipError_t Launch<T>::pad(const void* src, void* dst, int64_t rows, int size, int width,       \
+                            hipStream_t s) {                                                     \
+    const int blocks = (int)(rows < 4096 ? rows : 4096);                                         \
+    hipLaunchKernelGGL(pad_kernel<T>, dim3(blocks), dim3(256), 0, s, static_cast<const T*>(src), \
+                       static_cast<T*>(dst), rows, size, width);                                 \
+    return hipGetLastError();                                                                    \
+  }                                                                                              \
+  template <>                                                                                    \
+  hipError_t Launch<T>::score(int tile, const ScoreParams& p, int blocks, hipStream_t s) {       \
+    return with_tile<T, true, true>(tile, [&](auto t) {                                          \
+      using TL = decltype(t);                                                                    \
+      return launch(score_kernel<TL>, blocks, TL::kThreads, TL::kLdsBytes, s, p);                \
+    });                                                                                          \
+  }                                                                                              \
+  template <>                                                                                    \
+  hipError_t Launch<T>::upstream(const UpstreamParams& p, int blocks, hipStream_t s) {           \
+    return launch(upstream_kernel<T>, blocks, 256, 0, s, p);                                     \
+  }                                                                                              \
+  template <>                                                                                    \
+  hipError_t Launch<T>::dscore(int tile, const ScoreParams& p, int blocks, hipStream_t s) {      \
+    return with_tile<T, true, true>(tile, [&](auto t) {                                          \
+      using TL = decltype(t);                                                                    \
+      return launch(dscore_kernel<TL>, blocks, TL::kThreads, TL::kLdsBytes, s, p);               \
+    });                                                                                          \
+  }                                                                                              \
+  template <>                                                                                    \
+  hipError_t Launch<T>::grad(int tile, bool dw, const GradParams& p, int blocks,                 \
+                             hipStream_t s) {                                                    \
+    if (dw) {                                                                                    \
+      if (tile == kTile256) {                                                                    \
+        using TL = mma::Tile<T, 256, 256, 2, 4, false, false>;                                   \
+        return launch(grad_kernel<TL, true>, blocks, TL::kThreads, TL::kLdsBytes, s, p);         \
+      }                                                                                          \
+      using TL = mma::Tile<T, 128, 128, 2, 2, false, false>;                                     \
+      return launch(grad_kernel<TL, true>, blocks, TL::kThreads, TL::kLdsBytes, s, p);           \
+    }                                                                                            \
+    return with_tile<T, false, true>(tile, [&](auto t) {                                         \
+      using TL = decltype(t);                                                                    \
+      return launch(grad_kernel<TL, false>, blocks, TL::kThreads, TL::kLdsBytes, s, p);          \
+    });                                                                                          \
+  }                                                                                              \
+  template <>                                                                                    \
+  hipError_t Launch<T>::finish(bool dw, const FinishParams& p, int blocks, hipStream_t s) {      \
+    return dw ? launch(finish_kernel<T, true>, blocks, 256, 0, s, p)                             \
+              : launch(finish_kernel<T, false>, blocks, 256, 0, s, p);                           \
+  }
+
+}  // namespace vocab
+}  // namespace ace

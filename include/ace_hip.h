@@ -249,6 +249,55 @@ int ace_forward_noalloc(const void* x, int x_dtype, const void* target,
                         float* loss, double* stats, void* stream);
 
 /*
+ * Softmax cross entropy of hidden states against a vocabulary, and each
+ * token's top-label confidence.  No counterpart in the reference, whose losses
+ * take given logits of at most 64 channels (src/ace_kernels/registry.py:78-100).
+ * The logits s = hidden . weight^T are formed in pieces and never kept.
+ *
+ *   nll_t  = log(sum_v exp s_tv) - s_t,label      conf_t = max_v softmax(s_t)_v
+ *   correct_t = 1 where the label is the lowest index of the largest logit
+ *
+ * hidden [tokens, hidden_size] and weight [vocab, hidden_size] are contiguous,
+ * of one type (ACE_F32, ACE_BF16, ACE_F16), and start at multiples of 16 bytes;
+ * labels [tokens] are int64.  A token whose label is `ignore_index` or outside
+ * [0, vocab) is not counted: its nll, conf and correct are 0, its gradients are
+ * 0, and its hidden state is not looked at.
+ *
+ * ace_vocab_forward: loss[0] = mean over the counted tokens (0 if there are
+ * none) or sum, or loss[tokens] for ACE_RED_NONE.  `confidence` and `correct`
+ * ([tokens] float32) may be NULL.  `saved` (ace_vocab_saved_bytes, 16-byte
+ * aligned) is what the backward needs beside hidden and weight.
+ * ace_vocab_backward: the gradients of hidden and weight, each skipped if NULL,
+ * for upstream gradients of loss (one float32, or [tokens] for ACE_RED_NONE)
+ * and of confidence ([tokens]); either may be NULL, for 0.  It may be called
+ * any number of times on one `saved`.
+ *
+ * The workspace (ace_vocab_workspace_bytes, backward 0 or 1, 16-byte aligned)
+ * needs no clearing and holds nothing between calls; calls that overlap need
+ * one each.  Both calls are asynchronous on `stream`, allocate nothing and can
+ * be captured in a HIP graph.  Results do not vary from run to run: no sum
+ * depends on the order in which blocks finish.  Returns ACE_EINVAL for bad
+ * arguments (misaligned pointers among them), ACE_EUNSUPPORTED for tokens or
+ * vocab above 2^30 or hidden_size above 2^20, ACE_EWORKSPACE, or a HIP error.
+ */
+size_t ace_vocab_saved_bytes(int64_t tokens);
+size_t ace_vocab_workspace_bytes(int dtype, int64_t tokens,
+                                 int64_t hidden_size, int64_t vocab,
+                                 int backward);
+int ace_vocab_forward(const void* hidden, const void* weight, int dtype,
+                      const int64_t* labels, int64_t tokens,
+                      int64_t hidden_size, int64_t vocab, int64_t ignore_index,
+                      int reduction, void* saved, float* loss,
+                      float* confidence, float* correct, void* workspace,
+                      size_t workspace_bytes, void* stream);
+int ace_vocab_backward(const void* hidden, const void* weight, int dtype,
+                       int64_t tokens, int64_t hidden_size, int64_t vocab,
+                       int reduction, const void* saved,
+                       const float* grad_loss, const float* grad_confidence,
+                       void* d_hidden, void* d_weight, void* workspace,
+                       size_t workspace_bytes, void* stream);
+
+/*
  * Kernel timing.  This has no counterpart in the reference, whose benchmark
  * brackets each call with events recorded on the stream
  * (src/ace_bench/timing.py:48-77); on HIP such events also time the dispatch

@@ -1,0 +1,329 @@
+"""vocab_loss and vocab_loss_confidence on the GPU against their definition in
+float64, with derived bounds (vocab_reference.py)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from ace_kernels import VocabConfig, vocab_loss, vocab_loss_confidence
+from gpu_helpers import say
+from vocab_reference import U, exact, inputs
+
+pytestmark = pytest.mark.gpu
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+def _within(got, want, tol, what):
+    err = (got.double() - want).abs()
+    bad = ~(err <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {float((err / tol)[bad].max()):.3g} x bound"
+
+
+def _step(hidden, weight, labels, config, go=None, gc=None):
+    """(scores, gradients) of one calibrated step."""
+    h = hidden.detach().clone().requires_grad_(True)
+    w = weight.detach().clone().requires_grad_(True)
+    out = vocab_loss_confidence(h, w, labels, config)
+    go = torch.ones_like(out.loss) if go is None else go
+    gc = torch.zeros_like(out.confidence) if gc is None else gc
+    return out, torch.autograd.grad((out.loss, out.confidence), (h, w), (go, gc))
+
+
+def _compare(hidden, weight, labels, config=VocabConfig(), go=None, gc=None):
+    want = exact(hidden, weight, labels, config.ignore_index, config.reduction, go, gc)
+    out, (dh, dw) = _step(hidden, weight, labels, config, go, gc)
+    assert dh.dtype == hidden.dtype and dw.dtype == weight.dtype and out.loss.dtype == F32
+    if config.reduction == "none":
+        tol = want.tol_nll + 2 * U * want.loss.abs()
+    else:
+        tol = (want.tol_nll + 2 * U * float(want.nll.abs().max() if want.nll.numel() else 0)) * (
+            1 if config.reduction == "mean" else max(1, labels.numel()))
+    _within(out.loss, want.loss, tol, "loss")
+    _within(out.confidence, want.confidence, want.tol_confidence * want.confidence + 1e-30, "confidence")
+    assert torch.equal(out.correct[want.sure].double(), want.correct[want.sure])
+    if want.sure.all() or gc is None:
+        _within(dh, want.d_hidden, want.tol_hidden + 1e-30, "d hidden")
+        _within(dw, want.d_weight, want.tol_weight + 1e-30, "d weight")
+    return out, (dh, dw)
+
+
+# every tile and its borders; hidden sizes below, at and between a step of k,
+# and those whose rows are no whole 16 bytes; vocabularies of one word and up
+SIZES = [
+    (1, 8, 1), (1, 64, 2), (3, 1, 5), (2, 7, 300), (17, 72, 129), (31, 128, 1000), (32, 100, 257), (33, 64, 128),
+    (64, 200, 640), (65, 33, 1001), (128, 96, 384), (129, 512, 255), (255, 264, 2049), (300, 1000, 513),
+    (520, 64, 70), (1030, 40, 33), (700, 136, 5003),
+]
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n,size,v", SIZES)
+def test_sizes(n, size, v, dtype) -> None:
+    say(f"vocab {n}x{size}x{v} {dtype}")
+    hidden, weight, labels = inputs(n, size, v, dtype, seed=n + v, ignored=0.2)
+    gen = torch.Generator().manual_seed(5)
+    go = torch.tensor(0.7, device="cuda")
+    gc = (torch.randn(n, generator=gen) / n).cuda()
+    _compare(hidden, weight, labels, VocabConfig(), go, gc)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_reductions(reduction, dtype) -> None:
+    n = 150
+    hidden, weight, labels = inputs(n, 128, 777, dtype, seed=3, ignored=0.3)
+    gen = torch.Generator().manual_seed(6)
+    go = torch.randn(n if reduction == "none" else (), generator=gen).cuda()
+    _compare(hidden, weight, labels, VocabConfig(reduction=reduction), go, torch.randn(n, generator=gen).cuda())
+
+
+@pytest.mark.parametrize("n,size,v", [(2100, 128, 8200), (6000, 64, 30000), (9000, 72, 1024)])
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+def test_large_tiles_and_pieces(n, size, v, dtype) -> None:
+    """The 256-wide tiles; 6000 x 30000 takes two pieces of the vocabulary;
+    9000 tokens of a small head share out the tokens of the weight's gradient."""
+    hidden, weight, labels = inputs(n, size, v, dtype, seed=8, ignored=0.4)
+    _compare(hidden, weight, labels, VocabConfig(), torch.tensor(1.0, device="cuda"))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_nothing_counted(dtype) -> None:
+    hidden, weight, _ = inputs(40, 64, 100, dtype)
+    for labels in (torch.full((40,), -100), torch.full((40,), 100), torch.full((40,), -1)):
+        out, (dh, dw) = _step(hidden, weight, labels.cuda(), VocabConfig())
+        assert out.loss.item() == 0 and not out.confidence.any() and not out.correct.any()
+        assert not dh.any() and not dw.any()
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_no_tokens(reduction) -> None:
+    _, weight, _ = inputs(1, 64, 100, BF16)
+    hidden = torch.empty(0, 64, dtype=BF16, device="cuda")
+    out, (dh, dw) = _step(hidden, weight, torch.empty(0, dtype=torch.int64, device="cuda"), VocabConfig(reduction=reduction))
+    assert out.loss.shape == ((0,) if reduction == "none" else ()) and not out.loss.any()
+    assert dh.shape == (0, 64) and not dw.any()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_ignored_tokens_are_not_read(dtype) -> None:
+    """NaN and infinities in the hidden states of ignored tokens reach nothing,
+    and the results are those of the counted tokens alone, bit for bit."""
+    hidden, weight, labels = inputs(200, 96, 500, dtype, seed=4, ignored=0.5)
+    gone = labels == -100
+    hidden[gone] = float("nan")
+    hidden[gone.nonzero()[0]] = float("inf")
+    out, (dh, dw) = _compare(hidden.masked_fill(gone[:, None], 0), weight, labels)
+    out2, (dh2, dw2) = _step(hidden, weight, labels, VocabConfig())
+    for a, b in ((out.loss, out2.loss), (out.confidence, out2.confidence), (dh, dh2), (dw, dw2)):
+        assert torch.equal(a, b)
+    out3, (dh3, dw3) = _step(hidden[~gone], weight, labels[~gone], VocabConfig())
+    assert torch.equal(out3.loss, out2.loss) and torch.equal(out3.confidence, out2.confidence[~gone])
+
+
+def test_ignore_index_inside_the_vocabulary() -> None:
+    hidden, weight, labels = inputs(90, 64, 50, F32, seed=2)
+    _compare(hidden, weight, labels, VocabConfig(ignore_index=int(labels[0])))
+
+
+def test_ties_go_to_the_lowest_word() -> None:
+    """Equal rows of the weight give equal logits: the lowest index is the top
+    label wherever the two lie (one lane, two lanes, two tiles, two blocks)."""
+    hidden, weight, _ = inputs(40, 64, 3000, F32, seed=9)
+    for low, high in ((5, 6), (5, 9), (5, 21), (5, 100), (5, 300), (100, 2999)):
+        w = weight.clone()
+        w[high] = w[low] = 20 * hidden[0] / hidden[0].norm()
+        labels = torch.full((40,), low, device="cuda")
+        top = (hidden.double() @ w.double().t()).argmax(1)
+        assert vocab_loss_confidence(hidden, w, labels).correct[0] == 1
+        labels.fill_(high)
+        assert vocab_loss_confidence(hidden, w, labels).correct[0] == 0
+        assert int(top[0]) in (low, high)
+
+
+def test_nan_and_infinite_logits_stay_in_their_token() -> None:
+    hidden, weight, labels = inputs(70, 64, 300, F32, seed=1)
+    clean = vocab_loss(hidden, weight, labels, VocabConfig(reduction="none"))
+    hidden[3, 5] = float("nan")
+    hidden[40, 7] = float("inf")
+    got = vocab_loss(hidden, weight, labels, VocabConfig(reduction="none"))
+    assert torch.isnan(got[3]) and torch.isnan(got[40])
+    keep = torch.ones(70, dtype=torch.bool, device="cuda")
+    keep[[3, 40]] = False
+    assert torch.equal(got[keep], clean[keep])
+
+
+def test_words_at_minus_infinity() -> None:
+    """A weight of the type's lowest value takes a word's probability to 0."""
+    hidden, weight, labels = inputs(20, 64, 200, F32, seed=1)
+    hidden[:, 0] = 1.0
+    weight[150:, :] = 0.0
+    weight[150:, 0] = torch.finfo(F32).min
+    labels.clamp_(max=149)
+    part = vocab_loss(hidden, weight[:150], labels)
+    assert torch.allclose(vocab_loss(hidden, weight, labels), part, rtol=8 * U, atol=0)
+
+
+def test_confident_tokens_keep_their_digits() -> None:
+    """nll = log(1 + exp(-d)) of two words d apart, down to where it is below
+    float32's step at the size of the logits."""
+    d = torch.tensor([0.0, 1.0, 5.0, 10.0, 14.0], dtype=torch.float64)
+    hidden = torch.zeros(5, 8)
+    hidden[:, 0] = 1.0
+    hidden[:, 1] = -d.float()
+    hidden[:, 2] = 30.0
+    weight = torch.zeros(2, 8)
+    weight[:, 2] = 1.0
+    weight[1, 1] = 1.0
+    labels = torch.zeros(5, dtype=torch.int64)
+    got = vocab_loss(hidden.cuda(), weight.cuda(), labels.cuda(), VocabConfig(reduction="none")).double().cpu()
+    want = torch.log1p(torch.exp(-d))
+    # the sum 1 + exp(-d) rounds at u; logits of 30 - d round at 16 u
+    assert ((got - want).abs() <= 2 * U + 32 * U * torch.exp(-d)).all()
+
+
+def test_gradient_against_differences() -> None:
+    """A central difference of the float64 definition along a direction, at the
+    kernels' own gradient."""
+    hidden, weight, labels = inputs(60, 48, 211, F32, seed=12, ignored=0.2)
+    gc = torch.randn(60, generator=torch.Generator().manual_seed(1)).cuda() / 60
+    _, (dh, dw) = _step(hidden, weight, labels, VocabConfig(), None, gc)
+    gen = torch.Generator().manual_seed(2)
+    vh, vw = torch.randn(60, 48, generator=gen).cuda().double(), torch.randn(211, 48, generator=gen).cuda().double()
+
+    def f(t):
+        h, w = hidden.double() + t * vh, weight.double() + t * vw
+        e = exact(h.double(), w.double(), labels)
+        return float(e.loss + (gc.double() * e.confidence).sum())
+
+    step = 1e-5
+    want = (f(step) - f(-step)) / (2 * step)
+    got = float((dh.double() * vh).sum() + (dw.double() * vw).sum())
+    assert abs(got - want) <= 1e-5 * (1 + abs(want))
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])
+def test_strides_offsets_shapes_and_label_types(dtype) -> None:
+    hidden, weight, labels = inputs(48, 72, 300, dtype, seed=7, ignored=0.2)
+    want, (dh, dw) = _step(hidden, weight, labels, VocabConfig())
+    wide = torch.full((48, 100), float("nan"), dtype=dtype, device="cuda")
+    wide[:, 3:75] = hidden
+    flat = torch.empty(300 * 72 + 3, dtype=dtype, device="cuda")
+    flat[3:] = weight.reshape(-1)
+    for h in (wide[:, 3:75], hidden.t().contiguous().t(), hidden):
+        for w in (flat[3:].view(300, 72), weight.t().contiguous().t()):
+            for y in (labels, labels.int(), labels.repeat_interleave(2)[::2]):
+                out, (a, b) = _step(h, w, y, VocabConfig())
+                assert torch.equal(out.loss, want.loss) and torch.equal(a, dh) and torch.equal(b, dw)
+    out, (a, b) = _step(hidden.view(4, 12, 72), weight, labels.view(4, 12), VocabConfig(reduction="none"))
+    assert out.loss.shape == out.confidence.shape == out.correct.shape == (4, 12) and a.shape == (4, 12, 72)
+    one, (a, b) = _step(hidden[0], weight, labels[0], VocabConfig())
+    assert one.loss.shape == one.confidence.shape == () and a.shape == (72,)
+
+
+def test_float16_gradients_of_rare_words_survive() -> None:
+    """Probabilities far below float16's smallest number, times a loss scale,
+    still reach the weight's gradient."""
+    n, size, v = 256, 64, 20000
+    hidden, weight, labels = inputs(n, size, v, F16, seed=5)
+    hidden = hidden + 12 * weight[labels]
+    _compare(hidden, weight, labels, VocabConfig(), torch.tensor(65536.0, device="cuda"))
+
+
+def test_one_gradient_alone_and_the_same_bits_again() -> None:
+    hidden, weight, labels = inputs(200, 128, 3000, BF16, seed=6, ignored=0.1)
+    _, (dh, dw) = _step(hidden, weight, labels, VocabConfig())
+    h = hidden.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(vocab_loss(h, weight, labels), h)[0], dh)
+    w = weight.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(vocab_loss(hidden, w, labels), w)[0], dw)
+    h2, w2 = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+    loss = vocab_loss(h2, w2, labels)
+    for _ in range(3):  # one graph, several backward passes
+        a, b = torch.autograd.grad(loss, (h2, w2), retain_graph=True)
+        assert torch.equal(a, dh) and torch.equal(b, dw)
+
+
+def test_frozen_head_and_no_grad() -> None:
+    hidden, weight, labels = inputs(30, 64, 100, BF16)
+    assert not vocab_loss(hidden, weight, labels).requires_grad
+    h = hidden.clone().requires_grad_(True)
+    with torch.no_grad():
+        assert not vocab_loss(h, weight, labels).requires_grad
+    out = vocab_loss_confidence(h, weight, labels)
+    assert out.confidence.requires_grad and not out.correct.requires_grad
+    (only,) = torch.autograd.grad(out.confidence.sum(), h)
+    want = exact(hidden, weight, labels, grad_loss=torch.zeros((), device="cuda"), grad_confidence=torch.ones(30, device="cuda"))
+    assert want.sure.all()
+    _within(only, want.d_hidden, want.tol_hidden + 1e-30, "d hidden")
+
+
+def test_second_derivative_is_refused() -> None:
+    hidden, weight, labels = inputs(10, 64, 50, F32)
+    h = hidden.clone().requires_grad_(True)
+    (g,) = torch.autograd.grad(vocab_loss(h, weight, labels), h, create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g.sum(), h)
+
+
+def test_changed_input_is_refused_in_backward() -> None:
+    hidden, weight, labels = inputs(10, 64, 50, F32)
+    w = weight.clone().requires_grad_(True)
+    loss = vocab_loss(hidden, w, labels)
+    with torch.no_grad():
+        w += 1
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
+def test_streams() -> None:
+    """Calls on two streams at once do not share anything."""
+    a = inputs(300, 128, 4000, BF16, seed=21)
+    b = inputs(280, 128, 5000, BF16, seed=22)
+    want = [_step(*x, VocabConfig()) for x in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(3):
+        for i, x in enumerate((a, b)):
+            with torch.cuda.stream(streams[i]):
+                got[i] = _step(*x, VocabConfig())
+    torch.cuda.synchronize()
+    for (o, g), (o2, g2) in zip(want, got):
+        assert torch.equal(o.loss, o2.loss) and torch.equal(g[0], g2[0]) and torch.equal(g[1], g2[1])
+
+
+def test_captured_step_replays() -> None:
+    """A captured step with its gradients: new inputs each replay, eager work in
+    between, every replay compared with the eager result."""
+    hidden, weight, labels = inputs(200, 128, 3000, BF16, seed=1, ignored=0.1)
+    h, w, y = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True), labels.clone()
+
+    def step():
+        out = vocab_loss_confidence(h, w, y)
+        return [out.loss, out.confidence, *torch.autograd.grad((out.loss, out.confidence), (h, w),
+                                                               (torch.ones_like(out.loss), out.confidence.detach()))]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        new = inputs(200, 128, 3000, BF16, seed=30 + i, ignored=0.3 * (i % 2))
+        with torch.no_grad():
+            h.copy_(new[0])
+            w.copy_(new[1])
+            y.copy_(new[2])
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        want = step()
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert torch.equal(a, b), f"replay {i}"
