@@ -47,6 +47,10 @@ EXPORTS = (
     "ace_vocab_workspace_bytes",
     "ace_vocab_forward",
     "ace_vocab_backward",
+    "ace_balance_workspace_bytes",
+    "ace_balance_ticket_bytes",
+    "ace_balance_forward",
+    "ace_balance_backward",
 )
 
 # ace_forward_noalloc's scratch (ACE_NOALLOC_SCRATCH_BYTES) and its error code
@@ -184,6 +188,23 @@ def lib() -> ctypes.CDLL:
         _i, _p, _p, _p,            # reduction, saved, grad_loss, grad_confidence
         _p, _p,                    # d_hidden, d_weight
         _p, _sz, _p,               # workspace, bytes, stream
+    ]
+    handle.ace_balance_workspace_bytes.restype = _sz
+    handle.ace_balance_workspace_bytes.argtypes = [_i64, _i64, _i64]
+    handle.ace_balance_ticket_bytes.restype = _sz
+    handle.ace_balance_ticket_bytes.argtypes = [_i64]
+    handle.ace_balance_forward.restype = _i
+    handle.ace_balance_forward.argtypes = [
+        _p, _i, _p,                # logits, dtype, mask
+        _i64, _i64, _i64,          # groups, tokens, experts
+        _i, _i, _p, _p, _p,        # top_k, reduction, loss, counts, share
+        _p, _sz, _p, _sz, _p,      # tickets, bytes, workspace, bytes, stream
+    ]
+    handle.ace_balance_backward.restype = _i
+    handle.ace_balance_backward.argtypes = [
+        _p, _i, _p,                # logits, dtype, mask
+        _i64, _i64, _i64,          # groups, tokens, experts
+        _i, _p, _p, _p, _p,        # reduction, share, grad_loss, d_logits, stream
     ]
     handle.ace_set_launch_events.restype = _i
     handle.ace_set_launch_events.argtypes = [_p, _p]

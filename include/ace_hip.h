@@ -298,6 +298,42 @@ int ace_vocab_backward(const void* hidden, const void* weight, int dtype,
                        size_t workspace_bytes, void* stream);
 
 /*
+ * The balance loss of an expert router, and how many tokens take each expert.
+ * No counterpart in the reference.  logits [groups, tokens, experts] (ACE_F32,
+ * ACE_BF16 or ACE_F16, contiguous): each group (a layer's router, or a sequence)
+ * has a loss of its own over its M counted tokens, those whose byte of `mask`
+ * ([groups, tokens], NULL: all) is not 0.  A token takes its top_k largest
+ * logits, the lowest expert first where they are equal (NaN is above all).
+ *
+ *   loss_g = sum_e (E n_ge / (top_k M)) (1 / M) sum_t softmax(logits_gt)_e
+ *
+ * and 0 for a group without counted tokens, whose gradient is 0 as well.
+ * ace_balance_forward: loss[0] = mean or sum over the groups, or loss[groups] for
+ * ACE_RED_NONE; counts [groups, experts] = n; share [groups, experts], which the
+ * backward takes.  `tickets` (ace_balance_ticket_bytes) is zero when a call starts
+ * and left zero; calls that overlap need one each, and a workspace
+ * (ace_balance_workspace_bytes, 16-byte aligned) each.
+ * ace_balance_backward: the gradient of logits for an upstream gradient of loss
+ * (one float32, or [groups]); n counts as a constant.  Masked tokens get 0 and
+ * their logits are not read.  Both calls are one launch on `stream`, allocate
+ * nothing and can be captured; results do not vary from run to run.  Returns
+ * ACE_EINVAL, ACE_EUNSUPPORTED (experts above 512, top_k above 16, groups above
+ * 2^20), ACE_EWORKSPACE or a HIP error.
+ */
+size_t ace_balance_workspace_bytes(int64_t groups, int64_t tokens,
+                                   int64_t experts);
+size_t ace_balance_ticket_bytes(int64_t groups);
+int ace_balance_forward(const void* logits, int dtype, const uint8_t* mask,
+                        int64_t groups, int64_t tokens, int64_t experts,
+                        int top_k, int reduction, float* loss, int64_t* counts,
+                        float* share, void* tickets, size_t ticket_bytes,
+                        void* workspace, size_t workspace_bytes, void* stream);
+int ace_balance_backward(const void* logits, int dtype, const uint8_t* mask,
+                         int64_t groups, int64_t tokens, int64_t experts,
+                         int reduction, const float* share,
+                         const float* grad_loss, void* d_logits, void* stream);
+
+/*
  * Kernel timing.  This has no counterpart in the reference, whose benchmark
  * brackets each call with events recorded on the stream
  * (src/ace_bench/timing.py:48-77); on HIP such events also time the dispatch
