@@ -192,7 +192,7 @@ def lib() -> ctypes.CDLL:
     handle.ace_balance_workspace_bytes.restype = _sz
     handle.ace_balance_workspace_bytes.argtypes = [_i64, _i64, _i64]
     handle.ace_balance_ticket_bytes.restype = _sz
-    handle.ace_balance_ticket_bytes.argtypes = [_i64]
+    handle.ace_balance_ticket_bytes.argtypes = [_i64, _i64, _i64]
     handle.ace_balance_forward.restype = _i
     handle.ace_balance_forward.argtypes = [
         _p, _i, _p,                # logits, dtype, mask

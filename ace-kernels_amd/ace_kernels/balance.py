@@ -107,7 +107,7 @@ class _BalanceLoss(torch.autograd.Function):
         share = torch.empty((groups, experts), dtype=torch.float32, device=dev)
         with torch.cuda.device(dev):
             stream = _stream(dev)
-            need = lib.ace_balance_ticket_bytes(groups)
+            need = lib.ace_balance_ticket_bytes(groups, tokens, experts)
             tickets = _tickets(dev, stream, need)
             ws = torch.empty(lib.ace_balance_workspace_bytes(groups, tokens, experts), dtype=torch.uint8, device=dev)
             rc = lib.ace_balance_forward(

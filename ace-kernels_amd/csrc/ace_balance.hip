@@ -37,15 +37,16 @@ Geometry geometry(int64_t groups, int64_t tokens, int experts) {
 }
 
 struct Space {
-  size_t sum, count, loss, bytes;
+  size_t loss, bytes, ticket_bytes;
 };
 Space space(int64_t groups, int experts, const Geometry& g) {
   const auto round = [](size_t b) { return (b + 255) / 256 * 256; };
-  const size_t slots = (size_t)groups * (size_t)(g.blocks + kFan);
+  const size_t fans = (size_t)(g.blocks + kFan - 1) / kFan;
+  const size_t sets = (size_t)(groups + kFan - 1) / kFan;
   Space s{};
-  s.count = round(slots * (size_t)experts * 4);
-  s.loss = s.count + round(slots * (size_t)(experts + 1) * 4);
-  s.bytes = s.loss + round((size_t)groups * 8);
+  s.loss = round((size_t)groups * (g.blocks + fans) * (size_t)(experts + 1) * 8);
+  s.bytes = s.loss + round(((size_t)groups + sets) * 8);
+  s.ticket_bytes = ((size_t)groups * (fans + 1) + sets + 1) * kTicketStride * 4;
   return s;
 }
 
@@ -129,8 +130,9 @@ size_t ace_balance_workspace_bytes(int64_t groups, int64_t tokens, int64_t exper
   return space(groups, (int)experts, geometry(groups, tokens, (int)experts)).bytes;
 }
 
-size_t ace_balance_ticket_bytes(int64_t groups) {
-  return groups < 1 || groups > kMaxGroups ? 0 : (size_t)(groups * (kFan + 1) + 1) * 4;
+size_t ace_balance_ticket_bytes(int64_t groups, int64_t tokens, int64_t experts) {
+  if (!ace_balance_workspace_bytes(groups, tokens, experts)) return 0;
+  return space(groups, (int)experts, geometry(groups, tokens, (int)experts)).ticket_bytes;
 }
 
 int ace_balance_forward(const void* logits, int dtype, const uint8_t* mask, int64_t groups,
@@ -146,13 +148,11 @@ int ace_balance_forward(const void* logits, int dtype, const uint8_t* mask, int6
     return ACE_EINVAL;
   const Geometry g = geometry(groups, tokens, (int)experts);
   const Space at = space(groups, (int)experts, g);
-  if (workspace_bytes < at.bytes || ticket_bytes < ace_balance_ticket_bytes(groups))
-    return ACE_EWORKSPACE;
+  if (workspace_bytes < at.bytes || ticket_bytes < at.ticket_bytes) return ACE_EWORKSPACE;
   Params p = params(logits, mask, groups, tokens, experts, reduction, g);
   char* ws = static_cast<char*>(workspace);
   p.top_k = top_k;
-  p.part_sum = reinterpret_cast<float*>(ws);
-  p.part_count = reinterpret_cast<int*>(ws + at.count);
+  p.part = reinterpret_cast<unsigned long long*>(ws);
   p.part_loss = reinterpret_cast<double*>(ws + at.loss);
   p.tickets = static_cast<int*>(tickets);
   p.loss = loss;

@@ -30,12 +30,14 @@
 
 #include <type_traits>
 
+#include "ace_core.hpp"  // device-coherent accesses
+
 namespace ace {
 namespace balance {
 
-constexpr int kThreads = 256;
 constexpr int kFan = 32;             // partial sums that one block adds
 constexpr int kMaxBlocks = kFan * kFan;  // blocks of a group
+constexpr int kTicketStride = 64;    // words: a counter has a 256-byte line of its own
 constexpr int kMaxExperts = 512;
 constexpr int kMaxTopK = 16;
 
@@ -49,10 +51,10 @@ struct Params {
   int64_t per_block;      // tokens of a block
   int reduction;          // 0 mean, 1 sum, 2 none
   // forward
-  float* part_sum;        // [groups][blocks + kFan][experts]
-  int* part_count;        // [groups][blocks + kFan][experts + 1]: counts, then tokens
-  int* tickets;           // zero, left zero: [groups][kFan + 1], then 1
-  double* part_loss;      // [groups]
+  unsigned long long* part;  // [groups][blocks + fans][experts + 1]: count << 32 | the sum of
+                             // p; the last entry's count is the counted tokens
+  double* part_loss;      // [groups + ceil(groups / kFan)]
+  int* tickets;           // zero, left zero: [groups][fans + 1], [ceil(groups / kFan)], [1]
   float* loss;            // one value, or [groups]
   int64_t* counts;        // [groups, experts]
   float* share;           // [groups, experts]: q
@@ -285,22 +287,29 @@ __device__ inline float exponentials(const Row<T, C>& row, const T (&x)[C], int 
   return 1.f / over_lanes(sum, lanes, kAdd);
 }
 
-// The last of `n` blocks to come here, which then sees what the others wrote
-// before they came.  All threads of the block call it.
-__device__ inline bool last_of(int* ticket, int n) {
+// Whether this is the last of `n` blocks to come here; it then sees what the
+// others wrote (device-coherently) before they came, and leaves the counter zero.
+// All threads of the block call it.
+__device__ inline bool last_of(int* counter, int n) {
   __shared__ int s_last;
-  __threadfence();
+  wait_own_writes();
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int came = __hip_atomic_fetch_add(ticket, 1, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    s_last = came == n - 1;
-    if (s_last) __hip_atomic_store(ticket, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    s_last = ticket(counter) == n - 1;
+    if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
   }
   __syncthreads();
   const bool last = s_last;
   __syncthreads();
-  if (last) __threadfence();
   return last;
+}
+
+__device__ inline void store_dev(double* p, double v) {
+  ace::store_dev(reinterpret_cast<long long*>(p), __double_as_longlong(v));
+}
+__device__ inline double load_dev(const double* p) {
+  return __longlong_as_double(
+      (long long)ace::load_dev(reinterpret_cast<const unsigned long long*>(p)));
 }
 
 template <typename T, int C, int K>
@@ -367,39 +376,45 @@ __global__ __launch_bounds__(kThreads, C == 32 ? 3 : 4) void forward_kernel(Para
     __syncthreads();
   }
   // across the group's blocks: kFan of them, then those sums
-  float* part_sum = p.part_sum + (int64_t)group * (p.blocks + kFan) * E;
-  int* part_count = p.part_count + (int64_t)group * (p.blocks + kFan) * (E + 1);
-  int* tickets = p.tickets + group * (kFan + 1);
+  const int fans = (p.blocks + kFan - 1) / kFan;
+  unsigned long long* part = p.part + (int64_t)group * (p.blocks + fans) * (E + 1);
+  int* tickets = p.tickets + (int64_t)group * (fans + 1) * kTicketStride;
   const auto put = [&](int at) {
-    for (int e = tid; e <= E; e += kThreads) {
-      if (e < E) part_sum[(int64_t)at * E + e] = s_sum[e];
-      part_count[(int64_t)at * (E + 1) + e] = s_count[e];
-    }
+    for (int e = tid; e <= E; e += kThreads)
+      ace::store_dev(part + (int64_t)at * (E + 1) + e,
+                     (unsigned long long)(unsigned)s_count[e] << 32 |
+                         (e < E ? __float_as_uint(s_sum[e]) : 0u));
   };
   const auto add = [&](int first, int n) {
     for (int e = tid; e <= E; e += kThreads) {
+      const unsigned long long* at = part + (int64_t)first * (E + 1) + e;
       float s = 0.f;
       int c = 0;
-#pragma unroll 8
-      for (int i = 0; i < n; ++i) {
-        if (e < E) s += part_sum[(int64_t)(first + i) * E + e];
-        c += part_count[(int64_t)(first + i) * (E + 1) + e];
+      for (int i0 = 0; i0 < n; i0 += 8) {
+        unsigned long long w[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          w[i] = i0 + i < n ? ace::load_dev(at + (int64_t)(i0 + i) * (E + 1)) : 0ull;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          s += __uint_as_float((unsigned)w[i]);
+          c += (int)(w[i] >> 32);
+        }
       }
       if (e < E) s_sum[e] = s;
       s_count[e] = c;
     }
     __syncthreads();
   };
-  const int fans = (p.blocks + kFan - 1) / kFan;
   if (p.blocks > 1) {
     const int fan = block / kFan;
     const int in_fan = p.blocks - fan * kFan < kFan ? p.blocks - fan * kFan : kFan;
     put(block);
-    if (!last_of(&tickets[fan], in_fan)) return;
+    if (!last_of(tickets + fan * kTicketStride, in_fan)) return;
     add(fan * kFan, in_fan);
     if (fans > 1) {
       put(p.blocks + fan);
-      if (!last_of(&tickets[kFan], fans)) return;
+      if (!last_of(tickets + fans * kTicketStride, fans)) return;
       add(p.blocks, fans);
     }
   }
@@ -421,15 +436,26 @@ __global__ __launch_bounds__(kThreads, C == 32 ? 3 : 4) void forward_kernel(Para
     if (tid == 0) p.loss[group] = (float)loss;
     return;
   }
-  if (tid == 0) p.part_loss[group] = loss;
-  if (!last_of(p.tickets + p.groups * (kFan + 1), p.groups)) return;
-  if (wave == 0) {
+  // across the groups: kFan of them, then those sums
+  const int sets = (p.groups + kFan - 1) / kFan, set = group / kFan;
+  const int in_set = p.groups - set * kFan < kFan ? p.groups - set * kFan : kFan;
+  int* loss_tickets = p.tickets + (int64_t)p.groups * (fans + 1) * kTicketStride;
+  const auto sum_of = [&](const double* x, int n) {  // by the first wave
     double all = 0.0;
-    for (int g = lane; g < p.groups; g += 64) all += p.part_loss[g];
+    for (int g = lane; g < n; g += 64) all += load_dev(x + g);
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) all += __shfl_xor(all, d);
-    if (lane == 0) *p.loss = (float)(p.reduction == 0 ? all / p.groups : all);
+    return all;
+  };
+  if (tid == 0) store_dev(p.part_loss + group, loss);
+  if (!last_of(loss_tickets + set * kTicketStride, in_set)) return;
+  double all = wave == 0 ? sum_of(p.part_loss + set * kFan, in_set) : 0.0;
+  if (sets > 1) {
+    if (tid == 0) store_dev(p.part_loss + p.groups + set, all);
+    if (!last_of(loss_tickets + sets * kTicketStride, sets)) return;
+    if (wave == 0) all = sum_of(p.part_loss + p.groups, sets);
   }
+  if (tid == 0) *p.loss = (float)(p.reduction == 0 ? all / p.groups : all);
 }
 
 template <typename T, int C>

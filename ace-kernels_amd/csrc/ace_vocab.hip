@@ -4,6 +4,8 @@
 // or synchronises.
 #include "ace_vocab.hpp"
 
+#include "ace_core.hpp"  // device-coherent accesses
+
 #include "ace_hip.h"
 
 namespace ace {
@@ -86,12 +88,11 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
   if (tid == 0) {
     const double s = s_sum[0] + s_sum[64] + s_sum[128] + s_sum[192];
     __hip_atomic_store(&p.sums[blockIdx.x], s, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    __threadfence();
-    s_last = atomicAdd(p.ticket, 1) == (int)gridDim.x - 1;
+    wait_own_writes();
+    s_last = ticket(p.ticket) == (int)gridDim.x - 1;
   }
   __syncthreads();
   if (!s_last) return;
-  __threadfence();
   double s = 0.0;
   for (int b = tid; b < (int)gridDim.x; b += 256)
     s += __hip_atomic_load(&p.sums[b], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);

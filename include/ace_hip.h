@@ -322,7 +322,8 @@ int ace_vocab_backward(const void* hidden, const void* weight, int dtype,
  */
 size_t ace_balance_workspace_bytes(int64_t groups, int64_t tokens,
                                    int64_t experts);
-size_t ace_balance_ticket_bytes(int64_t groups);
+size_t ace_balance_ticket_bytes(int64_t groups, int64_t tokens,
+                                int64_t experts);
 int ace_balance_forward(const void* logits, int dtype, const uint8_t* mask,
                         int64_t groups, int64_t tokens, int64_t experts,
                         int top_k, int reduction, float* loss, int64_t* counts,

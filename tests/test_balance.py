@@ -89,8 +89,8 @@ def test_limits_and_workspace() -> None:
     assert _forward(experts=513) == _lib.EUNSUPPORTED and _backward(experts=513) == _lib.EUNSUPPORTED
     assert _forward(experts=64, top_k=17) == _lib.EUNSUPPORTED
     assert _forward(groups=(1 << 20) + 1) == _lib.EUNSUPPORTED
-    need, tickets = lib.ace_balance_workspace_bytes(2, 10, 8), lib.ace_balance_ticket_bytes(2)
+    need, tickets = lib.ace_balance_workspace_bytes(2, 10, 8), lib.ace_balance_ticket_bytes(2, 10, 8)
     assert need > 0 and tickets > 0
     assert _forward(nbytes=need - 1) == 3 and _forward(ticket_bytes=tickets - 1) == 3
-    assert lib.ace_balance_workspace_bytes(0, 10, 8) == 0 and lib.ace_balance_ticket_bytes(0) == 0
+    assert lib.ace_balance_workspace_bytes(0, 10, 8) == 0 and lib.ace_balance_ticket_bytes(0, 10, 8) == 0
     assert _backward(tokens=0, logits=None, share=None, grad=None, d=None) == 0  # nothing to do
