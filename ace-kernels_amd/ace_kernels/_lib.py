@@ -245,6 +245,10 @@ def autograd():
     mod.set_entry_points(addr(handle.ace_forward), addr(handle.ace_backward),
                          addr(handle.ace_forward_levels), addr(handle.ace_backward_levels),
                          addr(handle.ace_error_string))
+    mod.set_lm_entry_points(addr(handle.ace_vocab_saved_bytes), addr(handle.ace_vocab_workspace_bytes),
+                            addr(handle.ace_vocab_forward), addr(handle.ace_vocab_backward),
+                            addr(handle.ace_balance_workspace_bytes), addr(handle.ace_balance_forward),
+                            addr(handle.ace_balance_backward))
     return mod
 
 

@@ -15,22 +15,24 @@ they are in the definition.  Equal scores go to the lowest expert.
 Leading dimensions are groups with a loss of their own: ``[layers, tokens, E]`` is
 every layer's router of a step, ``[batch, tokens, E]`` a balance per sequence.  A
 group without counted tokens has loss 0 and gradient 0.
+
+The call and its backward node are C++ (``csrc/ace_autograd.cpp``).
 """
 
 from __future__ import annotations
 
 import math
-from typing import Any, Literal, NamedTuple, Optional, Tuple
+from functools import lru_cache
+from typing import Literal, NamedTuple, Optional
 
 import torch
 from pydantic import BaseModel, ConfigDict, Field
-from torch.autograd.function import once_differentiable
 
 from ace_kernels import _lib
 from ace_kernels.common import capturing, workspace
-from ace_kernels.impls.hip_mi355x import _ptr, _stream
+from ace_kernels.impls.hip_mi355x import _stream
 
-_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _REDUCTIONS = {"mean": _lib.RED_MEAN, "sum": _lib.RED_SUM, "none": _lib.RED_NONE}
 MAX_EXPERTS = 512
 MAX_TOP_K = 16
@@ -80,65 +82,18 @@ def _check(logits: torch.Tensor, config: BalanceConfig, mask: Optional[torch.Ten
             raise ValueError(f"mask is on {mask.device}, logits on {logits.device}")
 
 
-def _tickets(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+@lru_cache(maxsize=256)
+def _ticket_bytes(groups: int, tokens: int, experts: int) -> int:
+    return _lib.lib().ace_balance_ticket_bytes(groups, tokens, experts)
+
+
+def _tickets(device: torch.device, nbytes: int) -> torch.Tensor:
     """Zeroed counters that the call leaves zero: the stream's workspace, or in a
     capture counters of its own, cleared by the graph, so that replays of
     different graphs share none."""
     if capturing(device):
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return workspace(device, stream, nbytes)
-
-
-class _BalanceLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, logits: torch.Tensor, mask: Optional[torch.Tensor],
-                config: BalanceConfig) -> Tuple[torch.Tensor, torch.Tensor]:
-        lib = _lib.lib()
-        dev = logits.device
-        tokens, experts = logits.shape[-2:]
-        lead = logits.shape[:-2]
-        groups = math.prod(lead)
-        x = logits.contiguous()
-        m = None if mask is None else mask.contiguous()
-        reduction = _REDUCTIONS[config.reduction]
-        code = _DTYPES[logits.dtype]
-        loss = torch.empty(lead if reduction == _lib.RED_NONE else (), dtype=torch.float32, device=dev)
-        counts = torch.empty((*lead, experts), dtype=torch.int64, device=dev)
-        share = torch.empty((groups, experts), dtype=torch.float32, device=dev)
-        with torch.cuda.device(dev):
-            stream = _stream(dev)
-            need = lib.ace_balance_ticket_bytes(groups, tokens, experts)
-            tickets = _tickets(dev, stream, need)
-            ws = torch.empty(lib.ace_balance_workspace_bytes(groups, tokens, experts), dtype=torch.uint8, device=dev)
-            rc = lib.ace_balance_forward(
-                x.data_ptr(), code, _ptr(m), groups, tokens, experts, config.top_k, reduction,
-                loss.data_ptr(), counts.data_ptr(), share.data_ptr(), tickets.data_ptr(), tickets.numel(),
-                ws.data_ptr(), ws.numel(), stream)
-        _lib.check(rc, "ace_balance_forward")
-        ctx.save_for_backward(logits, mask, share)
-        ctx.call = (code, groups, tokens, experts, reduction)
-        ctx.mark_non_differentiable(counts)
-        ctx.set_materialize_grads(False)
-        return loss, counts
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, grad_loss: Optional[torch.Tensor], _counts: Optional[torch.Tensor] = None):
-        if grad_loss is None:
-            return None, None, None
-        logits, mask, share = ctx.saved_tensors
-        code, groups, tokens, experts, reduction = ctx.call
-        lib = _lib.lib()
-        dev = logits.device
-        x = logits.contiguous()
-        m = None if mask is None else mask.contiguous()
-        go = grad_loss.to(torch.float32).contiguous()
-        dx = torch.empty(logits.shape, dtype=logits.dtype, device=dev)
-        with torch.cuda.device(dev):
-            rc = lib.ace_balance_backward(x.data_ptr(), code, _ptr(m), groups, tokens, experts, reduction,
-                                          share.data_ptr(), go.data_ptr(), dx.data_ptr(), _stream(dev))
-        _lib.check(rc, "ace_balance_backward")
-        return dx, None, None
+    return workspace(device, _stream(device), nbytes)
 
 
 def balance_loss(logits: torch.Tensor, config: BalanceConfig,
@@ -148,4 +103,9 @@ def balance_loss(logits: torch.Tensor, config: BalanceConfig,
     ``[..., tokens]`` (bool): tokens that count (the others' scores are not
     read).  Differentiable once in ``logits``."""
     _check(logits, config, mask)
-    return BalanceLoss(*_BalanceLoss.apply(logits, mask, config))
+    dev = logits.device
+    tokens, experts = logits.shape[-2:]
+    groups = math.prod(logits.shape[:-2])
+    tickets = _tickets(dev, _ticket_bytes(groups, tokens, experts))
+    return BalanceLoss(*_lib.autograd().balance_loss(logits, mask, groups, config.top_k,
+                                                     _REDUCTIONS[config.reduction], tickets))

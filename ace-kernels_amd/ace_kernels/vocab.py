@@ -25,20 +25,20 @@ are not counted: their loss, confidence, correctness and gradients are 0 and
 their hidden states are not read (they may be NaN).  The mean is over the counted
 tokens, and 0 where there are none.  Logits, sums and gradients accumulate in
 float32; the gradients have the inputs' type, the losses are float32.
+
+The call and its backward node are C++ (``csrc/ace_autograd.cpp``).
 """
 
 from __future__ import annotations
 
-from typing import Any, Literal, NamedTuple, Optional, Tuple
+from typing import List, Literal, NamedTuple, Optional
 
 import torch
 from pydantic import BaseModel, ConfigDict
-from torch.autograd.function import once_differentiable
 
 from ace_kernels import _lib
-from ace_kernels.impls.hip_mi355x import _ptr, _stream
 
-_DTYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+_DTYPES = (torch.float32, torch.bfloat16, torch.float16)
 _REDUCTIONS = {"mean": _lib.RED_MEAN, "sum": _lib.RED_SUM, "none": _lib.RED_NONE}
 _LABEL_TYPES = (torch.int64, torch.int32, torch.int16, torch.int8, torch.uint8)
 
@@ -89,67 +89,13 @@ def _check(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor) -> 
         raise TypeError(f"labels must be integers, got {labels.dtype}")
 
 
-def _dense(t: torch.Tensor) -> torch.Tensor:
-    """``t`` contiguous and starting at a multiple of 16 bytes."""
-    t = t.contiguous()
-    return t.clone() if t.data_ptr() % 16 else t
-
-
-class _VocabLoss(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx: Any, hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
-                config: VocabConfig, scores: bool) -> Tuple[torch.Tensor, ...]:
-        lib = _lib.lib()
-        dev = hidden.device
-        size = weight.shape[1]
-        x, w = _dense(hidden.reshape(-1, size)), _dense(weight)
-        y = labels.reshape(-1).to(torch.int64).contiguous()
-        n = x.shape[0]
-        reduction = _REDUCTIONS[config.reduction]
-        dims = (n, size, weight.shape[0])
-        code = _DTYPES[hidden.dtype]
-        f32 = torch.float32
-        loss = torch.empty(labels.shape if reduction == _lib.RED_NONE else (), dtype=f32, device=dev)
-        confidence = torch.empty(labels.shape, dtype=f32, device=dev) if scores else None
-        correct = torch.empty(labels.shape, dtype=f32, device=dev) if scores else None
-        saved = torch.empty(lib.ace_vocab_saved_bytes(n), dtype=torch.uint8, device=dev)
-        with torch.cuda.device(dev):
-            ws = torch.empty(lib.ace_vocab_workspace_bytes(code, *dims, 0), dtype=torch.uint8, device=dev)
-            rc = lib.ace_vocab_forward(
-                x.data_ptr(), w.data_ptr(), code, y.data_ptr(), *dims, config.ignore_index, reduction,
-                saved.data_ptr(), loss.data_ptr(), _ptr(confidence), _ptr(correct),
-                ws.data_ptr(), ws.numel(), _stream(dev))
-        _lib.check(rc, "ace_vocab_forward")
-        ctx.save_for_backward(hidden, weight, saved)
-        ctx.call = (code, dims, reduction)
-        ctx.set_materialize_grads(False)
-        if not scores:
-            return (loss,)
-        ctx.mark_non_differentiable(correct)
-        return loss, confidence, correct
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx: Any, grad_loss: Optional[torch.Tensor], grad_confidence: Optional[torch.Tensor] = None,
-                 _correct: Optional[torch.Tensor] = None):
-        hidden, weight, saved = ctx.saved_tensors
-        code, dims, reduction = ctx.call
-        lib = _lib.lib()
-        dev = hidden.device
-        if grad_loss is None and grad_confidence is None:
-            return None, None, None, None, None
-        go = None if grad_loss is None else grad_loss.to(torch.float32).contiguous()
-        gc = None if grad_confidence is None else grad_confidence.to(torch.float32).contiguous()
-        x, w = _dense(hidden.reshape(-1, dims[1])), _dense(weight)
-        dx = torch.empty(hidden.shape, dtype=hidden.dtype, device=dev) if ctx.needs_input_grad[0] else None
-        dw = torch.empty(weight.shape, dtype=weight.dtype, device=dev) if ctx.needs_input_grad[1] else None
-        with torch.cuda.device(dev):
-            ws = torch.empty(lib.ace_vocab_workspace_bytes(code, *dims, 1), dtype=torch.uint8, device=dev)
-            rc = lib.ace_vocab_backward(
-                x.data_ptr(), w.data_ptr(), code, *dims, reduction, saved.data_ptr(), _ptr(go), _ptr(gc),
-                _ptr(dx), _ptr(dw), ws.data_ptr(), ws.numel(), _stream(dev))
-        _lib.check(rc, "ace_vocab_backward")
-        return dx, dw, None, None, None
+def _call(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor, config: Optional[VocabConfig],
+          scores: bool) -> List[torch.Tensor]:
+    _check(hidden, weight, labels)
+    config = config or _DEFAULT
+    out: List[torch.Tensor] = _lib.autograd().vocab_loss(hidden, weight, labels, config.ignore_index,
+                                                         _REDUCTIONS[config.reduction], scores)
+    return out
 
 
 def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
@@ -161,13 +107,11 @@ def vocab_loss(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
     scalar, or one value per token with ``reduction="none"``.  Differentiable
     once in ``hidden`` and ``weight``.
     """
-    _check(hidden, weight, labels)
-    return _VocabLoss.apply(hidden, weight, labels, config or _DEFAULT, False)[0]
+    return _call(hidden, weight, labels, config, False)[0]
 
 
 def vocab_loss_confidence(hidden: torch.Tensor, weight: torch.Tensor, labels: torch.Tensor,
                           config: Optional[VocabConfig] = None) -> VocabScores:
     """``vocab_loss`` with each token's top-label confidence and correctness,
     from the same pass."""
-    _check(hidden, weight, labels)
-    return VocabScores(*_VocabLoss.apply(hidden, weight, labels, config or _DEFAULT, True))
+    return VocabScores(*_call(hidden, weight, labels, config, True))

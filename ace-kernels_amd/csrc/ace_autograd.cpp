@@ -11,7 +11,13 @@
 // points that the Python loader hands over (set_entry_points), so that this
 // module and the ctypes binding drive the same loaded library.  Host code
 // only: it builds with g++ against torch's headers.
+//
+// The vocabulary losses (ace_kernels/vocab.py) and the balance loss
+// (ace_kernels/balance.py) have their calls and nodes here too, for any
+// arguments: the Python side checks them, nothing is remembered between calls.
+#include <ATen/DeviceGuard.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
@@ -271,6 +277,231 @@ std::vector<at::Tensor> ace_loss_levels(const std::vector<at::Tensor>& xs,
   return losses;
 }
 
+// ------------------------------------------------- language-model losses
+std::atomic<decltype(&ace_vocab_saved_bytes)> g_vocab_saved{nullptr};
+std::atomic<decltype(&ace_vocab_workspace_bytes)> g_vocab_workspace{nullptr};
+std::atomic<decltype(&ace_vocab_forward)> g_vocab_forward{nullptr};
+std::atomic<decltype(&ace_vocab_backward)> g_vocab_backward{nullptr};
+std::atomic<decltype(&ace_balance_workspace_bytes)> g_balance_workspace{nullptr};
+std::atomic<decltype(&ace_balance_forward)> g_balance_forward{nullptr};
+std::atomic<decltype(&ace_balance_backward)> g_balance_backward{nullptr};
+
+int dtype_code(const at::Tensor& t) {
+  switch (t.scalar_type()) {
+    case at::kFloat: return ACE_F32;
+    case at::kBFloat16: return ACE_BF16;
+    case at::kHalf: return ACE_F16;
+    default: throw std::invalid_argument("float32, bfloat16 or float16 tensors only");
+  }
+}
+
+// t contiguous and starting at a multiple of 16 bytes.
+at::Tensor dense(const at::Tensor& t) {
+  at::Tensor c = t.contiguous();
+  return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+}
+
+at::Tensor scratch(const at::Tensor& like, size_t bytes) {
+  return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte).requires_grad(false));
+}
+
+at::Tensor float32(const at::Tensor& g) {
+  return g.defined() ? g.to(at::kFloat).contiguous() : at::Tensor();
+}
+
+// Gradients of a backward that is itself recorded (create_graph) refuse to be
+// differentiated again, rather than pass as constants.
+void refuse_second_derivative(variable_list& out, const variable_list& inputs, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  auto node = std::make_shared<torch::autograd::Error>(
+      std::string(what) + " can be differentiated only once",
+      torch::autograd::collect_next_edges(inputs));
+  for (at::Tensor& t : out)
+    if (t.defined()) torch::autograd::set_history(t, node);
+}
+
+struct VocabLossBackward : public Node {
+  std::string name() const override { return "VocabLossBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(2);
+    const at::Tensor& gl = grads[0];
+    const at::Tensor gc = grads.size() > 1 ? grads[1] : at::Tensor();
+    if (!gl.defined() && !gc.defined()) return out;
+    const at::Tensor hidden = hidden_.unpack(), weight = weight_.unpack(), saved = saved_.unpack();
+    {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(hidden.device());
+      const at::Tensor x = dense(hidden.reshape({-1, size})), w = dense(weight);
+      const at::Tensor go = float32(gl), co = float32(gc);
+      if (task_should_compute_output(0))
+        out[0] = at::empty(hidden.sizes(), hidden.options().requires_grad(false));
+      if (task_should_compute_output(1))
+        out[1] = at::empty(weight.sizes(), weight.options().requires_grad(false));
+      const int code = dtype_code(hidden);
+      const at::Tensor ws = scratch(hidden, g_vocab_workspace.load()(code, tokens, size, vocab, 1));
+      const int rc = g_vocab_backward.load()(
+          x.data_ptr(), w.data_ptr(), code, tokens, size, vocab, reduction, saved.data_ptr(),
+          go.defined() ? go.data_ptr<float>() : nullptr,
+          co.defined() ? co.data_ptr<float>() : nullptr,
+          out[0].defined() ? out[0].data_ptr() : nullptr,
+          out[1].defined() ? out[1].data_ptr() : nullptr, ws.data_ptr(), (size_t)ws.numel(),
+          current_stream(hidden));
+      if (rc) fail(rc, "ace_vocab_backward");
+    }
+    refuse_second_derivative(out, {hidden, weight}, "vocab_loss");
+    return out;
+  }
+
+  void release_variables() override {
+    hidden_.reset_data();
+    weight_.reset_data();
+    saved_.reset_data();
+  }
+
+  int64_t tokens = 0, size = 0, vocab = 0;
+  int reduction = 0;
+  SavedVariable hidden_, weight_, saved_;
+};
+
+// (loss) or (loss, confidence, correct) of checked arguments.
+std::vector<at::Tensor> vocab_loss(const at::Tensor& hidden, const at::Tensor& weight,
+                                   const at::Tensor& labels, int64_t ignore_index, int reduction,
+                                   bool scores) {
+  if (!g_vocab_forward.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  const bool record = torch::autograd::compute_requires_grad(hidden, weight);
+  const c10::DeviceGuard guard(hidden.device());
+  std::vector<at::Tensor> out;
+  at::Tensor saved;
+  const int64_t size = weight.size(1), vocab = weight.size(0), tokens = labels.numel();
+  {
+    const at::NoGradGuard no_grad;
+    const at::Tensor x = dense(hidden.reshape({-1, size})), w = dense(weight);
+    const at::Tensor y = labels.to(at::kLong).contiguous();
+    const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
+    const int code = dtype_code(hidden);
+    out.push_back(reduction == ACE_RED_NONE ? at::empty(labels.sizes(), f32) : at::empty({}, f32));
+    if (scores)
+      for (int i = 0; i < 2; ++i) out.push_back(at::empty(labels.sizes(), f32));
+    saved = scratch(hidden, g_vocab_saved.load()(tokens));
+    const at::Tensor ws = scratch(hidden, g_vocab_workspace.load()(code, tokens, size, vocab, 0));
+    const int rc = g_vocab_forward.load()(
+        x.data_ptr(), w.data_ptr(), code, y.data_ptr<int64_t>(), tokens, size, vocab, ignore_index,
+        reduction, saved.data_ptr(), out[0].data_ptr<float>(),
+        scores ? out[1].data_ptr<float>() : nullptr, scores ? out[2].data_ptr<float>() : nullptr,
+        ws.data_ptr(), (size_t)ws.numel(), current_stream(hidden));
+    if (rc) fail(rc, "ace_vocab_forward");
+  }
+  if (record) {
+    auto node = std::shared_ptr<VocabLossBackward>(new VocabLossBackward(),
+                                                   torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(hidden, weight));
+    node->tokens = tokens;
+    node->size = size;
+    node->vocab = vocab;
+    node->reduction = reduction;
+    node->hidden_ = SavedVariable(hidden, false);
+    node->weight_ = SavedVariable(weight, false);
+    node->saved_ = SavedVariable(saved, false);
+    torch::autograd::set_history(out[0], node);
+    if (scores) torch::autograd::set_history(out[1], node);
+  }
+  return out;
+}
+
+struct BalanceLossBackward : public Node {
+  std::string name() const override { return "BalanceLossBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(1);
+    if (!grads[0].defined()) return out;
+    const at::Tensor logits = logits_.unpack(), share = share_.unpack(), mask = mask_.unpack();
+    {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(logits.device());
+      const at::Tensor x = logits.contiguous(), go = float32(grads[0]);
+      const at::Tensor m = mask.defined() ? mask.contiguous() : mask;
+      out[0] = at::empty(logits.sizes(), logits.options().requires_grad(false));
+      const int rc = g_balance_backward.load()(
+          x.data_ptr(), dtype_code(logits),
+          m.defined() ? static_cast<const uint8_t*>(m.data_ptr()) : nullptr, groups, tokens,
+          experts, reduction, share.data_ptr<float>(), go.data_ptr<float>(), out[0].data_ptr(),
+          current_stream(logits));
+      if (rc) fail(rc, "ace_balance_backward");
+    }
+    refuse_second_derivative(out, {logits}, "balance_loss");
+    return out;
+  }
+
+  void release_variables() override {
+    logits_.reset_data();
+    mask_.reset_data();
+    share_.reset_data();
+  }
+
+  int64_t groups = 0, tokens = 0, experts = 0;
+  int reduction = 0;
+  SavedVariable logits_, mask_, share_;
+};
+
+// (loss, counts) of checked arguments; `tickets`: zero, left zero.
+std::vector<at::Tensor> balance_loss(const at::Tensor& logits, const std::optional<at::Tensor>& mask,
+                                     int64_t groups, int top_k, int reduction,
+                                     const at::Tensor& tickets) {
+  if (!g_balance_forward.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  const bool record = torch::autograd::compute_requires_grad(logits);
+  const c10::DeviceGuard guard(logits.device());
+  const int64_t tokens = logits.size(-2), experts = logits.size(-1);
+  at::Tensor loss, counts, share;
+  {
+    const at::NoGradGuard no_grad;
+    const at::Tensor x = logits.contiguous();
+    const at::Tensor m = mask ? mask->contiguous() : at::Tensor();
+    const auto options = logits.options().requires_grad(false);
+    std::vector<int64_t> lead(logits.sizes().begin(), logits.sizes().end() - 2);
+    loss = at::empty(reduction == ACE_RED_NONE ? lead : std::vector<int64_t>{},
+                     options.dtype(at::kFloat));
+    lead.push_back(experts);
+    counts = at::empty(lead, options.dtype(at::kLong));
+    share = at::empty({groups, experts}, options.dtype(at::kFloat));
+    const at::Tensor ws = scratch(logits, g_balance_workspace.load()(groups, tokens, experts));
+    const int rc = g_balance_forward.load()(
+        x.data_ptr(), dtype_code(logits),
+        m.defined() ? static_cast<const uint8_t*>(m.data_ptr()) : nullptr, groups, tokens, experts,
+        top_k, reduction, loss.data_ptr<float>(), counts.data_ptr<int64_t>(),
+        share.data_ptr<float>(), tickets.data_ptr(), (size_t)tickets.numel(), ws.data_ptr(),
+        (size_t)ws.numel(), current_stream(logits));
+    if (rc) fail(rc, "ace_balance_forward");
+  }
+  if (record) {
+    auto node = std::shared_ptr<BalanceLossBackward>(new BalanceLossBackward(),
+                                                     torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->groups = groups;
+    node->tokens = tokens;
+    node->experts = experts;
+    node->reduction = reduction;
+    node->logits_ = SavedVariable(logits, false);
+    if (mask) node->mask_ = SavedVariable(*mask, false);
+    node->share_ = SavedVariable(share, false);
+    torch::autograd::set_history(loss, node);
+  }
+  return {loss, counts};
+}
+
+void set_lm_entry_points(uintptr_t vocab_saved, uintptr_t vocab_workspace, uintptr_t vocab_forward,
+                         uintptr_t vocab_backward, uintptr_t balance_workspace,
+                         uintptr_t balance_forward, uintptr_t balance_backward) {
+  g_vocab_saved.store(reinterpret_cast<decltype(&ace_vocab_saved_bytes)>(vocab_saved));
+  g_vocab_workspace.store(reinterpret_cast<decltype(&ace_vocab_workspace_bytes)>(vocab_workspace));
+  g_vocab_forward.store(reinterpret_cast<decltype(&ace_vocab_forward)>(vocab_forward));
+  g_vocab_backward.store(reinterpret_cast<decltype(&ace_vocab_backward)>(vocab_backward));
+  g_balance_workspace.store(
+      reinterpret_cast<decltype(&ace_balance_workspace_bytes)>(balance_workspace));
+  g_balance_forward.store(reinterpret_cast<decltype(&ace_balance_forward)>(balance_forward));
+  g_balance_backward.store(reinterpret_cast<decltype(&ace_balance_backward)>(balance_backward));
+}
+
 std::shared_ptr<LevelSignature> make_level_signature(
     int x_dtype, int64_t batch, int64_t channels, int num_bins, int binning, int include_background,
     int ignore_empty, int reduction, int right, float empty_weight, uintptr_t class_weight,
@@ -362,4 +593,8 @@ PYBIND11_MODULE(_ace_autograd, m) {
   m.def("set_entry_points", &set_entry_points);
   m.def("ace_loss", &ace_loss);
   m.def("ace_loss_levels", &ace_loss_levels);
+  m.def("set_lm_entry_points", &set_lm_entry_points);
+  m.def("vocab_loss", &vocab_loss);
+  m.def("balance_loss", &balance_loss, pybind11::arg(), pybind11::arg().none(true), pybind11::arg(),
+        pybind11::arg(), pybind11::arg(), pybind11::arg());
 }

@@ -21,14 +21,14 @@ Geometry geometry(int64_t groups, int64_t tokens, int experts) {
   Geometry g{};
   // one lane a token up to 16 experts, then 16 scores a lane up to 64, 32 above:
   // fewer lanes mean fewer exchanges, more registers
-  g.c = experts <= 8 ? 8 : experts <= 64 ? 16 : 32;
+  g.c = experts <= 8 ? 8 : 16;
   while ((g.c << g.lanes_log2) < experts) ++g.lanes_log2;
   const int64_t at_once = kThreads >> g.lanes_log2;  // tokens of a block at a time
   const int64_t most = (tokens + at_once - 1) / at_once;
   int64_t blocks = (kTarget + groups - 1) / groups;
   if (blocks > most) blocks = most;
   if (blocks > kMaxBlocks) blocks = kMaxBlocks;
-  if (blocks < 1) blocks = 1;
+  if (blocks < 1 || most <= 4) blocks = 1;  // a few rounds cost less than joining blocks
   const int64_t rounds = (most + blocks - 1) / blocks;
   g.per_block = (rounds > 0 ? rounds : 1) * at_once;
   g.blocks = (int)((tokens + g.per_block - 1) / g.per_block);
@@ -94,15 +94,12 @@ void launch_forward(const Params& p, hipStream_t s) {
 template <typename T>
 int launch(const Params& p, int c, bool backward, hipStream_t s) {
   const dim3 grid((unsigned)(p.groups * p.blocks)), block(kThreads);
-  if (!backward) {
-    c == 8 ? launch_forward<T, 8>(p, s) : c == 16 ? launch_forward<T, 16>(p, s) : launch_forward<T, 32>(p, s);
-  } else if (c == 8) {
+  if (!backward)
+    c == 8 ? launch_forward<T, 8>(p, s) : launch_forward<T, 16>(p, s);
+  else if (c == 8)
     hipLaunchKernelGGL((backward_kernel<T, 8>), grid, block, 0, s, p);
-  } else if (c == 16) {
+  else
     hipLaunchKernelGGL((backward_kernel<T, 16>), grid, block, 0, s, p);
-  } else {
-    hipLaunchKernelGGL((backward_kernel<T, 32>), grid, block, 0, s, p);
-  }
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? ACE_OK : ACE_EHIP + (int)e;
 }

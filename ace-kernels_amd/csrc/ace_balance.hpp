@@ -75,11 +75,13 @@ struct Row {
   static_assert(C % V == 0, "whole pieces");
   int at[P];       // first expert of a piece, or -1: none
   uint32_t fresh;  // bit i: score i counts
-  bool ragged;     // some row of the kernel has a piece that is partly fresh
+  bool ragged;     // some lane has a piece that is partly fresh
+  bool partial;    // some lane has fewer than C scores
 
   __device__ void init(int experts, int lane, int lanes) {
     fresh = 0;
     ragged = experts % V != 0;
+    partial = lanes * C != experts;
 #pragma unroll
     for (int i = 0; i < P; ++i) {
       const int first = (lane + lanes * i) * V;
@@ -133,7 +135,8 @@ struct Row {
 // D already agree: neighbours, pairs, then mirror images of 8 and of 16 lanes.
 template <int D>
 __device__ inline uint32_t across(uint32_t x) {
-  static_assert(D == 1 || D == 2 || D == 4 || D == 8, "at most 16 lanes");
+  static_assert(D == 1 || D == 2 || D == 4 || D == 8 || D == 16, "at most 32 lanes");
+  if constexpr (D == 16) return (uint32_t)__shfl_xor((int)x, 16);
   constexpr int ctrl = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;
   return (uint32_t)__builtin_amdgcn_mov_dpp((int)x, ctrl, 0xf, 0xf, false);
 }
@@ -149,6 +152,7 @@ __device__ inline X over_lanes(X x, int lanes, Op op) {
   if (lanes > 2) x = op(x, other(std::integral_constant<int, 2>{}));
   if (lanes > 4) x = op(x, other(std::integral_constant<int, 4>{}));
   if (lanes > 8) x = op(x, other(std::integral_constant<int, 8>{}));
+  if (lanes > 16) x = op(x, other(std::integral_constant<int, 16>{}));
   return x;
 }
 
@@ -156,19 +160,17 @@ constexpr auto kAdd = [](auto a, auto b) { return a + b; };
 constexpr auto kMin = [](auto a, auto b) { return a < b ? a : b; };
 constexpr auto kFmax = [](float a, float b) { return fmaxf(a, b); };
 
-// Unsigned, in the scores' order: -0 is 0, and NaN is above everything.
-__device__ inline uint32_t key_of(float x) {
-  if (x != x) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(x + 0.f);
+// Unsigned, in the scores' order, -0 as 0.  NaN is somewhere: `choose` puts it
+// above everything where there is one.  For 16-bit scores the upper half
+// suffices.
+__device__ inline uint32_t ordered(uint32_t b) {
   return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
-// For 16-bit scores the upper half suffices.
-__device__ inline uint32_t half_key(__bf16 x) { return key_of((float)x) & 0xffff0000u; }
-__device__ inline uint32_t half_key(_Float16 x) {
-  if (x != x) return 0xffff0000u;
+__device__ inline uint32_t key_of(float x) { return ordered(__float_as_uint(x + 0.f)); }
+__device__ inline uint32_t key_of(__bf16 x) { return key_of((float)x) & 0xffff0000u; }
+__device__ inline uint32_t key_of(_Float16 x) {
   const _Float16 y = x + (_Float16)0.f;
-  const uint32_t b = (uint32_t)__builtin_bit_cast(uint16_t, y) << 16;
-  return b ^ (((uint32_t)((int32_t)b >> 31) | 0x80000000u) & 0xffff0000u);
+  return ordered((uint32_t)__builtin_bit_cast(uint16_t, y) << 16) & 0xffff0000u;
 }
 
 __device__ inline uint32_t median(uint32_t a, uint32_t b, uint32_t c) {
@@ -177,27 +179,28 @@ __device__ inline uint32_t median(uint32_t a, uint32_t b, uint32_t c) {
 
 // The scores' keys and the threshold that the k largest reach: score i is taken
 // where key[i] >= the result.  `on`: the token is counted, its scores are there;
-// others take nothing.
+// others take nothing.  `nans`: some score of the wave may be NaN.
 template <typename T, int C, int K>
 __device__ inline uint32_t choose(const Row<T, C>& row, const T (&x)[C], int lanes, int top_k,
-                                  bool on, uint32_t (&key)[C]) {
-  constexpr int V = Row<T, C>::V;
+                                  bool on, bool nans, uint32_t (&key)[C]) {
   constexpr bool numbered = sizeof(T) == 2;
   uint32_t list[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) list[k] = 0;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    if constexpr (numbered)
-      key[i] = half_key(x[i]) | (0xffffu ^ (uint32_t)row.expert(i));
-    else
-      key[i] = key_of(x[i]);
-    if (row.at[i / V] < 0) key[i] = 0;  // below every score's key
+    key[i] = key_of(x[i]);
+    if constexpr (numbered) key[i] |= 0xffffu ^ (uint32_t)row.expert(i);
   }
-  if (row.ragged) {
+  if (nans) {
 #pragma unroll
     for (int i = 0; i < C; ++i)
-      if (!row.is_fresh(i)) key[i] = 0;
+      if (x[i] != x[i]) key[i] |= 0xffff0000u | (numbered ? 0u : 0xffffu);
+  }
+  if (row.partial) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (!row.is_fresh(i)) key[i] = 0;  // below every score's key
   }
 #pragma unroll
   for (int i = 0; i < C; ++i) {
@@ -227,6 +230,7 @@ __device__ inline uint32_t choose(const Row<T, C>& row, const T (&x)[C], int lan
   if (lanes > 2) merge(std::integral_constant<int, 2>{});
   if (lanes > 4) merge(std::integral_constant<int, 4>{});
   if (lanes > 8) merge(std::integral_constant<int, 8>{});
+  if (lanes > 16) merge(std::integral_constant<int, 16>{});
   uint32_t least = list[0];
 #pragma unroll
   for (int k = 1; k < K; ++k) least = k < top_k ? list[k] : least;
@@ -269,10 +273,14 @@ __device__ inline float exponentials(const Row<T, C>& row, const T (&x)[C], int 
   constexpr int V = Row<T, C>::V;
   float top = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < C; ++i) {
-    e[i] = row.at[i / V] < 0 ? -INFINITY : (float)x[i];
-    top = fmaxf(top, e[i]);
+  for (int i = 0; i < C; ++i) e[i] = (float)x[i];
+  if (row.partial) {
+#pragma unroll
+    for (int i = 0; i < C; ++i)
+      if (row.at[i / V] < 0) e[i] = -INFINITY;
   }
+#pragma unroll
+  for (int i = 0; i < C; ++i) top = fmaxf(top, e[i]);
   top = over_lanes(top, lanes, kFmax);
 #pragma unroll
   for (int i = 0; i < C; ++i) e[i] = __builtin_amdgcn_exp2f((e[i] - top) * 1.4426950408889634f);
@@ -313,7 +321,7 @@ __device__ inline double load_dev(const double* p) {
 }
 
 template <typename T, int C, int K>
-__global__ __launch_bounds__(kThreads, C == 32 ? 3 : 4) void forward_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, 4) void forward_kernel(Params p) {
   __shared__ float s_sum[kMaxExperts];
   __shared__ int s_count[kMaxExperts + 1];
   __shared__ double s_loss[kThreads / 64];
@@ -342,16 +350,17 @@ __global__ __launch_bounds__(kThreads, C == 32 ? 3 : 4) void forward_kernel(Para
 #pragma unroll
     for (int i = 0; i < C; ++i) x[i] = (T)0.f;
     if (counted) row.load(logits + mine * E, E, x);
-    uint32_t key[C];
-    const uint32_t least = choose<T, C, K>(row, x, lanes, p.top_k, counted, key);
-#pragma unroll
-    for (int i = 0; i < C; ++i) count[i] += key[i] >= least;
     float e[C];
     const float inv = exponentials<T, C>(row, x, lanes, e);
     const float of = counted ? inv : 0.f;
 #pragma unroll
     for (int i = 0; i < C; ++i) sum[i] = fmaf(e[i], of, sum[i]);
     tokens += counted && j == 0;
+    uint32_t key[C];
+    const uint32_t least =
+        choose<T, C, K>(row, x, lanes, p.top_k, counted, __ballot(inv != inv) != 0, key);
+#pragma unroll
+    for (int i = 0; i < C; ++i) count[i] += key[i] >= least;
   }
   // across the wave's tokens, then the waves in turn
   for (int d = lanes; d < 64; d *= 2) {
@@ -459,7 +468,7 @@ __global__ __launch_bounds__(kThreads, C == 32 ? 3 : 4) void forward_kernel(Para
 }
 
 template <typename T, int C>
-__global__ __launch_bounds__(kThreads, C == 32 ? 3 : 4) void backward_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, 4) void backward_kernel(Params p) {
   constexpr int V = Row<T, C>::V;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lanes = 1 << p.lanes_log2, j = lane & (lanes - 1);
