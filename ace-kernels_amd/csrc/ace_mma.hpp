@@ -15,12 +15,13 @@
 //                 the group's 4 x 16 block), so no operand is ever transposed
 //                 in memory.
 //
-// A step of k is 128 bytes wide (64 elements of 16 bits, 32 floats).  Operands
-// go from memory to LDS directly (global_load_lds, 16 bytes a lane), one step
-// ahead of the products, into the other of two buffers.  Rows of LDS are
-// swizzled in units of 16 bytes (k contiguous) or of 16 columns (m contiguous),
-// on the side of the global address because the LDS side of such a load is
-// fixed, so that the lanes one LDS cycle serves touch different banks.
+// A step of k is 64 bytes wide (32 elements of 16 bits, 16 floats).  LDS holds a
+// ring of four steps: while the products of step s run, step s + 1 goes from LDS
+// to registers and step s + 3 from memory to LDS directly (global_load_lds, 16
+// bytes a lane), so that neither latency is waited for; one barrier a step.  Rows
+// of LDS are swizzled in units of 16 bytes (k contiguous) or of 16 columns (m
+// contiguous), on the side of the global address because the LDS side of such a
+// load is fixed, so that the lanes one LDS cycle serves touch different banks.
 //
 // Accumulators are float32 throughout.  In C, lane l of a wave holds, for each
 // 16 x 16 piece, column n = l % 16 and the four rows m = 4 (l / 16) + 0..3.
@@ -38,7 +39,9 @@ using s16x8 = short __attribute__((ext_vector_type(8)));
 using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 
-constexpr int kStepBytes = 128;  // bytes of k in one step
+constexpr int kStepBytes = 64;  // bytes of k in one step
+constexpr int kRing = 4;        // steps in LDS
+constexpr int kAhead = 3;       // steps between loading one and multiplying it
 
 template <typename T>
 constexpr int kStep = kStepBytes / (int)sizeof(T);  // elements of k in one step
@@ -48,21 +51,54 @@ __device__ inline char* lds_base() {
   return ace_mma_lds;
 }
 
-// 16 bytes a lane from `src` (the lane's own address) to LDS at `dst` (the
-// wave's) + 16 lane.
+// 16 bytes a lane from memory to LDS at `dst` (the wave's) + 16 lane: from a
+// uniform base and the lane's offset, or from the lane's own address.  With ASM
+// it is written as assembler: the compiler waits for every load to LDS that it
+// knows of before each transposing LDS read, which takes the whole pipeline away
+// (8192 x 8192 x 4096 in bfloat16: 820 TFLOP/s instead of 1146).  Nothing here has
+// an output, the waits are landed_barrier's, and nothing else in a kernel that
+// uses it needs m0.  Where no transposing reads are,
+// the builtin leaves the compiler more freedom (1200 instead of 1140).
+__device__ inline uint32_t lds_address(const char* p) {
+  return (uint32_t)__builtin_amdgcn_readfirstlane(
+      (int)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
+}
+__device__ inline const char* uniform(const char* p) {
+  const uint64_t a = (uint64_t)p;
+  const uint32_t low = (uint32_t)__builtin_amdgcn_readfirstlane((int)a);
+  const uint32_t high = (uint32_t)__builtin_amdgcn_readfirstlane((int)(a >> 32));
+  return (const char*)((uint64_t)high << 32 | low);
+}
+template <bool ASM>
+__device__ inline void load_to_lds(const char* base, uint32_t off, char* dst) {
+  if constexpr (ASM)
+    asm volatile(
+        "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_address(dst)),
+        "v"(off), "s"(uniform(base)));
+  else
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + off),
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+}
+template <bool ASM>
 __device__ inline void load_to_lds(const char* src, char* dst) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+  if constexpr (ASM)
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
+                     lds_address(dst)),
+                 "v"(src));
+  else
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                     (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
 }
 
-// Every load to LDS of this wave has landed, and every wave has come here.
+// All but the wave's last N memory operations are done, its LDS reads are, and
+// every wave has come here.
+template <int N>
 __device__ inline void landed_barrier() {
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
-  __syncthreads();
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
 }
 
 // One operand's side of a tile: R rows (free index) by one step of k.
-template <typename T, int R, bool KC, int THREADS>
+template <typename T, int R, bool KC, int THREADS, bool ASM>
 struct Operand {
   static constexpr int kBytes = R * kStepBytes;
   static constexpr int kChunks = KC ? kStepBytes / 16 : R * (int)sizeof(T) / 16;  // per LDS row
@@ -73,7 +109,9 @@ struct Operand {
   // Which 16-byte chunk of the row holds logical chunk c (its own inverse).
   __device__ static int swizzle(int row, int c) {
     if constexpr (KC) {
-      return c ^ (row & 7);
+      // a cycle of 16-byte reads serves lanes l..l+7 and l+16..l+23: eight rows,
+      // two neighbouring chunks of each
+      return c ^ ((row >> 1) & 2);
     } else if constexpr (sizeof(T) == 2) {
       // units of 16 columns: the 16 rows of one transposing read are
       // 8 g + j (+ 4), g and j in 0..3
@@ -107,32 +145,37 @@ struct Operand {
     }
   }
 
-  // Loads one step into LDS at `lds`.  `base`: the operand at the tile's first
-  // free index and the step's first k.  With TAIL, `left` k's are left (fewer
-  // than a step); the others are read from `zeros` (16 zero bytes).
-  template <bool TAIL>
-  __device__ void load(const char* base, char* lds, int left, const char* zeros) const {
-    const int wave = (int)threadIdx.x / 64;
+  // Whether this wave has a part in load i.
+  __device__ static bool has(int i) {
+    return kBytes % (16 * THREADS) == 0 || i < kLoads - 1 ||
+           (i * THREADS + (int)threadIdx.x / 64 * 64) * 16 < kBytes;
+  }
+  __device__ static char* at(char* lds, int i) {
+    return lds + (i * THREADS + (int)threadIdx.x / 64 * 64) * 16;
+  }
+
+  // Load i of one step into LDS at `lds`.  `base` (uniform): the operand at the
+  // tile's first free index and the step's first k.
+  __device__ void load(int i, const char* base, char* lds) const {
+    if (has(i)) load_to_lds<ASM>(base, off[i], at(lds, i));
+  }
+
+  // All loads of a step of which only `left` k's exist; the others are read from
+  // `zeros` (16 zero bytes).
+  __device__ void load_tail(const char* base, char* lds, int left, const char* zeros) const {
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
-      if (kBytes % (16 * THREADS) != 0 && i == kLoads - 1 &&
-          (i * THREADS + wave * 64) * 16 >= kBytes)
-        break;  // whole waves have nothing to load
-      const char* src = base + off[i];
-      if constexpr (TAIL) {
-        const int c = i * THREADS + (int)threadIdx.x;
-        const int row = c / kChunks;
-        const int k = KC ? swizzle(row, c % kChunks) * (16 / (int)sizeof(T)) : row;
-        if (k >= left) src = zeros;
-      }
-      load_to_lds(src, lds + (i * THREADS + wave * 64) * 16);
+      const int c = i * THREADS + (int)threadIdx.x;
+      const int row = c / kChunks;
+      const int k = KC ? swizzle(row, c % kChunks) * (16 / (int)sizeof(T)) : row;
+      if (has(i)) load_to_lds<ASM>(k < left ? base + off[i] : zeros, at(lds, i));
     }
   }
 };
 
-// Fragments of the matrix instructions.  16 bits: 32 k's an instruction, lane
-// group g = l / 16 holds k = 8 g + 0..7.  float32: four instructions of 4 k's
-// for 16 k's, instruction j takes k = 4 g + j of lane group g.
+// Fragments of the matrix instructions, one a step.  16 bits: 32 k's an
+// instruction, lane group g = l / 16 holds k = 8 g + 0..7.  float32: four
+// instructions of 4 k's, instruction j takes k = 4 g + j of lane group g.
 template <typename T>
 struct Frag {
   s16x8 v;
@@ -142,24 +185,22 @@ struct Frag<float> {
   f32x4 v;
 };
 
-constexpr int kSub = 2;  // fragments of k per step
-
-// The fragment `kk` of the 16 rows that begin at `row`.
+// The fragment of the 16 rows that begin at `row`.
 template <typename T, int R, bool KC>
-__device__ inline Frag<T> read_frag(const char* lds, int row, int kk) {
-  using Op = Operand<T, R, KC, 64>;
+__device__ inline Frag<T> read_frag(const char* lds, int row) {
+  using Op = Operand<T, R, KC, 64, false>;
   const int lane = (int)threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
   Frag<T> f;
   if constexpr (KC) {
     const int r = row + n;
-    const char* at = lds + r * kStepBytes + Op::swizzle(r, kk * 4 + g) * 16;
+    const char* at = lds + r * kStepBytes + Op::swizzle(r, g) * 16;
     f.v = *reinterpret_cast<const decltype(f.v)*>(at);
   } else if constexpr (sizeof(T) == 2) {
     s16x4 h[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int k = kk * 32 + 8 * g + 4 * i + (n >> 2);  // the lane's row of the 4 x 16 block
+      const int k = 8 * g + 4 * i + (n >> 2);  // the lane's row of the 4 x 16 block
       const char* at =
           lds + k * (R * 2) + Op::swizzle(k, row / 8 + ((n >> 1) & 1)) * 16 + (n & 1) * 8;
       h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -169,7 +210,7 @@ __device__ inline Frag<T> read_frag(const char* lds, int row, int kk) {
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int k = kk * 16 + 4 * g + j;
+      const int k = 4 * g + j;
       const int c = row + n;
       f.v[j] = *reinterpret_cast<const float*>(lds + k * (R * 4) + Op::swizzle(k, c / 4) * 16 +
                                                (c & 3) * 4);
@@ -206,10 +247,11 @@ struct Tile {
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // 16 x 16 pieces of a wave
   static constexpr int kStageBytes = (BM + BN) * kStepBytes;
-  static constexpr int kLdsBytes = 2 * kStageBytes;
+  static constexpr int kLdsBytes = kRing * kStageBytes;
   static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "whole pieces");
-  using OpA = Operand<T, BM, AKC_, kThreads>;
-  using OpB = Operand<T, BN, BKC_, kThreads>;
+  static constexpr bool kAsm = sizeof(T) == 2 && !(AKC_ && BKC_);  // transposing reads
+  using OpA = Operand<T, BM, AKC_, kThreads, kAsm>;
+  using OpB = Operand<T, BN, BKC_, kThreads, kAsm>;
 
   // What one operand needs of memory: its address at the tile's first free
   // index and k = 0, and the bytes from one step of k to the next.
@@ -231,49 +273,148 @@ struct Tile {
   __device__ static void load(const OpA& a, const OpB& b, Source sa, Source sb, int step, int k,
                               char* lds, const char* zeros) {
     const int left = k - step * kStep<T>;
-    const char* pa = sa.base + step * sa.step;
-    const char* pb = sb.base + step * sb.step;
     if (left >= kStep<T>) {
-      a.template load<false>(pa, lds, left, zeros);
-      b.template load<false>(pb, lds + OpA::kBytes, left, zeros);
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) load_one(i, a, b, sa, sb, step, lds);
     } else {
-      a.template load<true>(pa, lds, left, zeros);
-      b.template load<true>(pb, lds + OpA::kBytes, left, zeros);
+      a.load_tail(sa.base + step * sa.step, lds, left, zeros);
+      b.load_tail(sb.base + step * sb.step, lds + OpA::kBytes, left, zeros);
     }
   }
+  static constexpr int kLoads = OpA::kLoads + OpB::kLoads;  // of a step
+  __device__ static void load_one(int i, const OpA& a, const OpB& b, Source sa, Source sb, int step,
+                                  char* lds) {
+    if (i < OpA::kLoads)
+      a.load(i, sa.base + step * sa.step, lds);
+    else
+      b.load(i - OpA::kLoads, sb.base + step * sb.step, lds + OpA::kBytes);
+  }
 
-  __device__ static void step(const char* lds, f32x4 (&acc)[MT][NT]) {
+  struct Frags {
+    Frag<T> a[MT], b[NT];
+  };
+
+  // Fragments first..last-1 of a step, those of b before those of a.
+  __device__ static void read(const char* lds, Frags& f, int first = 0, int last = MT + NT) {
     const int m0 = wave_m(), n0 = wave_n();
 #pragma unroll
-    for (int kk = 0; kk < kSub; ++kk) {
-      Frag<T> a[MT], b[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-        b[j] = read_frag<T, BN, BKC_>(lds + OpA::kBytes, n0 + 16 * j, kk);
-#pragma unroll
-      for (int i = 0; i < MT; ++i) a[i] = read_frag<T, BM, AKC_>(lds, m0 + 16 * i, kk);
-#pragma unroll
-      for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) acc[i][j] = multiply<T>(a[i], b[j], acc[i][j]);
+    for (int i = first; i < last; ++i) {
+      if (i < NT)
+        f.b[i] = read_frag<T, BN, BKC_>(lds + OpA::kBytes, n0 + 16 * i);
+      else
+        f.a[i - NT] = read_frag<T, BM, AKC_>(lds, m0 + 16 * (i - NT));
     }
   }
 
-  // acc += the product over steps first..last-1 of a k values long product.  The
-  // caller's waves all come here with the same arguments, with nothing reading
-  // LDS any more.
-  __device__ static void product(const OpA& a, const OpB& b, Source sa, Source sb, int first,
-                                 int last, int k, const char* zeros, f32x4 (&acc)[MT][NT]) {
-    char* lds = lds_base();
-    if (first >= last) return;
-    load(a, b, sa, sb, first, k, lds, zeros);
-    for (int s = first; s < last; ++s) {
-      char* here = lds + ((s - first) & 1) * kStageBytes;
-      landed_barrier();  // step s is in LDS, and nothing reads the other buffer
-      if (s + 1 < last)
-        load(a, b, sa, sb, s + 1, k, lds + ((s + 1 - first) & 1) * kStageBytes, zeros);
-      step(here, acc);
+  __device__ static void multiply_all(const Frags& f, f32x4 (&acc)[MT][NT]) {
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+      for (int j = 0; j < NT; ++j) acc[i][j] = multiply<T>(f.a[i], f.b[j], acc[i][j]);
+  }
+
+  // False: this wave has no part in the last load of a step.
+  __device__ static bool loads_all() {
+    static_assert(OpA::kBytes % (16 * kThreads) == 0, "whole loads of the first operand");
+    return OpB::has(OpB::kLoads - 1);
+  }
+
+  // Spreads a step's LDS reads (and with them the loads between them) evenly among
+  // its matrix instructions, so that the matrix cores do not wait for a burst.
+  __device__ static void interleave() {
+    constexpr int per = sizeof(T) == 4 ? 4 : 1;  // matrix instructions of a piece
+    constexpr int reads_a = MT * (AKC_ ? 1 : sizeof(T) == 4 ? 4 : 2);
+    constexpr int reads_b = NT * (BKC_ ? 1 : sizeof(T) == 4 ? 4 : 2);
+    constexpr int n = MT * NT * per, reads = reads_a + reads_b;
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction
+      const int r = (i + 1) * reads / n - i * reads / n;
+      if (r == 1) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);  // LDS reads
+      if (r == 2) __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
+      if (r > 2) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+      if (!kAsm && (i + 1) * kLoads / n > i * kLoads / n)
+        __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);  // a load
     }
+  }
+
+  // The main loop over a sequence of steps that may span tiles.
+  struct Pipe {
+    int fed = 0, done = 0;  // steps loaded, and multiplied
+    Frags now;
+
+    __device__ char* slot(int step) const { return lds_base() + (step % kRing) * kStageBytes; }
+
+    // Nothing else may be reading LDS.  `feed(lds)` loads the next step of the
+    // sequence to `lds` and says whether there was one.
+    template <typename Feed>
+    __device__ void begin(Feed feed) {
+      for (int i = 0; i < kAhead; ++i)
+        if (feed(slot(fed))) ++fed;
+      landed_barrier<0>();
+      if (fed) read(slot(0), now);
+    }
+
+    // `n` steps into acc, of which at least the first `plain` have a `simple(i, lds)`
+    // in place of the feed: it makes load i of a whole step, without a condition.
+    template <typename Simple, typename Feed>
+    __device__ void run(int n, int plain, Simple simple, Feed feed, f32x4 (&acc)[MT][NT]) {
+      Frags next;
+      int s = 0;
+      for (; s + 2 <= plain; s += 2) {
+        plain_step(simple, now, next, acc);
+        plain_step(simple, next, now, acc);
+      }
+      for (; s + 2 <= n; s += 2) {
+        any_step(feed, now, next, acc);
+        any_step(feed, next, now, acc);
+      }
+      if (s < n) {
+        any_step(feed, now, next, acc);
+        now = next;
+      }
+    }
+
+    template <typename Simple>
+    __device__ void plain_step(Simple simple, const Frags& f, Frags& next, f32x4 (&acc)[MT][NT]) {
+      if (loads_all())  // step done + 1 has landed
+        landed_barrier<kLoads*(kAhead - 2)>();
+      else
+        landed_barrier<(kLoads - 1) * (kAhead - 2)>();
+      // loads and reads in turn: neither is moved past the other
+      constexpr int all = MT + NT;
+#pragma unroll
+      for (int i = 0; i < kLoads; ++i) {
+        simple(i, slot(fed));
+        read(slot(done + 1), next, i * all / kLoads, (i + 1) * all / kLoads);
+      }
+      multiply_all(f, acc);
+      interleave();
+      ++fed;
+      ++done;
+    }
+
+    template <typename Feed>
+    __device__ void any_step(Feed feed, const Frags& f, Frags& next, f32x4 (&acc)[MT][NT]) {
+      if (fed - done < kAhead)  // the end of the sequence
+        landed_barrier<0>();
+      else if (loads_all())
+        landed_barrier<kLoads*(kAhead - 2)>();
+      else
+        landed_barrier<(kLoads - 1) * (kAhead - 2)>();
+      if (feed(slot(fed))) ++fed;
+      read(slot(done + 1), next);  // past the end: whatever the slot holds, unused
+      multiply_all(f, acc);
+      ++done;
+    }
+  };
+
+  // How many of a tile's steps first..last-1 of k values may feed simply: those
+  // whose step kAhead on is whole and in the tile.
+  __device__ static int plain_steps(int first, int last, int k) {
+    const int whole = k / kStep<T> < last ? k / kStep<T> : last;
+    const int n = whole - first - kAhead;
+    return n > 0 ? n : 0;
   }
 };
 

@@ -186,7 +186,7 @@ Plan make_plan(int dtype, int64_t n, int64_t h, int64_t v) {
   // whole tiles, unless they leave half of the CUs idle while there are tokens
   // to share out
   p.dw_seg = dw_tiles < kCus && n >= 512;
-  p.dw_blocks = p.dw_seg ? kCus * wt.per_cu : (int)dw_tiles;
+  p.dw_blocks = p.dw_seg ? kCus * wt.per_cu : blocks_of(p.dw_tile, dw_tiles);
   p.dw_segs = p.dw_seg ? p.dw_blocks + dw_tiles : 0;
   return p;
 }
@@ -378,8 +378,7 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
       g.seg = p.dw_seg ? reinterpret_cast<float*>(ws + at.dw) : nullptr;
       g.out = static_cast<char*>(d_weight) + v0 * p.h * p.es;
       g.out_vec = p.h % 4 == 0;
-      const int blocks =
-          p.dw_seg ? p.dw_blocks : (int)(parts(p.width, wt.bm) * parts(v1 - v0, wt.bn));
+      const int blocks = p.dw_blocks;
       ACE_TRY(Launch<T>::grad(p.dw_tile, true, g, blocks, s));
       if (p.dw_seg) {
         FinishParams f{};

@@ -227,7 +227,8 @@ struct ScoreParams {
 // The tile walk that forward and backward share: this block's units are tiles
 // (token tile, vocabulary tile), vocabulary fastest.  `fold(tt, vt, acc)` takes
 // a finished tile, `enter(tt)` and `leave(tt)` a token tile's run of them.  The
-// first step of the next tile loads while `fold` works.
+// pipeline runs on across tiles: the next one's first steps load while `fold`
+// works.
 template <class TL, class Enter, class Fold, class Leave>
 __device__ inline void walk_tiles(const ScoreParams& p, int64_t v0, int64_t v1, Enter enter,
                                   Fold fold, Leave leave) {
@@ -240,49 +241,60 @@ __device__ inline void walk_tiles(const ScoreParams& p, int64_t v0, int64_t v1, 
   const int b = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
   const int64_t u0 = spread.begin(b), u1 = spread.begin(b + 1);
   if (u0 >= u1) return;
-  char* lds = mma::lds_base();
   const int64_t row_bytes = (int64_t)p.width * sizeof(T);
   const int k = p.width;
   const int steps = (k + kStep<T> - 1) / kStep<T>;
+  int tt = (int)(u0 / vts), vt = (int)(u0 % vts);
+  // what is loaded next: step `at` of tile (to_tt, to_vt)
   typename TL::OpA a;
   typename TL::OpB bo;
   typename TL::Source sa, sb;
   sa.step = sb.step = mma::kStepBytes;
-  int tt = (int)(u0 / vts), vt = (int)(u0 % vts);
-  auto aim = [&](bool tokens) {
-    a.init(row_bytes, v0 + (int64_t)vt * TL::BM, v1);
-    sa.base = p.weight + (v0 + (int64_t)vt * TL::BM) * row_bytes;
+  int at = 0, to_tt = tt, to_vt = vt;
+  int64_t to = u0;
+  const auto aim = [&](bool tokens) {
+    a.init(row_bytes, v0 + (int64_t)to_vt * TL::BM, v1);
+    sa.base = p.weight + (v0 + (int64_t)to_vt * TL::BM) * row_bytes;
     if (tokens) {
-      bo.init(row_bytes, (int64_t)tt * TL::BN, count);
-      sb.base = p.rows + (int64_t)tt * TL::BN * row_bytes;
+      bo.init(row_bytes, (int64_t)to_tt * TL::BN, count);
+      sb.base = p.rows + (int64_t)to_tt * TL::BN * row_bytes;
     }
   };
+  const auto feed = [&](char* lds) {
+    if (at == steps) {
+      if (to + 1 >= u1) return false;
+      ++to;
+      at = 0;
+      const bool turn = ++to_vt == vts;
+      if (turn) {
+        to_vt = 0;
+        ++to_tt;
+      }
+      aim(turn);
+    }
+    TL::load(a, bo, sa, sb, at, k, lds, p.zeros);
+    ++at;
+    return true;
+  };
+  const auto simple = [&](int i, char* lds) {
+    TL::load_one(i, a, bo, sa, sb, at, lds);
+    if (i == TL::kLoads - 1) ++at;
+  };
   aim(true);
-  TL::load(a, bo, sa, sb, 0, k, lds, p.zeros);
-  int buf = 0;
+  typename TL::Pipe pipe;
+  pipe.begin(feed);
   f32x4 acc[TL::MT][TL::NT];
   enter(tt);
   for (int64_t u = u0; u < u1; ++u) {
-    const int this_tt = tt, this_vt = vt;
-    const bool more = u + 1 < u1, turn = more && vt + 1 == vts;
     TL::clear(acc);
-    for (int s = 0; s < steps; ++s) {
-      mma::landed_barrier();
-      if (s + 1 < steps) {
-        TL::load(a, bo, sa, sb, s + 1, k, lds + (buf ^ 1) * TL::kStageBytes, p.zeros);
-      } else if (more) {
-        vt = turn ? 0 : vt + 1;
-        tt += turn;
-        aim(turn);
-        TL::load(a, bo, sa, sb, 0, k, lds + (buf ^ 1) * TL::kStageBytes, p.zeros);
-      }
-      TL::step(lds + buf * TL::kStageBytes, acc);
-      buf ^= 1;
-    }
-    fold(this_tt, this_vt, acc);
-    if (turn || !more) {
-      leave(this_tt);
-      if (turn) enter(tt);
+    pipe.run(steps, TL::plain_steps(0, steps, k), simple, feed, acc);
+    fold(tt, vt, acc);
+    const bool turn = ++vt == vts;
+    if (turn || u + 1 == u1) leave(tt);
+    if (turn) {
+      vt = 0;
+      ++tt;
+      if (u + 1 < u1) enter(tt);
     }
   }
 }
@@ -525,7 +537,7 @@ struct GradParams {
 // dw (DW = true):  C[h][v] = sum over rows of rows[row][h] ds[row][v].
 // With `seg`, tiles x steps of k are spread evenly over the blocks, and each
 // block's part of a tile goes to (or is added to) a partial tile of its own,
-// which finish_kernel adds in order.  Without it a block does a whole tile.
+// which finish_kernel adds in order.  Without it whole tiles are spread.
 template <class TL, bool DW>
 __global__ __launch_bounds__(TL::kThreads) void grad_kernel(GradParams p) {
   using T = typename TL::T;
@@ -536,65 +548,92 @@ __global__ __launch_bounds__(TL::kThreads) void grad_kernel(GradParams p) {
   const int k = DW ? count : (int)p.k;
   const int mts = (int)((p.m + TL::BM - 1) / TL::BM);
   const int nts = (int)((nn + TL::BN - 1) / TL::BN);
-  const int all = (k + kStep<T> - 1) / kStep<T>;             // steps there are
-  const int ks = DW ? all : (int)((p.k_map + kStep<T> - 1) / kStep<T>);  // steps they are spread as
+  const int all = (k + kStep<T> - 1) / kStep<T>;  // steps there are
+  // steps that a tile is spread as: dh spreads every piece of the vocabulary alike
+  const int ks = !p.seg ? 1 : DW ? all : (int)((p.k_map + kStep<T> - 1) / kStep<T>);
   if (nts == 0) return;
   const int blk = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
   const mma::Spread spread{(int64_t)mts * nts * ks, (int)gridDim.x};
-  int64_t u = p.seg ? spread.begin(blk) : 0, end = p.seg ? spread.begin(blk + 1) : 1;
-  while (u < end) {
-    int tile, s0, s1;
-    if (p.seg) {
-      tile = (int)(u / ks);
-      s0 = (int)(u % ks);
-      const int64_t upto = end - (int64_t)tile * ks;
-      s1 = upto < ks ? (int)upto : ks;
-    } else {
-      tile = blk;
-      s0 = 0;
-      s1 = ks;
-    }
-    u += s1 - s0 > 0 ? s1 - s0 : 1;
-    if (s1 > all) s1 = all;
+  const int64_t begin = spread.begin(blk), end = spread.begin(blk + 1);
+
+  struct Part {  // of a tile: its place, and its steps
+    int tile, first, last;
+    int64_t m0, n0;
+  };
+  const auto part_at = [&](int64_t u) {
+    Part q;
+    q.tile = (int)(u / ks);
+    q.first = p.seg ? (int)(u % ks) : 0;
+    const int64_t upto = end - (int64_t)q.tile * ks;
+    q.last = !p.seg ? all : upto < ks ? (int)upto : ks;
     // tiles in groups of 8 along n: a group's operands are shared in L2
     constexpr int kGroup = 8;
-    const int group = tile / (kGroup * mts), first = group * kGroup;
-    const int width = nts - first < kGroup ? nts - first : kGroup;
-    const int in_group = tile - first * mts;
-    const int64_t n0 = (int64_t)(first + in_group % width) * TL::BN;
-    const int64_t m0 = (int64_t)(in_group / width) * TL::BM;
-    const int64_t seg = (int64_t)blk + tile;
-    float* part = p.seg ? p.seg + seg * (TL::BM * TL::BN) : nullptr;
-    if (p.seg && p.accumulate && s0 >= s1) continue;
-    typename TL::OpA a;
-    typename TL::OpB b;
-    a.init(p.a_stride, m0, p.m);
-    b.init(p.b_stride, n0, DW ? (nn + 16 / es - 1) / (16 / es) * (16 / es) : nn);
-    const typename TL::Source sa{p.a + m0 * es, kStep<T> * p.a_stride};
-    const typename TL::Source sb{p.b + n0 * (DW ? (int64_t)es : p.b_stride),
-                                 DW ? kStep<T> * p.b_stride : mma::kStepBytes};
+    const int group = q.tile / (kGroup * mts), start = group * kGroup;
+    const int width = nts - start < kGroup ? nts - start : kGroup;
+    const int in_group = q.tile - start * mts;
+    q.n0 = (int64_t)(start + in_group % width) * TL::BN;
+    q.m0 = (int64_t)(in_group / width) * TL::BM;
+    return q;
+  };
+  const auto units = [&](const Part& q) { return p.seg ? q.last - q.first : 1; };
+
+  typename TL::OpA a;
+  typename TL::OpB b;
+  typename TL::Source sa, sb;
+  sa.step = kStep<T> * p.a_stride;
+  sb.step = DW ? kStep<T> * p.b_stride : mma::kStepBytes;
+  int64_t to = begin;  // what is loaded next: steps at..upto-1 of the part at `to`
+  int at = 0, upto = 0;
+  const auto feed = [&](char* lds) {
+    while (at >= upto) {
+      if (to >= end) return false;
+      const Part q = part_at(to);
+      to += units(q);
+      at = q.first;
+      upto = q.last < all ? q.last : all;
+      if (at >= upto) continue;
+      a.init(p.a_stride, q.m0, p.m);
+      b.init(p.b_stride, q.n0, DW ? (nn + 16 / es - 1) / (16 / es) * (16 / es) : nn);
+      sa.base = p.a + q.m0 * es;
+      sb.base = p.b + q.n0 * (DW ? (int64_t)es : p.b_stride);
+    }
+    TL::load(a, b, sa, sb, at, k, lds, p.zeros);
+    ++at;
+    return true;
+  };
+  const auto simple = [&](int i, char* lds) {
+    TL::load_one(i, a, b, sa, sb, at, lds);
+    if (i == TL::kLoads - 1) ++at;
+  };
+  typename TL::Pipe pipe;
+  pipe.begin(feed);
+  for (int64_t u = begin; u < end;) {
+    const Part q = part_at(u);
+    u += units(q);
+    const int first = q.first, last = q.last < all ? q.last : all;
+    float* part = p.seg ? p.seg + ((int64_t)blk + q.tile) * (TL::BM * TL::BN) : nullptr;
+    const auto place = [&](int i, int j) {
+      return reinterpret_cast<f32x4*>(part + (TL::wave_n() + 16 * j + col) * TL::BM + TL::wave_m() +
+                                      16 * i + 4 * g);
+    };
     f32x4 acc[MT][NT];
     TL::clear(acc);
-    __syncthreads();  // the tile before is done with LDS
-    TL::product(a, b, sa, sb, s0, s1, k, p.zeros, acc);
+    if (first < last) pipe.run(last - first, TL::plain_steps(first, last, k), simple, feed, acc);
     if (p.seg) {
+      if (p.accumulate && first >= last) continue;
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          f32x4* at = reinterpret_cast<f32x4*>(part + (TL::wave_n() + 16 * j + col) * TL::BM +
-                                               TL::wave_m() + 16 * i + 4 * g);
-          *at = p.accumulate ? *at + acc[i][j] : acc[i][j];
-        }
+        for (int i = 0; i < MT; ++i) *place(i, j) = p.accumulate ? *place(i, j) + acc[i][j] : acc[i][j];
     } else {
       const float inv = p.scale ? 1.f / *p.scale : 1.f;
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int64_t n = n0 + TL::wave_n() + 16 * j + col;
+        const int64_t n = q.n0 + TL::wave_n() + 16 * j + col;
         if (n >= nn) continue;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const int64_t m = m0 + TL::wave_m() + 16 * i + 4 * g;
+          const int64_t m = q.m0 + TL::wave_m() + 16 * i + 4 * g;
           store4(static_cast<T*>(p.out) + n * p.out_stride + m, acc[i][j] * inv, p.out_stride - m,
                  p.out_vec);
         }
