@@ -249,6 +249,8 @@ struct Tile {
   static constexpr int kStageBytes = (BM + BN) * kStepBytes;
   static constexpr int kLdsBytes = kRing * kStageBytes;
   static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "whole pieces");
+  // waves a SIMD that the registers must allow: two, or as many blocks as LDS holds
+  static constexpr int kWaves = kThreads == 512 || BN >= 128 ? 2 : 3;
   static constexpr bool kAsm = sizeof(T) == 2 && !(AKC_ && BKC_);  // transposing reads
   using OpA = Operand<T, BM, AKC_, kThreads, kAsm>;
   using OpB = Operand<T, BN, BKC_, kThreads, kAsm>;
@@ -418,20 +420,38 @@ struct Tile {
   }
 };
 
-// Work of a kernel in `total` equal units spread evenly over `blocks` blocks:
-// block b does units [begin(b), begin(b + 1)).  Units are dealt in order, so a
-// block's units are neighbours; consecutive launch indices go to the 8 XCDs in
-// turn, and `order` gives each XCD a run of neighbouring blocks, which then share
-// its L2.
-struct Spread {
-  int64_t total;
-  int blocks;
-  __device__ int64_t begin(int b) const { return b * total / blocks; }
-  __device__ int owner(int64_t unit) const {
-    return (int)(((unit + 1) * blocks - 1) / total);
-  }
+// How work of `tiles` tiles, each `units` long, is dealt to `blocks` blocks: every
+// tile is cut into `splits` equal parts, and block b takes parts b, b + blocks,
+// and so on.  Whole tiles would leave blocks idle in the last round (or in the
+// only one); cutting costs each part `overhead` units (its own start, and a partial
+// result that is written and read once more).  At most `rounds` rounds, unless
+// the whole tiles need more.
+struct Deal {
+  int tiles, splits;
+  __device__ int parts() const { return tiles * splits; }
 };
 
+__device__ inline Deal deal(int tiles, int units, int blocks, int overhead, int rounds) {
+  Deal d{tiles, 1};
+  const auto cost = [&](int s) {
+    return (int64_t)((tiles * (int64_t)s + blocks - 1) / blocks) * ((units + s - 1) / s + overhead);
+  };
+  int64_t best = cost(1);
+  for (int r = 1; r <= rounds; ++r) {
+    int64_t s = (int64_t)r * blocks / (tiles > 0 ? tiles : 1);
+    if (s > units) s = units;
+    if (s <= 1) continue;
+    const int64_t c = cost((int)s);
+    if (c < best) {
+      best = c;
+      d.splits = (int)s;
+    }
+  }
+  return d;
+}
+
+// Consecutive launch indices go to the 8 XCDs in turn: this numbers the blocks so
+// that each XCD has a run of neighbours, which share its L2.
 __device__ inline int xcd_order(int b, int blocks) {
   const int x = b & 7, base = blocks >> 3, rest = blocks & 7;
   return x * base + (x < rest ? x : rest) + (b >> 3);

@@ -50,24 +50,22 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
   const int count = *p.saved.count;
   const int tts = (count + p.bn - 1) / p.bn;
   const int64_t vts = (p.vocab + p.bm - 1) / p.bm;
-  const mma::Spread spread{tts * vts, p.score_blocks};
+  const mma::Deal d = score_deal(tts, (int)vts, p.score_blocks);
   const int per = (count + (int)gridDim.x * 4 - 1) / ((int)gridDim.x * 4);
   const int first = ((int)blockIdx.x * 4 + wave) * per;
   const int last = first + per < count ? first + per : count;
   double total = 0.0;
   for (int r = first; r < last; ++r) {
     const int tt = r / p.bn;
-    const int b0 = spread.owner(tt * vts), b1 = spread.owner((tt + 1) * vts - 1);
     float top = -FLT_MAX, sum = 0.f;
     int best = kNone;
-    for (int b = b0 + lane; b <= b1; b += 64) {
-      if (spread.begin(b) >= spread.begin(b + 1)) continue;  // a block without work wrote nothing
-      const Part q = p.part[((int64_t)b + tt) * p.bn + r % p.bn];
+    for (int s = lane; s < d.splits; s += 64) {
+      const Part q = p.part[((int64_t)tt * d.splits + s) * p.bn + r % p.bn];
       join(top, sum, best, q.top, q.sum, q.best);
     }
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2)
-      join(top, sum, best, __shfl_xor(top, d), __shfl_xor(sum, d), __shfl_xor(best, d));
+    for (int x = 1; x < 64; x *= 2)
+      join(top, sum, best, __shfl_xor(top, x), __shfl_xor(sum, x), __shfl_xor(best, x));
     if (lane == 0) {
       // log(sum) and top - label apart: a confident token's nll keeps its digits
       const float nll = logf(sum) + (top - p.label_logit[r]);
@@ -126,6 +124,12 @@ int pick_tile(int64_t m, int64_t n) {
   return parts(m, 256) * parts(n, 256) >= kCus ? kTile256 : kTile128;
 }
 
+// Most parts that mma::deal makes of at most `tiles` tiles.
+int64_t parts_of(int blocks, int rounds, int64_t tiles) {
+  const int64_t cut = (int64_t)blocks * rounds;
+  return tiles > cut ? tiles : cut;
+}
+
 struct Cursor {  // lays out a workspace
   size_t at = 0;
   size_t take(size_t bytes) {
@@ -178,8 +182,8 @@ Plan make_plan(int dtype, int64_t n, int64_t h, int64_t v) {
   if (p.dh_tile == kTile128 && n > 128 && n * p.width >= (int64_t)1 << 22) p.dh_tile = kTile256;
   const TileShape ht = kShape[p.dh_tile];
   const int64_t dh_tiles = parts(p.width, ht.bm) * parts(n, ht.bn);
-  p.dh_blocks = blocks_of(p.dh_tile, dh_tiles * parts(p.piece, 128 / p.es));
-  p.dh_segs = p.dh_blocks + dh_tiles;
+  p.dh_blocks = blocks_of(p.dh_tile, dh_tiles * parts(p.piece, mma::kStepBytes / p.es));
+  p.dh_segs = parts_of(p.dh_blocks, kGradRounds, dh_tiles);
   p.dw_tile = parts(p.width, 256) * parts(p.piece, 256) >= kCus ? kTile256 : kTile128;
   const TileShape wt = kShape[p.dw_tile];
   const int64_t dw_tiles = parts(p.width, wt.bm) * parts(p.piece, wt.bn);
@@ -187,7 +191,7 @@ Plan make_plan(int dtype, int64_t n, int64_t h, int64_t v) {
   // to share out
   p.dw_seg = dw_tiles < kCus && n >= 512;
   p.dw_blocks = p.dw_seg ? kCus * wt.per_cu : blocks_of(p.dw_tile, dw_tiles);
-  p.dw_segs = p.dw_seg ? p.dw_blocks + dw_tiles : 0;
+  p.dw_segs = p.dw_seg ? parts_of(p.dw_blocks, kGradRounds, dw_tiles) : 0;
   return p;
 }
 
@@ -202,7 +206,8 @@ ForwardSpace forward_space(const Plan& p) {
   s.ticket = c.take(4);
   s.sums = c.take((size_t)p.join_blocks * 8);
   s.label_logit = c.take((size_t)p.n * 4);
-  s.part = c.take((size_t)(p.score_blocks + parts(p.n, st.bn)) * st.bn * sizeof(Part));
+  const size_t score_parts = parts_of(p.score_blocks, kScoreRounds, parts(p.n, st.bn));
+  s.part = c.take(score_parts * st.bn * sizeof(Part));
   s.rows = c.take((size_t)(p.n * p.width) * p.es);
   s.weight = c.take(p.pad ? (size_t)(p.v * p.width) * p.es : 0);
   s.bytes = c.at;
@@ -317,7 +322,6 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
              void* d_hidden, void* d_weight, char* ws, hipStream_t s) {
   const BackwardSpace at = backward_space(p);
   const bool f16 = __is_same(T, _Float16);
-  const int step = kStep<T>;
   UpstreamParams q{};
   q.copy.hidden = hidden;
   q.copy.rows = ws + at.rows;
@@ -389,7 +393,6 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
         f.hidden_size = p.h;
         f.bm = wt.bm;
         f.bn = wt.bn;
-        f.step = step;
         f.grad_blocks = blocks;
         f.out = g.out;
         f.out_vec = g.out_vec;
@@ -417,7 +420,6 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
         f.hidden_size = p.h;
         f.bm = ht.bm;
         f.bn = ht.bn;
-        f.step = step;
         f.grad_blocks = p.dh_blocks;
         f.out = d_hidden;
         f.out_vec = p.h % 4 == 0;

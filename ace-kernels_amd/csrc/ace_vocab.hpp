@@ -210,7 +210,7 @@ struct ScoreParams {
   Saved saved;
   const char* zeros;
   // forward
-  Part* part;          // [blocks + token tiles][BN]
+  Part* part;          // [parts][BN]
   float* label_logit;  // row -> s_ty
   // backward
   int64_t v0;          // first word of this piece
@@ -224,11 +224,18 @@ struct ScoreParams {
   float* scale;        // float16: the power of two that ds is multiplied by (out)
 };
 
-// The tile walk that forward and backward share: this block's units are tiles
-// (token tile, vocabulary tile), vocabulary fastest.  `fold(tt, vt, acc)` takes
-// a finished tile, `enter(tt)` and `leave(tt)` a token tile's run of them.  The
-// pipeline runs on across tiles: the next one's first steps load while `fold`
-// works.
+// How the score kernels deal (token tile) x (vocabulary tiles): part s of a token
+// tile has the vocabulary tiles s, s + splits, ..., so that all blocks of an XCD
+// walk the same few vocabulary tiles at a time.  A part costs about a quarter of a
+// tile more.
+constexpr int kScoreRounds = 4;
+__device__ inline mma::Deal score_deal(int tts, int vts, int blocks) {
+  return mma::deal(tts, vts, blocks, 0, kScoreRounds);
+}
+
+// The tile walk that forward and backward share: `fold(tt, vt, acc)` takes a
+// finished tile, `enter(tt)` and `leave(part)` a part's run of them.  The pipeline
+// runs on across tiles: the next one's first steps load while `fold` works.
 template <class TL, class Enter, class Fold, class Leave>
 __device__ inline void walk_tiles(const ScoreParams& p, int64_t v0, int64_t v1, Enter enter,
                                   Fold fold, Leave leave) {
@@ -237,40 +244,34 @@ __device__ inline void walk_tiles(const ScoreParams& p, int64_t v0, int64_t v1, 
   const int tts = (count + TL::BN - 1) / TL::BN;
   const int vts = (int)((v1 - v0 + TL::BM - 1) / TL::BM);
   if (tts == 0) return;
-  const mma::Spread spread{(int64_t)tts * vts, (int)gridDim.x};
-  const int b = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const int64_t u0 = spread.begin(b), u1 = spread.begin(b + 1);
-  if (u0 >= u1) return;
+  const int blocks = (int)gridDim.x;
+  const mma::Deal d = score_deal(tts, vts, blocks);
+  const int first = mma::xcd_order((int)blockIdx.x, blocks);
   const int64_t row_bytes = (int64_t)p.width * sizeof(T);
   const int k = p.width;
   const int steps = (k + kStep<T> - 1) / kStep<T>;
-  int tt = (int)(u0 / vts), vt = (int)(u0 % vts);
-  // what is loaded next: step `at` of tile (to_tt, to_vt)
+  // what is loaded next: step `at` of vocabulary tile `to_vt` of part `to`
   typename TL::OpA a;
   typename TL::OpB bo;
   typename TL::Source sa, sb;
   sa.step = sb.step = mma::kStepBytes;
-  int at = 0, to_tt = tt, to_vt = vt;
-  int64_t to = u0;
-  const auto aim = [&](bool tokens) {
-    a.init(row_bytes, v0 + (int64_t)to_vt * TL::BM, v1);
-    sa.base = p.weight + (v0 + (int64_t)to_vt * TL::BM) * row_bytes;
-    if (tokens) {
-      bo.init(row_bytes, (int64_t)to_tt * TL::BN, count);
-      sb.base = p.rows + (int64_t)to_tt * TL::BN * row_bytes;
-    }
-  };
+  int at = steps, to = first - blocks, to_vt = vts;
   const auto feed = [&](char* lds) {
     if (at == steps) {
-      if (to + 1 >= u1) return false;
-      ++to;
-      at = 0;
-      const bool turn = ++to_vt == vts;
+      to_vt += d.splits;
+      const bool turn = to_vt >= vts;
       if (turn) {
-        to_vt = 0;
-        ++to_tt;
+        if (to + blocks >= d.parts()) return false;
+        to += blocks;
+        to_vt = to % d.splits;
+        const int tt = to / d.splits;
+        bo.init(row_bytes, (int64_t)tt * TL::BN, count);
+        sb.base = p.rows + (int64_t)tt * TL::BN * row_bytes;
       }
-      aim(turn);
+      const int64_t v = v0 + (int64_t)to_vt * TL::BM;
+      a.init(row_bytes, v, v1);
+      sa.base = p.weight + v * row_bytes;
+      at = 0;
     }
     TL::load(a, bo, sa, sb, at, k, lds, p.zeros);
     ++at;
@@ -280,27 +281,23 @@ __device__ inline void walk_tiles(const ScoreParams& p, int64_t v0, int64_t v1, 
     TL::load_one(i, a, bo, sa, sb, at, lds);
     if (i == TL::kLoads - 1) ++at;
   };
-  aim(true);
   typename TL::Pipe pipe;
   pipe.begin(feed);
   f32x4 acc[TL::MT][TL::NT];
-  enter(tt);
-  for (int64_t u = u0; u < u1; ++u) {
-    TL::clear(acc);
-    pipe.run(steps, TL::plain_steps(0, steps, k), simple, feed, acc);
-    fold(tt, vt, acc);
-    const bool turn = ++vt == vts;
-    if (turn || u + 1 == u1) leave(tt);
-    if (turn) {
-      vt = 0;
-      ++tt;
-      if (u + 1 < u1) enter(tt);
+  for (int part = first; part < d.parts(); part += blocks) {
+    const int tt = part / d.splits;
+    enter(tt);
+    for (int vt = part % d.splits; vt < vts; vt += d.splits) {
+      TL::clear(acc);
+      pipe.run(steps, TL::plain_steps(0, steps, k), simple, feed, acc);
+      fold(tt, vt, acc);
     }
+    leave(part);
   }
 }
 
 template <class TL>
-__global__ __launch_bounds__(TL::kThreads) void score_kernel(ScoreParams p) {
+__global__ __launch_bounds__(TL::kThreads, TL::kWaves) void score_kernel(ScoreParams p) {
   constexpr int NT = TL::NT, MT = TL::MT;
   __shared__ Part s_part[TL::WM][TL::BN];
   const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -370,8 +367,7 @@ __global__ __launch_bounds__(TL::kThreads) void score_kernel(ScoreParams p) {
       top[j] = t;
     }
   };
-  const int blk = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
-  auto leave = [&](int tt) {
+  auto leave = [&](int part) {
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
 #pragma unroll
@@ -388,7 +384,7 @@ __global__ __launch_bounds__(TL::kThreads) void score_kernel(ScoreParams p) {
 #pragma unroll
       for (int w = 1; w < TL::WM; ++w)
         join(q.top, q.sum, q.best, s_part[w][c].top, s_part[w][c].sum, s_part[w][c].best);
-      p.part[((int64_t)blk + tt) * TL::BN + c] = q;
+      p.part[(int64_t)part * TL::BN + c] = q;
     }
     __syncthreads();
   };
@@ -458,7 +454,7 @@ __device__ inline float scale_of(float bound) {
 }
 
 template <class TL>
-__global__ __launch_bounds__(TL::kThreads) void dscore_kernel(ScoreParams p) {
+__global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreParams p) {
   using T = typename TL::T;
   constexpr int NT = TL::NT, MT = TL::MT;
   const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
@@ -523,9 +519,9 @@ struct GradParams {
   int64_t m;            // hidden size rounded up to 16 bytes
   int64_t n;            // words of the piece (dw), unused for dh
   int64_t k;            // words of the piece (dh), unused for dw
-  int64_t k_map;        // dh: words of a whole piece: every piece is spread alike
+  int64_t k_map;        // dh: words of a whole piece: every piece is cut alike
   int accumulate;       // dh: not the first piece
-  float* seg;           // partial tiles [blocks + tiles][BN][BM], or null: store `out`
+  float* seg;           // partial tiles [parts][BN][BM], or null: store `out`
   void* out;            // [n, out_stride]
   int64_t out_stride;   // elements: the hidden size
   int out_vec;          // rows of `out` are whole aligned groups of four
@@ -533,13 +529,19 @@ struct GradParams {
   const char* zeros;
 };
 
+// A part of a tile costs its partial tile's way to memory and back: about as long
+// as this many steps of k.
+template <typename T>
+constexpr int kPartSteps = sizeof(T) == 2 ? 24 : 8;
+constexpr int kGradRounds = 2;
+
 // dh (DW = false): C[h][row] = sum over words of w[v][h] ds[row][v];
 // dw (DW = true):  C[h][v] = sum over rows of rows[row][h] ds[row][v].
-// With `seg`, tiles x steps of k are spread evenly over the blocks, and each
-// block's part of a tile goes to (or is added to) a partial tile of its own,
-// which finish_kernel adds in order.  Without it whole tiles are spread.
+// With `seg`, tiles are cut along k where that fills the CUs better, and each
+// part's sum goes to (or is added to) a partial tile of its own, which
+// finish_kernel adds in order.  Without it blocks take whole tiles.
 template <class TL, bool DW>
-__global__ __launch_bounds__(TL::kThreads) void grad_kernel(GradParams p) {
+__global__ __launch_bounds__(TL::kThreads, TL::kWaves) void grad_kernel(GradParams p) {
   using T = typename TL::T;
   constexpr int NT = TL::NT, MT = TL::MT, es = (int)sizeof(T);
   const int lane = (int)threadIdx.x & 63, col = lane & 15, g = lane >> 4;
@@ -549,48 +551,48 @@ __global__ __launch_bounds__(TL::kThreads) void grad_kernel(GradParams p) {
   const int mts = (int)((p.m + TL::BM - 1) / TL::BM);
   const int nts = (int)((nn + TL::BN - 1) / TL::BN);
   const int all = (k + kStep<T> - 1) / kStep<T>;  // steps there are
-  // steps that a tile is spread as: dh spreads every piece of the vocabulary alike
-  const int ks = !p.seg ? 1 : DW ? all : (int)((p.k_map + kStep<T> - 1) / kStep<T>);
+  // steps by which tiles are cut
+  const int ks = DW ? all : (int)((p.k_map + kStep<T> - 1) / kStep<T>);
   if (nts == 0) return;
-  const int blk = mma::xcd_order((int)blockIdx.x, (int)gridDim.x);
-  const mma::Spread spread{(int64_t)mts * nts * ks, (int)gridDim.x};
-  const int64_t begin = spread.begin(blk), end = spread.begin(blk + 1);
+  const int blocks = (int)gridDim.x;
+  const mma::Deal d = p.seg ? mma::deal(mts * nts, ks, blocks, kPartSteps<T>, kGradRounds)
+                            : mma::Deal{mts * nts, 1};
+  const int start = mma::xcd_order((int)blockIdx.x, blocks);
 
-  struct Part {  // of a tile: its place, and its steps
-    int tile, first, last;
+  struct Part {
+    int first, last;  // steps
     int64_t m0, n0;
   };
-  const auto part_at = [&](int64_t u) {
+  const auto part_at = [&](int part) {
     Part q;
-    q.tile = (int)(u / ks);
-    q.first = p.seg ? (int)(u % ks) : 0;
-    const int64_t upto = end - (int64_t)q.tile * ks;
-    q.last = !p.seg ? all : upto < ks ? (int)upto : ks;
+    const int tile = part % d.tiles, s = part / d.tiles;
+    q.first = (int)((int64_t)s * ks / d.splits);
+    q.last = (int)((int64_t)(s + 1) * ks / d.splits);
+    if (q.last > all) q.last = all;
     // tiles in groups of 8 along n: a group's operands are shared in L2
     constexpr int kGroup = 8;
-    const int group = q.tile / (kGroup * mts), start = group * kGroup;
-    const int width = nts - start < kGroup ? nts - start : kGroup;
-    const int in_group = q.tile - start * mts;
-    q.n0 = (int64_t)(start + in_group % width) * TL::BN;
+    const int group = tile / (kGroup * mts), from = group * kGroup;
+    const int width = nts - from < kGroup ? nts - from : kGroup;
+    const int in_group = tile - from * mts;
+    q.n0 = (int64_t)(from + in_group % width) * TL::BN;
     q.m0 = (int64_t)(in_group / width) * TL::BM;
     return q;
   };
-  const auto units = [&](const Part& q) { return p.seg ? q.last - q.first : 1; };
 
   typename TL::OpA a;
   typename TL::OpB b;
   typename TL::Source sa, sb;
   sa.step = kStep<T> * p.a_stride;
   sb.step = DW ? kStep<T> * p.b_stride : mma::kStepBytes;
-  int64_t to = begin;  // what is loaded next: steps at..upto-1 of the part at `to`
+  int to = start;  // what is loaded next: steps at..upto-1 of the part before `to`
   int at = 0, upto = 0;
   const auto feed = [&](char* lds) {
     while (at >= upto) {
-      if (to >= end) return false;
+      if (to >= d.parts()) return false;
       const Part q = part_at(to);
-      to += units(q);
+      to += blocks;
       at = q.first;
-      upto = q.last < all ? q.last : all;
+      upto = q.last;
       if (at >= upto) continue;
       a.init(p.a_stride, q.m0, p.m);
       b.init(p.b_stride, q.n0, DW ? (nn + 16 / es - 1) / (16 / es) * (16 / es) : nn);
@@ -607,11 +609,10 @@ __global__ __launch_bounds__(TL::kThreads) void grad_kernel(GradParams p) {
   };
   typename TL::Pipe pipe;
   pipe.begin(feed);
-  for (int64_t u = begin; u < end;) {
-    const Part q = part_at(u);
-    u += units(q);
-    const int first = q.first, last = q.last < all ? q.last : all;
-    float* part = p.seg ? p.seg + ((int64_t)blk + q.tile) * (TL::BM * TL::BN) : nullptr;
+  for (int index = start; index < d.parts(); index += blocks) {
+    const Part q = part_at(index);
+    const int first = q.first, last = q.last;
+    float* part = p.seg ? p.seg + (int64_t)index * (TL::BM * TL::BN) : nullptr;
     const auto place = [&](int i, int j) {
       return reinterpret_cast<f32x4*>(part + (TL::wave_n() + 16 * j + col) * TL::BM + TL::wave_m() +
                                       16 * i + 4 * g);
@@ -650,7 +651,7 @@ struct FinishParams {
   int64_t n;          // dw: words
   int64_t k_map;      // dh: words of a whole piece
   int64_t m, hidden_size;
-  int bm, bn, step, grad_blocks;
+  int bm, bn, grad_blocks;
   void* out;
   int out_vec;
   const float* scale;
@@ -663,10 +664,11 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
   const int64_t nn = DW ? p.n : count;
   const int k = DW ? count : (int)p.k_map;
   const int mts = (int)((p.m + p.bm - 1) / p.bm), nts = (int)((nn + p.bn - 1) / p.bn);
-  const int ks = (k + p.step - 1) / p.step;
-  const mma::Spread spread{(int64_t)mts * nts * ks, p.grad_blocks};
+  const int ks = (k + kStep<T> - 1) / kStep<T>;
+  const mma::Deal d = mma::deal(mts * nts, ks, p.grad_blocks, kPartSteps<T>, kGradRounds);
   const float inv = p.scale ? 1.f / *p.scale : 1.f;
   const int64_t quads = (p.hidden_size + 3) / 4;
+  const int64_t stride = (int64_t)d.tiles * p.bm * p.bn;  // from a split to the next
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.out_rows * quads;
        i += (int64_t)gridDim.x * 256) {
     const int64_t o = i / quads, m = i % quads * 4;
@@ -674,14 +676,18 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
     f32x4 sum{0.f, 0.f, 0.f, 0.f};
     if (n >= 0 && ks > 0) {
       constexpr int kGroup = 8;
-      const int nt = (int)(n / p.bn), mt = (int)(m / p.bm), first = nt / kGroup * kGroup;
-      const int width = nts - first < kGroup ? nts - first : kGroup;
-      const int64_t tile = (int64_t)first * mts + mt * width + (nt - first);
-      const int b0 = spread.owner(tile * ks), b1 = spread.owner((tile + 1) * ks - 1);
-      for (int b = b0; b <= b1; ++b) {
-        if (spread.begin(b) >= spread.begin(b + 1)) continue;
-        sum += *reinterpret_cast<const f32x4*>(p.seg + (b + tile) * p.bm * p.bn +
-                                               (n % p.bn) * p.bm + m % p.bm);
+      const int nt = (int)(n / p.bn), mt = (int)(m / p.bm), from = nt / kGroup * kGroup;
+      const int width = nts - from < kGroup ? nts - from : kGroup;
+      const int64_t tile = (int64_t)from * mts + mt * width + (nt - from);
+      const float* at = p.seg + tile * p.bm * p.bn + (n % p.bn) * p.bm + m % p.bm;
+      for (int s0 = 0; s0 < d.splits; s0 += 8) {
+        f32x4 x[8];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+          x[s] = s0 + s < d.splits ? *reinterpret_cast<const f32x4*>(at + (s0 + s) * stride)
+                                   : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < 8; ++s) sum += x[s];
       }
     }
     store4(static_cast<T*>(p.out) + o * p.hidden_size + m, sum * inv, p.hidden_size - m, p.out_vec);
