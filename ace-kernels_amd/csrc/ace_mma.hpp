@@ -98,7 +98,10 @@ __device__ inline void landed_barrier() {
 }
 
 // One operand's side of a tile: R rows (free index) by one step of k.
-template <typename T, int R, bool KC, int THREADS, bool ASM>
+// PAIRED: fragments come in pairs of 32 rows, in which the first has rows
+// 8 q + 0..3 and the second 8 q + 4..7 (q = 0..3), so that a lane's eight values of
+// the pair are neighbours in C.
+template <typename T, int R, bool KC, int THREADS, bool ASM, bool PAIRED = false>
 struct Operand {
   static constexpr int kBytes = R * kStepBytes;
   static constexpr int kChunks = KC ? kStepBytes / 16 : R * (int)sizeof(T) / 16;  // per LDS row
@@ -110,8 +113,8 @@ struct Operand {
   __device__ static int swizzle(int row, int c) {
     if constexpr (KC) {
       // a cycle of 16-byte reads serves lanes l..l+7 and l+16..l+23: eight rows,
-      // two neighbouring chunks of each
-      return c ^ ((row >> 1) & 2);
+      // two neighbouring chunks of each; rows 4 (paired: 8) apart share banks
+      return c ^ ((row >> (PAIRED ? 2 : 1)) & 2);
     } else if constexpr (sizeof(T) == 2) {
       // units of 16 columns: the 16 rows of one transposing read are
       // 8 g + j (+ 4), g and j in 0..3
@@ -185,25 +188,27 @@ struct Frag<float> {
   f32x4 v;
 };
 
-// The fragment of the 16 rows that begin at `row`.
-template <typename T, int R, bool KC>
-__device__ inline Frag<T> read_frag(const char* lds, int row) {
-  using Op = Operand<T, R, KC, 64, false>;
+// Fragment i of the rows that begin at `row`.
+template <typename T, int R, bool KC, bool PAIRED = false>
+__device__ inline Frag<T> read_frag(const char* lds, int row, int i) {
+  static_assert(KC || !PAIRED, "pairs: k contiguous only");
+  using Op = Operand<T, R, KC, 64, false, PAIRED>;
+  if constexpr (!PAIRED) row += 16 * i;
   const int lane = (int)threadIdx.x & 63;
   const int n = lane & 15, g = lane >> 4;
   Frag<T> f;
   if constexpr (KC) {
-    const int r = row + n;
+    const int r = PAIRED ? row + 32 * (i >> 1) + 8 * (n >> 2) + 4 * (i & 1) + (n & 3) : row + n;
     const char* at = lds + r * kStepBytes + Op::swizzle(r, g) * 16;
     f.v = *reinterpret_cast<const decltype(f.v)*>(at);
   } else if constexpr (sizeof(T) == 2) {
     s16x4 h[2];
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int k = 8 * g + 4 * i + (n >> 2);  // the lane's row of the 4 x 16 block
+    for (int half = 0; half < 2; ++half) {
+      const int k = 8 * g + 4 * half + (n >> 2);  // the lane's row of the 4 x 16 block
       const char* at =
           lds + k * (R * 2) + Op::swizzle(k, row / 8 + ((n >> 1) & 1)) * 16 + (n & 1) * 8;
-      h[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(at));
     }
     f.v = __builtin_shufflevector(h[0], h[1], 0, 1, 2, 3, 4, 5, 6, 7);
@@ -240,7 +245,8 @@ __device__ inline f32x4 multiply<float>(Frag<float> a, Frag<float> b, f32x4 c) {
 }
 
 // A BM x BN tile by WM x WN waves.
-template <typename T_, int BM_, int BN_, int WM_, int WN_, bool AKC_, bool BKC_>
+template <typename T_, int BM_, int BN_, int WM_, int WN_, bool AKC_, bool BKC_,
+          bool PAIRED_ = false>
 struct Tile {
   using T = T_;
   static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;
@@ -252,7 +258,8 @@ struct Tile {
   // waves a SIMD that the registers must allow: two, or as many blocks as LDS holds
   static constexpr int kWaves = kThreads == 512 || BN >= 128 ? 2 : 3;
   static constexpr bool kAsm = sizeof(T) == 2 && !(AKC_ && BKC_);  // transposing reads
-  using OpA = Operand<T, BM, AKC_, kThreads, kAsm>;
+  static constexpr bool kPaired = PAIRED_;  // the first operand's fragments
+  using OpA = Operand<T, BM, AKC_, kThreads, kAsm, PAIRED_>;
   using OpB = Operand<T, BN, BKC_, kThreads, kAsm>;
 
   // What one operand needs of memory: its address at the tile's first free
@@ -302,9 +309,9 @@ struct Tile {
 #pragma unroll
     for (int i = first; i < last; ++i) {
       if (i < NT)
-        f.b[i] = read_frag<T, BN, BKC_>(lds + OpA::kBytes, n0 + 16 * i);
+        f.b[i] = read_frag<T, BN, BKC_>(lds + OpA::kBytes, n0, i);
       else
-        f.a[i - NT] = read_frag<T, BM, AKC_>(lds, m0 + 16 * (i - NT));
+        f.a[i - NT] = read_frag<T, BM, AKC_, PAIRED_>(lds, m0, i - NT);
     }
   }
 

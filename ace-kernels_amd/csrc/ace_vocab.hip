@@ -296,6 +296,7 @@ int forward(const Plan& p, const void* hidden, const void* weight, const int64_t
     r.zeros = q.zeros;
     r.part = reinterpret_cast<Part*>(ws + at.part);
     r.label_logit = reinterpret_cast<float*>(ws + at.label_logit);
+    r.want_best = confidence || correct;
     ACE_TRY(Launch<T>::score(p.score_tile, r, p.score_blocks, s));
   }
   JoinParams j{};

@@ -81,12 +81,27 @@ __device__ inline void store4(T* at, f32x4 x, int64_t left, bool vec) {
   }
 }
 
+// Eight neighbouring values at `at` (a multiple of 16 bytes), in T.
+template <typename T>
+__device__ inline void store8(T* at, f32x4 x, f32x4 y) {
+  if constexpr (sizeof(T) == 2) {
+    typedef T Eight __attribute__((ext_vector_type(8)));
+    *reinterpret_cast<Eight*>(at) = Eight{(T)x[0], (T)x[1], (T)x[2], (T)x[3],
+                                          (T)y[0], (T)y[1], (T)y[2], (T)y[3]};
+  } else {
+    reinterpret_cast<f32x4*>(at)[0] = x;
+    reinterpret_cast<f32x4*>(at)[1] = y;
+  }
+}
+
 // A block's share of one token's softmax.
 struct Part {
   float top, sum;
   int best, pad;
 };
 
+// Both take NaN along.
+__device__ inline float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ inline float exp_of(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
 
 // (top, sum, best) of two disjoint sets of words: the larger logit, the lower
@@ -212,6 +227,7 @@ struct ScoreParams {
   // forward
   Part* part;          // [parts][BN]
   float* label_logit;  // row -> s_ty
+  int want_best;       // somebody asks for the top label
   // backward
   int64_t v0;          // first word of this piece
   int64_t v1;          // end of it
@@ -332,16 +348,16 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void score_kernel(ScorePa
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t = fmaxf(t, acc[i][j][e]);
-      if (__ballot(t > top[j])) {
+        for (int e = 0; e < 4; e += 2) t = max_of(max_of(t, acc[i][j][e]), acc[i][j][e + 1]);
+      if (p.want_best && __ballot(t > top[j])) {
         // a new largest logit somewhere in the wave: where it stands.  Words
         // come in ascending order, so the first place that has it stays.
         int at = kNone;
 #pragma unroll
         for (int i = MT - 1; i >= 0; --i)
 #pragma unroll
-          for (int e = 3; e >= 0; --e) at = acc[i][j][e] == t ? v_wave + 16 * i + 4 * g + e : at;
-        if (t > top[j]) best[j] = at;
+          for (int e = 3; e >= 0; --e) at = acc[i][j][e] == t ? 16 * i + e : at;
+        if (t > top[j]) best[j] = v_wave + 4 * g + at;
       }
       // the lane's words that the label may be among: v_wave + 4 g + 16 i + e
       const int y = label[j] - v_wave - 4 * g;
@@ -482,28 +498,46 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreP
       of_label[j] = gr;
       of_best[j] = cr;
       label[j] = in ? p.saved.label[r] : -1;
-      best[j] = in && p.c ? p.saved.best[r] : kNone;
+      best[j] = in && p.c ? p.saved.best[r] : -1;
     }
   };
+  // the lane's words of a wave's piece: of pair h, 32 h + 8 g + 0..7
+  static_assert(TL::kPaired && MT % 2 == 0, "pairs of fragments");
   auto fold = [&](int tt, int vt, f32x4(&acc)[MT][NT]) {
-    const int64_t v_tile = p.v0 + (int64_t)vt * TL::BM;
-    const int v_wave = (int)(v_tile + TL::wave_m() + 4 * g);
+    const int v_wave = (int)(p.v0 + (int64_t)vt * TL::BM + TL::wave_m());
+    const int left = (int)(p.vocab - v_wave) - 8 * g;  // words that exist from the lane's first
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[i][j][e] = of_p[j] * exp_of(acc[i][j][e] - top[j]);
+      // the two words that have more to them are rarely in the wave's piece
+      const int y = label[j] - v_wave - 8 * g, z = best[j] - v_wave - 8 * g;
+      const bool here = (y >= 0 && y < TL::BM / TL::WM && (y & 24) == 0) ||
+                        (z >= 0 && z < TL::BM / TL::WM && (z & 24) == 0);
+      if (__ballot(here)) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int w = 32 * (i >> 1) + 4 * (i & 1) + e;
+            acc[i][j][e] -= y == w ? of_label[j] : 0.f;
+            acc[i][j][e] += z == w ? of_best[j] : 0.f;
+          }
+      }
+      if (p.vocab - v_wave < TL::BM / TL::WM) {  // ragged end: words that do not exist
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (32 * (i >> 1) + 4 * (i & 1) + e >= left) acc[i][j][e] = 0.f;
+      }
       const int64_t r = (int64_t)tt * TL::BN + TL::wave_n() + 16 * j + n;
-      T* out = static_cast<T*>(p.ds) + r * p.stride + (v_wave - p.v0);
+      if (r < count) {
+        T* out = static_cast<T*>(p.ds) + r * p.stride + (v_wave + 8 * g - p.v0);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) {
-        f32x4 d;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int v = v_wave + 16 * i + e;
-          float x = of_p[j] * exp_of(acc[i][j][e] - top[j]);
-          if (v == label[j]) x -= of_label[j];
-          if (v == best[j]) x += of_best[j];
-          d[e] = v < p.vocab ? x : 0.f;
-        }
-        if (r < count) store4(out + 16 * i, d, 4, true);
+        for (int h = 0; h < MT / 2; ++h) store8(out + 32 * h, acc[2 * h][j], acc[2 * h + 1][j]);
       }
     }
   };
@@ -728,13 +762,13 @@ inline hipError_t launch(void (*kern)(P), int blocks, int threads, size_t lds, h
   return hipGetLastError();
 }
 
-template <typename T, bool AKC, bool BKC, typename F>
+template <typename T, bool AKC, bool BKC, bool PAIRED = false, typename F>
 inline hipError_t with_tile(int tile, F f) {
   switch (tile) {
-    case kTile256: return f(mma::Tile<T, 256, 256, 2, 4, AKC, BKC>{});
-    case kTile128: return f(mma::Tile<T, 128, 128, 2, 2, AKC, BKC>{});
-    case kTile64: return f(mma::Tile<T, 128, 64, 4, 1, AKC, BKC>{});
-    default: return f(mma::Tile<T, 128, 32, 4, 1, AKC, BKC>{});
+    case kTile256: return f(mma::Tile<T, 256, 256, 2, 4, AKC, BKC, PAIRED>{});
+    case kTile128: return f(mma::Tile<T, 128, 128, 2, 2, AKC, BKC, PAIRED>{});
+    case kTile64: return f(mma::Tile<T, 128, 64, 4, 1, AKC, BKC, PAIRED>{});
+    default: return f(mma::Tile<T, 128, 32, 4, 1, AKC, BKC, PAIRED>{});
   }
 }
 
@@ -764,7 +798,7 @@ inline hipError_t with_tile(int tile, F f) {
   }                                                                                              \
   template <>                                                                                    \
   hipError_t Launch<T>::dscore(int tile, const ScoreParams& p, int blocks, hipStream_t s) {      \
-    return with_tile<T, true, true>(tile, [&](auto t) {                                          \
+    return with_tile<T, true, true, true>(tile, [&](auto t) {                                    \
       using TL = decltype(t);                                                                    \
       return launch(dscore_kernel<TL>, blocks, TL::kThreads, TL::kLdsBytes, s, p);               \
     });                                                                                          \
