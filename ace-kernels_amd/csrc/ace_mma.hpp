@@ -191,7 +191,7 @@ struct Frag<float> {
 // Fragment i of the rows that begin at `row`.
 template <typename T, int R, bool KC, bool PAIRED = false>
 __device__ inline Frag<T> read_frag(const char* lds, int row, int i) {
-  static_assert(KC || !PAIRED, "pairs: k contiguous only");
+  static_assert(KC || sizeof(T) == 2 || !PAIRED, "pairs: not through single floats");
   using Op = Operand<T, R, KC, 64, false, PAIRED>;
   if constexpr (!PAIRED) row += 16 * i;
   const int lane = (int)threadIdx.x & 63;
@@ -206,8 +206,9 @@ __device__ inline Frag<T> read_frag(const char* lds, int row, int i) {
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const int k = 8 * g + 4 * half + (n >> 2);  // the lane's row of the 4 x 16 block
+      const int c = PAIRED ? row / 8 + 4 * (i >> 1) + (n & 3) : row / 8 + ((n >> 1) & 1);
       const char* at =
-          lds + k * (R * 2) + Op::swizzle(k, row / 8 + ((n >> 1) & 1)) * 16 + (n & 1) * 8;
+          lds + k * (R * 2) + Op::swizzle(k, c) * 16 + (PAIRED ? i & 1 : n & 1) * 8;
       h[half] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(at));
     }

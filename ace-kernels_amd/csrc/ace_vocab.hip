@@ -114,14 +114,32 @@ int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t parts(int64_t x, int64_t of) { return (x + of - 1) / of; }
 int elem_size(int dtype) { return dtype == ACE_F32 ? 4 : 2; }
 
-// Tiles for `n` columns (tokens, or words of a piece) and `m` rows: the narrow
-// ones where the columns do not fill a wider one, the widest where there are
-// enough of them for every CU.
-int pick_tile(int64_t m, int64_t n) {
-  if (n <= 32) return kTile32;
-  if (n <= 64) return kTile64;
-  if (n <= 128) return kTile128;
-  return parts(m, 256) * parts(n, 256) >= kCus ? kTile256 : kTile128;
+// Rates of the tiles relative to each other, measured on large products: with 16
+// bits 1146, 870 and less (TFLOP/s), which small tiles lose to the traffic of LDS;
+// with float32 the matrix cores alone bound all of them.
+float rate_of(int es, int tile) {
+  constexpr float half[kTiles] = {1.2f, 0.85f, 0.65f, 0.4f}, single[kTiles] = {1.f, 1.f, 0.95f, 0.85f};
+  return es == 2 ? half[tile] : single[tile];
+}
+
+// The tile for m x n results: the one that takes the least time, counting what
+// its edges waste.  `whole`: tiles are not cut, so that a round of blocks counts
+// in full however few they are.
+int pick_tile(int es, int64_t m, int64_t n, bool whole, int first = kTile256) {
+  int best = first;
+  double least = 0.0;
+  for (int t = first; t < kTiles; ++t) {
+    const TileShape s = kShape[t];
+    const double slots = (double)kCus * s.per_cu;
+    double rounds = (double)(parts(m, s.bm) * parts(n, s.bn)) / slots;
+    if (whole) rounds = (double)(int64_t)(rounds + 1.0 - 1e-9);
+    const double cost = rounds * s.per_cu * s.bm * s.bn / rate_of(es, t);
+    if (t == first || cost < least) {
+      best = t;
+      least = cost;
+    }
+  }
+  return best;
 }
 
 // Most parts that mma::deal makes of at most `tiles` tiles.
@@ -163,7 +181,7 @@ Plan make_plan(int dtype, int64_t n, int64_t h, int64_t v) {
   p.es = elem_size(dtype);
   p.width = up(h, 16 / p.es);
   p.pad = p.width != h;
-  p.score_tile = pick_tile(v, n);
+  p.score_tile = pick_tile(p.es, v, n, true);
   const auto blocks_of = [](int tile, int64_t tiles) {
     const int64_t most = (int64_t)kCus * kShape[tile].per_cu;
     return (int)(tiles < most ? (tiles > 0 ? tiles : 1) : most);
@@ -178,18 +196,18 @@ Plan make_plan(int dtype, int64_t n, int64_t h, int64_t v) {
   if (most < 2048) most = 2048;
   p.piece = up(parts(v, parts(v, most)), 256);
   p.dscore_blocks = blocks_of(p.score_tile, parts(p.piece, st.bm) * parts(n, st.bn));
-  p.dh_tile = pick_tile(p.width, n);
-  if (p.dh_tile == kTile128 && n > 128 && n * p.width >= (int64_t)1 << 22) p.dh_tile = kTile256;
+  p.dh_tile = pick_tile(p.es, p.width, n, false);
   const TileShape ht = kShape[p.dh_tile];
   const int64_t dh_tiles = parts(p.width, ht.bm) * parts(n, ht.bn);
   p.dh_blocks = blocks_of(p.dh_tile, dh_tiles * parts(p.piece, mma::kStepBytes / p.es));
   p.dh_segs = parts_of(p.dh_blocks, kGradRounds, dh_tiles);
-  p.dw_tile = parts(p.width, 256) * parts(p.piece, 256) >= kCus ? kTile256 : kTile128;
+  // few tokens: what is written bounds it, and blocks that share a CU overlap
+  p.dw_tile = pick_tile(p.es, p.width, p.piece, true, n > 256 ? kTile256 : kTile128);
+  // the tokens are shared out as well where whole tiles leave half of the CUs idle
+  p.dw_seg = n >= 512 && parts(p.width, 128) * parts(p.piece, 128) < kCus;
+  if (p.dw_seg) p.dw_tile = kTile128;
   const TileShape wt = kShape[p.dw_tile];
   const int64_t dw_tiles = parts(p.width, wt.bm) * parts(p.piece, wt.bn);
-  // whole tiles, unless they leave half of the CUs idle while there are tokens
-  // to share out
-  p.dw_seg = dw_tiles < kCus && n >= 512;
   p.dw_blocks = p.dw_seg ? kCus * wt.per_cu : blocks_of(p.dw_tile, dw_tiles);
   p.dw_segs = p.dw_seg ? parts_of(p.dw_blocks, kGradRounds, dw_tiles) : 0;
   return p;
@@ -322,7 +340,6 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
              const void* saved, const float* grad_loss, const float* grad_confidence,
              void* d_hidden, void* d_weight, char* ws, hipStream_t s) {
   const BackwardSpace at = backward_space(p);
-  const bool f16 = __is_same(T, _Float16);
   UpstreamParams q{};
   q.copy.hidden = hidden;
   q.copy.rows = ws + at.rows;
@@ -344,7 +361,7 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
     ACE_TRY(Launch<T>::pad(weight, ws + at.weight, p.v, (int)p.h, (int)p.width, s));
     weight = ws + at.weight;
   }
-  float* scale = f16 ? reinterpret_cast<float*>(ws + at.scale) : nullptr;
+  float* scale = sizeof(T) == 2 ? reinterpret_cast<float*>(ws + at.scale) : nullptr;
   const TileShape ht = kShape[p.dh_tile], wt = kShape[p.dw_tile];
   const int64_t row_bytes = p.width * p.es;
   for (int64_t v0 = 0; v0 < p.v; v0 += p.piece) {
@@ -364,6 +381,7 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
     r.ds = ws + at.ds;
     r.g = q.g;
     r.c = q.c;
+    r.one_g = grad_loss && reduction != ACE_RED_NONE;
     r.bound = q.bound;
     r.bounds = p.prep_blocks;
     r.scale = scale;
@@ -383,6 +401,7 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
       g.seg = p.dw_seg ? reinterpret_cast<float*>(ws + at.dw) : nullptr;
       g.out = static_cast<char*>(d_weight) + v0 * p.h * p.es;
       g.out_vec = p.h % 4 == 0;
+      g.out_vec8 = p.h % 8 == 0;
       const int blocks = p.dw_blocks;
       ACE_TRY(Launch<T>::grad(p.dw_tile, true, g, blocks, s));
       if (p.dw_seg) {

@@ -235,9 +235,10 @@ struct ScoreParams {
   void* ds;            // [n, stride]
   const float* g;      // row -> upstream of nll
   const float* c;      // row -> upstream of conf, times conf; null: none
+  int one_g;           // g is the same for all rows
   const float* bound;  // float16: blocks' largest |g| + |c|, and how many
   int bounds;
-  float* scale;        // float16: the power of two that ds is multiplied by (out)
+  float* scale;        // 16 bits: what ds is multiplied by (out)
 };
 
 // How the score kernels deal (token tile) x (vocabulary tiles): part s of a token
@@ -458,9 +459,16 @@ __global__ __launch_bounds__(256) void upstream_kernel(UpstreamParams p) {
   if (tid == 0) p.bound[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
 }
 
-// float16 holds dS as dS times a power of two that takes the largest |g| + |c|,
-// dS's bound, to 2^13..2^14: without it the probabilities of a large vocabulary
-// are below float16's smallest numbers.  The other types have float32's range.
+// dS is held times a scale that its products are divided by at the end.
+// Where all tokens have the same upstream gradient (mean, sum), the scale is its
+// reciprocal, so that the label's entry, p - 1, is near a number that the type
+// holds exactly: every token's largest entry would else be rounded alike.
+// float16 takes 2^13 of that, or for other upstream gradients a power of two that
+// takes the largest |g| + |c|, dS's bound, to 2^13..2^14: without it the
+// probabilities of a large vocabulary are below float16's smallest numbers.
+template <typename T>
+constexpr float kHalfScale = __is_same(T, _Float16) ? 8192.f : 1.f;
+
 __device__ inline float scale_of(float bound) {
   if (!(bound > 0.f) || bound > FLT_MAX) return 1.f;
   int e;
@@ -476,12 +484,19 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreP
   const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int count = *p.saved.count;
   float scale = 1.f;
-  if constexpr (sizeof(T) == 2 && !__is_same(T, __bf16)) {
-    float most = 0.f;  // every wave on its own
-    for (int i = lane; i < p.bounds; i += 64) most = fmaxf(most, p.bound[i]);
+  if constexpr (sizeof(T) == 2) {
+    const float g0 = p.one_g && count > 0 ? fabsf(p.g[0]) : 0.f;
+    if (g0 >= FLT_MIN * 8192.f && g0 <= FLT_MAX / 8192.f) {
+      scale = kHalfScale<T> / g0;
+    }
+    if (__is_same(T, _Float16) && (scale == 1.f || p.c)) {
+      float most = 0.f;  // every wave on its own
+      for (int i = lane; i < p.bounds; i += 64) most = fmaxf(most, p.bound[i]);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    scale = scale_of(most);
+      for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+      // with confidences: no more than the largest |g| + |c| allows
+      if (scale == 1.f || !(most * scale <= 32768.f)) scale = scale_of(most);
+    }
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.scale = scale;
   }
   float top[NT], of_p[NT], of_label[NT], of_best[NT];
@@ -559,7 +574,8 @@ struct GradParams {
   void* out;            // [n, out_stride]
   int64_t out_stride;   // elements: the hidden size
   int out_vec;          // rows of `out` are whole aligned groups of four
-  const float* scale;   // float16
+  int out_vec8;         // and of eight
+  const float* scale;   // 16 bits
   const char* zeros;
 };
 
@@ -648,8 +664,9 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void grad_kernel(GradPara
     const int first = q.first, last = q.last;
     float* part = p.seg ? p.seg + (int64_t)index * (TL::BM * TL::BN) : nullptr;
     const auto place = [&](int i, int j) {
-      return reinterpret_cast<f32x4*>(part + (TL::wave_n() + 16 * j + col) * TL::BM + TL::wave_m() +
-                                      16 * i + 4 * g);
+      return reinterpret_cast<f32x4*>(
+          part + (TL::wave_n() + 16 * j + col) * TL::BM + TL::wave_m() +
+          (TL::kPaired ? 32 * (i >> 1) + 8 * g + 4 * (i & 1) : 16 * i + 4 * g));
     };
     f32x4 acc[MT][NT];
     TL::clear(acc);
@@ -668,9 +685,14 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void grad_kernel(GradPara
         if (n >= nn) continue;
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const int64_t m = q.m0 + TL::wave_m() + 16 * i + 4 * g;
-          store4(static_cast<T*>(p.out) + n * p.out_stride + m, acc[i][j] * inv, p.out_stride - m,
-                 p.out_vec);
+          const int64_t m = q.m0 + TL::wave_m() +
+                            (TL::kPaired ? 32 * (i >> 1) + 8 * g + 4 * (i & 1) : 16 * i + 4 * g);
+          T* at = static_cast<T*>(p.out) + n * p.out_stride + m;
+          if (TL::kPaired && p.out_vec8 && m + (i & 1 ? 4 : 8) <= p.out_stride) {
+            if (!(i & 1)) store8(at, acc[i][j] * inv, acc[i ^ 1][j] * inv);
+          } else {
+            store4(at, acc[i][j] * inv, p.out_stride - m, p.out_vec);
+          }
         }
       }
     }
@@ -806,14 +828,11 @@ inline hipError_t with_tile(int tile, F f) {
   template <>                                                                                    \
   hipError_t Launch<T>::grad(int tile, bool dw, const GradParams& p, int blocks,                 \
                              hipStream_t s) {                                                    \
-    if (dw) {                                                                                    \
-      if (tile == kTile256) {                                                                    \
-        using TL = mma::Tile<T, 256, 256, 2, 4, false, false>;                                   \
+    if (dw)                                                                                      \
+      return with_tile<T, false, false, sizeof(T) == 2>(tile, [&](auto t) {                      \
+        using TL = decltype(t);                                                                  \
         return launch(grad_kernel<TL, true>, blocks, TL::kThreads, TL::kLdsBytes, s, p);         \
-      }                                                                                          \
-      using TL = mma::Tile<T, 128, 128, 2, 2, false, false>;                                     \
-      return launch(grad_kernel<TL, true>, blocks, TL::kThreads, TL::kLdsBytes, s, p);           \
-    }                                                                                            \
+      });                                                                                        \
     return with_tile<T, false, true>(tile, [&](auto t) {                                         \
       using TL = decltype(t);                                                                    \
       return launch(grad_kernel<TL, false>, blocks, TL::kThreads, TL::kLdsBytes, s, p);          \
