@@ -8,7 +8,7 @@ namespace ace {
 namespace balance {
 namespace {
 
-constexpr int64_t kMaxTokens = (int64_t)1 << 40;
+constexpr int64_t kMaxTokens = (int64_t)1 << 30;  // counts are 32 bits on the way
 constexpr int kMaxGroups = 1 << 20;
 constexpr int kTarget = 1024;  // blocks to aim at: four on each CU
 

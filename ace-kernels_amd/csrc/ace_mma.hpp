@@ -225,24 +225,27 @@ __device__ inline Frag<T> read_frag(const char* lds, int row, int i) {
   return f;
 }
 
+// Instruction j of kParts<T> that multiply two fragments.
 template <typename T>
-__device__ inline f32x4 multiply(Frag<T> a, Frag<T> b, f32x4 c);
+constexpr int kParts = sizeof(T) == 4 ? 4 : 1;
+template <typename T>
+__device__ inline f32x4 multiply(const Frag<T>& a, const Frag<T>& b, f32x4 c, int j);
 template <>
-__device__ inline f32x4 multiply<__bf16>(Frag<__bf16> a, Frag<__bf16> b, f32x4 c) {
+__device__ inline f32x4 multiply<__bf16>(const Frag<__bf16>& a, const Frag<__bf16>& b, f32x4 c,
+                                         int) {
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a.v),
                                                  __builtin_bit_cast(bf16x8, b.v), c, 0, 0, 0);
 }
 template <>
-__device__ inline f32x4 multiply<_Float16>(Frag<_Float16> a, Frag<_Float16> b, f32x4 c) {
+__device__ inline f32x4 multiply<_Float16>(const Frag<_Float16>& a, const Frag<_Float16>& b,
+                                           f32x4 c, int) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a.v),
                                                 __builtin_bit_cast(f16x8, b.v), c, 0, 0, 0);
 }
 template <>
-__device__ inline f32x4 multiply<float>(Frag<float> a, Frag<float> b, f32x4 c) {
-#pragma unroll
-  for (int j = 0; j < 4; ++j)
-    c = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
-  return c;
+__device__ inline f32x4 multiply<float>(const Frag<float>& a, const Frag<float>& b, f32x4 c,
+                                        int j) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[j], b.v[j], c, 0, 0, 0);
 }
 
 // A BM x BN tile by WM x WN waves.
@@ -316,11 +319,15 @@ struct Tile {
     }
   }
 
+  // Neighbouring instructions add to different pieces: one that waits for the
+  // result of the one before takes longer.
   __device__ static void multiply_all(const Frags& f, f32x4 (&acc)[MT][NT]) {
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
+    for (int q = 0; q < kParts<T>; ++q)
 #pragma unroll
-      for (int j = 0; j < NT; ++j) acc[i][j] = multiply<T>(f.a[i], f.b[j], acc[i][j]);
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j] = multiply<T>(f.a[i], f.b[j], acc[i][j], q);
   }
 
   // False: this wave has no part in the last load of a step.
@@ -332,10 +339,9 @@ struct Tile {
   // Spreads a step's LDS reads (and with them the loads between them) evenly among
   // its matrix instructions, so that the matrix cores do not wait for a burst.
   __device__ static void interleave() {
-    constexpr int per = sizeof(T) == 4 ? 4 : 1;  // matrix instructions of a piece
     constexpr int reads_a = MT * (AKC_ ? 1 : sizeof(T) == 4 ? 4 : 2);
     constexpr int reads_b = NT * (BKC_ ? 1 : sizeof(T) == 4 ? 4 : 2);
-    constexpr int n = MT * NT * per, reads = reads_a + reads_b;
+    constexpr int n = MT * NT * kParts<T>, reads = reads_a + reads_b;
 #pragma unroll
     for (int i = 0; i < n; ++i) {
       __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // a matrix instruction

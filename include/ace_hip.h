@@ -269,8 +269,9 @@ int ace_forward_noalloc(const void* x, int x_dtype, const void* target,
  * aligned) is what the backward needs beside hidden and weight.
  * ace_vocab_backward: the gradients of hidden and weight, each skipped if NULL,
  * for upstream gradients of loss (one float32, or [tokens] for ACE_RED_NONE)
- * and of confidence ([tokens]); either may be NULL, for 0.  It may be called
- * any number of times on one `saved`.
+ * and of confidence ([tokens], only after a forward that was asked for
+ * confidence or correct); either may be NULL, for 0.  It may be called any
+ * number of times on one `saved`.
  *
  * The workspace (ace_vocab_workspace_bytes, backward 0 or 1, 16-byte aligned)
  * needs no clearing and holds nothing between calls; calls that overlap need
@@ -318,7 +319,7 @@ int ace_vocab_backward(const void* hidden, const void* weight, int dtype,
  * their logits are not read.  Both calls are one launch on `stream`, allocate
  * nothing and can be captured; results do not vary from run to run.  Returns
  * ACE_EINVAL, ACE_EUNSUPPORTED (experts above 512, top_k above 16, groups above
- * 2^20), ACE_EWORKSPACE or a HIP error.
+ * 2^20, tokens above 2^30), ACE_EWORKSPACE or a HIP error.
  */
 size_t ace_balance_workspace_bytes(int64_t groups, int64_t tokens,
                                    int64_t experts);

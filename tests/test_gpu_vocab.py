@@ -43,7 +43,7 @@ def _compare(hidden, weight, labels, config=VocabConfig(), go=None, gc=None):
     _within(out.loss, want.loss, tol, "loss")
     _within(out.confidence, want.confidence, want.tol_confidence * want.confidence + 1e-30, "confidence")
     assert torch.equal(out.correct[want.sure].double(), want.correct[want.sure])
-    if want.sure.all() or gc is None:
+    if want.sure.all() or gc is None:  # else the confidence's gradient may be another word's
         _within(dh, want.d_hidden, want.tol_hidden + 1e-30, "d hidden")
         _within(dw, want.d_weight, want.tol_weight + 1e-30, "d weight")
     return out, (dh, dw)
@@ -67,6 +67,31 @@ def test_sizes(n, size, v, dtype) -> None:
     go = torch.tensor(0.7, device="cuda")
     gc = (torch.randn(n, generator=gen) / n).cuda()
     _compare(hidden, weight, labels, VocabConfig(), go, gc)
+
+
+def _drawn(seed):
+    gen = torch.Generator().manual_seed(seed)
+
+    def between(low, high):
+        return int(round(low * (high / low) ** float(torch.rand((), generator=gen))))
+
+    n, size, v = between(1, 3000), between(3, 700), between(2, 9000)
+    if float(torch.rand((), generator=gen)) < 0.5:
+        size = max(8, size // 8 * 8)
+    share = [0.0, 0.3, 0.9][int(torch.randint(3, (), generator=gen))]
+    return n, size, v, [F32, BF16, F16][seed % 3], share
+
+
+@pytest.mark.parametrize("seed", range(48))
+def test_drawn_sizes(seed) -> None:
+    """Tiles, cuts of the work and edges that nobody thought of: the counted
+    tokens' number is known on the device only."""
+    n, size, v, dtype, share = _drawn(seed)
+    say(f"vocab drawn {n}x{size}x{v} {dtype} ignored {share}")
+    hidden, weight, labels = inputs(n, size, v, dtype, seed=seed, ignored=share)
+    gc = (torch.randn(n, generator=torch.Generator().manual_seed(seed)) / n).cuda() if seed % 2 else None
+    reduction = ["mean", "sum", "none"][seed // 3 % 3]
+    _compare(hidden, weight, labels, VocabConfig(reduction=reduction), None, gc)
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16, F16], ids=["f32", "bf16", "f16"])

@@ -68,7 +68,7 @@ def exact(hidden, weight, labels, ignore_index=-100, reduction="mean", grad_loss
         conf[rows] = p[here, best]
         correct[rows] = (best == yc).double()
         go = torch.ones((), **f64) if grad_loss is None else grad_loss.double()
-        g = go[rows] if reduction == "none" else go.expand(rows.numel()) / (count if reduction == "mean" else 1)
+        g = go.expand(n)[rows] if reduction == "none" else go.expand(rows.numel()) / (count if reduction == "mean" else 1)
         c = torch.zeros(rows.numel(), **f64) if grad_confidence is None else grad_confidence.double()[rows]
         c = c * conf[rows]
         ds = (g - c)[:, None] * p
