@@ -44,9 +44,10 @@ Space space(int64_t groups, int experts, const Geometry& g) {
   const size_t fans = (size_t)(g.blocks + kFan - 1) / kFan;
   const size_t sets = (size_t)(groups + kFan - 1) / kFan;
   Space s{};
-  s.loss = round((size_t)groups * (g.blocks + fans) * (size_t)(experts + 1) * 8);
+  const bool cut = g.blocks > 1;
+  s.loss = cut ? round((size_t)groups * (g.blocks + fans) * (size_t)(experts + 1) * 8) : 0;
   s.bytes = s.loss + round(((size_t)groups + sets) * 8);
-  s.ticket_bytes = ((size_t)groups * (fans + 1) + sets + 1) * kTicketStride * 4;
+  s.ticket_bytes = ((cut ? (size_t)groups * (fans + 1) : 0) + sets + 1) * kTicketStride * 4;
   return s;
 }
 

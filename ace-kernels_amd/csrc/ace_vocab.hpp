@@ -21,7 +21,17 @@
 // takes dS from the kept maximum and sum and stores it (in the inputs' type: the
 // matrix cores' operand), one forms the piece's dw, and one adds its part of dh.
 //
-// All sums, the running maxima, the logits and the partial dh are float32.
+// All sums, the running maxima, the logits and the partial dh are float32.  The one
+// rounding beside the results' own is dS's to the inputs' type, half a step of each
+// entry (2^-9 relatively in bfloat16 at most twice that): the gradients' errors
+// against 64 bits are 1.1 times those of a gradient that is only rounded at the end.
+//
+// What bounds it: the matrix cores.  8192 tokens (5 % ignored) x 4096 x 65536 words
+// in bfloat16 take 13.9 ms for four products of 4.2 TFLOP, 1.2 PFLOP/s, the rate
+// of the library's products of this size (1.1 to 1.4 PFLOP/s); the logits are
+// formed twice because they are not kept.  With few tokens it is the weight, which
+// is read three times and whose gradient is written: 96 tokens x 2048 x 50304 words
+// in float16 take 0.28 ms for 0.83 GB.
 #pragma once
 
 #include <float.h>
@@ -243,8 +253,9 @@ struct ScoreParams {
 
 // How the score kernels deal (token tile) x (vocabulary tiles): part s of a token
 // tile has the vocabulary tiles s, s + splits, ..., so that all blocks of an XCD
-// walk the same few vocabulary tiles at a time.  A part costs about a quarter of a
-// tile more.
+// walk the same few vocabulary tiles at a time (4 to 8 of them and 4 to 8 token
+// tiles): 1250 TFLOP/s at 8192 x 4096 x 65536, against 995 where each block had a
+// run of vocabulary tiles of its own.
 constexpr int kScoreRounds = 4;
 __device__ inline mma::Deal score_deal(int tts, int vts, int blocks) {
   return mma::deal(tts, vts, blocks, 0, kScoreRounds);
@@ -313,6 +324,10 @@ __device__ inline void walk_tiles(const ScoreParams& p, int64_t v0, int64_t v1, 
   }
 }
 
+// The forward: each lane keeps a running maximum and sum for each of its tokens
+// over the words that it holds, without an exchange until its part ends.  Per
+// tile of 256 x 256 the exponentials cost about 8 us of which nothing overlaps the
+// products (28 us at a hidden size of 1024, 113 us at 4096).
 template <class TL>
 __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void score_kernel(ScoreParams p) {
   constexpr int NT = TL::NT, MT = TL::MT;
@@ -477,6 +492,10 @@ __device__ inline float scale_of(float bound) {
   return ldexpf(1.f, e > 100 ? 100 : e < -100 ? -100 : e);
 }
 
+// dS of a piece.  The first operand's rows are paired (ace_mma.hpp), so that a lane
+// stores 16 bytes at a time and four lanes 64: with the label, the top label and
+// the ragged end out of the common path this took 163 us instead of 194 at 2048 x
+// 1024 x 32768.
 template <class TL>
 __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreParams p) {
   using T = typename TL::T;
@@ -589,7 +608,9 @@ constexpr int kGradRounds = 2;
 // dw (DW = true):  C[h][v] = sum over rows of rows[row][h] ds[row][v].
 // With `seg`, tiles are cut along k where that fills the CUs better, and each
 // part's sum goes to (or is added to) a partial tile of its own, which
-// finish_kernel adds in order.  Without it blocks take whole tiles.
+// finish_kernel adds in order.  Without it blocks take whole tiles.  Parts that run
+// at once are at the same place along k: 1194 TFLOP/s for dh at 8192 x 4096 x 65536,
+// against 913 with the work cut evenly wherever that fell.  dw: 1.25 PFLOP/s.
 template <class TL, bool DW>
 __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void grad_kernel(GradParams p) {
   using T = typename TL::T;

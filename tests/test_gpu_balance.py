@@ -88,7 +88,8 @@ def test_experts(experts, dtype) -> None:
 
 
 @TYPES
-@pytest.mark.parametrize("lead,tokens", [((), 1), ((3,), 1), ((2, 3), 17), ((), 4097), ((5,), 1000), ((), 100003), ((300,), 40)])
+@pytest.mark.parametrize("lead,tokens", [((), 1), ((3,), 1), ((2, 3), 17), ((), 4097), ((5,), 1000), ((), 100003), ((300,), 40),
+                                         ((33,), 2000), ((40, 40), 5)])
 def test_groups_and_lengths(lead, tokens, dtype) -> None:
     x = _scores(lead, tokens, 24, dtype, seed=tokens)
     _compare(x, 2)
