@@ -16,8 +16,8 @@
 //                 in memory.
 //
 // A step of k is 64 bytes wide (32 elements of 16 bits, 16 floats).  LDS holds a
-// ring of four steps: while the products of step s run, step s + 1 goes from LDS
-// to registers and step s + 3 from memory to LDS directly (global_load_lds, 16
+// ring of steps, four in the large tiles: while the products of step s run, step
+// s + 1 goes from LDS to registers and step s + 3 from memory to LDS directly (global_load_lds, 16
 // bytes a lane), so that neither latency is waited for; one barrier a step.  Rows
 // of LDS are swizzled in units of 16 bytes (k contiguous) or of 16 columns (m
 // contiguous), on the side of the global address because the LDS side of such a
@@ -40,8 +40,6 @@ using bf16x8 = __bf16 __attribute__((ext_vector_type(8)));
 using f16x8 = _Float16 __attribute__((ext_vector_type(8)));
 
 constexpr int kStepBytes = 64;  // bytes of k in one step
-constexpr int kRing = 4;        // steps in LDS
-constexpr int kAhead = 3;       // steps between loading one and multiplying it
 
 template <typename T>
 constexpr int kStep = kStepBytes / (int)sizeof(T);  // elements of k in one step
@@ -257,10 +255,13 @@ struct Tile {
   static constexpr int kThreads = 64 * WM * WN;
   static constexpr int MT = BM / WM / 16, NT = BN / WN / 16;  // 16 x 16 pieces of a wave
   static constexpr int kStageBytes = (BM + BN) * kStepBytes;
+  // steps in LDS, and between loading one and multiplying it: the narrowest tiles have
+  // little to do in a step, and wait for memory unless more of them are on the way
+  static constexpr int kRing = BN <= 32 ? 7 : 4, kAhead = kRing - 1;
   static constexpr int kLdsBytes = kRing * kStageBytes;
   static_assert(BM % (16 * WM) == 0 && BN % (16 * WN) == 0, "whole pieces");
   // waves a SIMD that the registers must allow: two, or as many blocks as LDS holds
-  static constexpr int kWaves = kThreads == 512 || BN >= 128 ? 2 : 3;
+  static constexpr int kWaves = BN == 64 ? 3 : 2;
   static constexpr bool kAsm = sizeof(T) == 2 && !(AKC_ && BKC_);  // transposing reads
   static constexpr bool kPaired = PAIRED_;  // the first operand's fragments
   using OpA = Operand<T, BM, AKC_, kThreads, kAsm, PAIRED_>;
@@ -438,24 +439,29 @@ struct Tile {
 // tile is cut into `splits` equal parts, and block b takes parts b, b + blocks,
 // and so on.  Whole tiles would leave blocks idle in the last round (or in the
 // only one); cutting costs each part `overhead` units (its own start, and a partial
-// result that is written and read once more).  At most `rounds` rounds, unless
-// the whole tiles need more.
+// result that is written), and a little more for each split where the results
+// are joined.  At most `rounds` rounds, unless the whole tiles need more.
 struct Deal {
   int tiles, splits;
   __device__ int parts() const { return tiles * splits; }
 };
 
+// Every block works this out for itself: 32-bit divisions only, as a 64-bit one takes
+// about a microsecond.
 __device__ inline Deal deal(int tiles, int units, int blocks, int overhead, int rounds) {
   Deal d{tiles, 1};
-  const auto cost = [&](int s) {
-    return (int64_t)((tiles * (int64_t)s + blocks - 1) / blocks) * ((units + s - 1) / s + overhead);
+  const uint32_t t = tiles > 0 ? (uint32_t)tiles : 1u, u = (uint32_t)units, n = (uint32_t)blocks;
+  const auto cost = [&](uint32_t s) {
+    return (float)((t * s + n - 1) / n) * (float)((u + s - 1) / s + (uint32_t)overhead) +
+           (overhead ? (float)s / 16.f : 0.f);
   };
-  int64_t best = cost(1);
-  for (int r = 1; r <= rounds; ++r) {
-    int64_t s = (int64_t)r * blocks / (tiles > 0 ? tiles : 1);
-    if (s > units) s = units;
+  float best = cost(1);
+  // a quarter, a half, and whole numbers of rounds
+  for (uint32_t q = 1; q <= 4u * (uint32_t)rounds; q += q < 4 ? q : 4) {
+    uint32_t s = q * n / (4 * t);
+    if (s > u) s = u;
     if (s <= 1) continue;
-    const int64_t c = cost((int)s);
+    const float c = cost(s);
     if (c < best) {
       best = c;
       d.splits = (int)s;

@@ -417,7 +417,7 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
         f.out = g.out;
         f.out_vec = g.out_vec;
         f.scale = scale;
-        const int64_t need = parts((v1 - v0) * parts(p.h, 4), 256);
+        const int64_t need = parts((v1 - v0) * parts(p.h, 4), 32);
         ACE_TRY(Launch<T>::finish(true, f, (int)(need < 4096 ? need : 4096), s));
       }
     }
@@ -444,7 +444,7 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
         f.out = d_hidden;
         f.out_vec = p.h % 4 == 0;
         f.scale = scale;
-        const int64_t need = parts(p.n * parts(p.h, 4), 256);
+        const int64_t need = parts(p.n * parts(p.h, 4), 32);
         ACE_TRY(Launch<T>::finish(false, f, (int)(need < 4096 ? need : 4096), s));
       }
     }

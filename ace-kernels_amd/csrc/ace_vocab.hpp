@@ -39,6 +39,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "ace_mma.hpp"
 
 namespace ace {
@@ -148,17 +150,18 @@ template <typename T>
 __device__ inline void copy_rows(const void* hidden, void* rows, int hidden_size, int width,
                                  int vec, const int* token, int count, int64_t at) {
   if (vec) {
-    const int chunks = width * (int)sizeof(T) / 16;
-    for (int64_t i = threadIdx.x; i < (int64_t)count * chunks; i += blockDim.x) {
-      const int j = (int)(i / chunks), c = (int)(i % chunks);
+    // at most 256 rows of 2^18 chunks: 32 bits
+    const uint32_t chunks = (uint32_t)(width * (int)sizeof(T) / 16);
+    for (uint32_t i = threadIdx.x; i < (uint32_t)count * chunks; i += blockDim.x) {
+      const uint32_t j = i / chunks, c = i % chunks;
       reinterpret_cast<uint4*>(rows)[(at + j) * chunks + c] =
           reinterpret_cast<const uint4*>(hidden)[(int64_t)token[j] * chunks + c];
     }
   } else {
-    for (int64_t i = threadIdx.x; i < (int64_t)count * width; i += blockDim.x) {
-      const int j = (int)(i / width), c = (int)(i % width);
+    for (uint32_t i = threadIdx.x; i < (uint32_t)count * (uint32_t)width; i += blockDim.x) {
+      const uint32_t j = i / (uint32_t)width, c = i % (uint32_t)width;
       T v{};
-      if (c < hidden_size) v = static_cast<const T*>(hidden)[(int64_t)token[j] * hidden_size + c];
+      if (c < (uint32_t)hidden_size) v = static_cast<const T*>(hidden)[(int64_t)token[j] * hidden_size + c];
       static_cast<T*>(rows)[(at + j) * width + c] = v;
     }
   }
@@ -619,8 +622,7 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void grad_kernel(GradPara
   const int count = *p.count;
   const int64_t nn = DW ? p.n : count;
   const int k = DW ? count : (int)p.k;
-  const int mts = (int)((p.m + TL::BM - 1) / TL::BM);
-  const int nts = (int)((nn + TL::BN - 1) / TL::BN);
+  const int mts = (int)((p.m + TL::BM - 1) / TL::BM), nts = (int)((nn + TL::BN - 1) / TL::BN);
   const int all = (k + kStep<T> - 1) / kStep<T>;  // steps there are
   // steps by which tiles are cut
   const int ks = DW ? all : (int)((p.k_map + kStep<T> - 1) / kStep<T>);
@@ -637,8 +639,9 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void grad_kernel(GradPara
   const auto part_at = [&](int part) {
     Part q;
     const int tile = part % d.tiles, s = part / d.tiles;
-    q.first = (int)((int64_t)s * ks / d.splits);
-    q.last = (int)((int64_t)(s + 1) * ks / d.splits);
+    const int each = ks / d.splits, more = ks % d.splits;  // the first `more` parts have one more
+    q.first = s * each + (s < more ? s : more);
+    q.last = q.first + each + (s < more);
     if (q.last > all) q.last = all;
     // tiles in groups of 8 along n: a group's operands are shared in L2
     constexpr int kGroup = 8;
@@ -734,40 +737,78 @@ struct FinishParams {
   const float* scale;
 };
 
-// out = the sum of each tile's partial tiles in order, in the output's type.
+// out = the sum of each tile's partial tiles in order, in the output's type.  Where
+// there are many for few results (few tokens, a long vocabulary), eight threads share
+// a group of four values: 20 tokens of a hidden size of 256 have 1280 such groups
+// of up to 384 parts, which took one thread each 29 us, and takes eight 7 us.
 template <typename T, bool DW>
 __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
+  __shared__ f32x4 s_sum[8][32];
   const int count = *p.count;
   const int64_t nn = DW ? p.n : count;
   const int k = DW ? count : (int)p.k_map;
-  const int mts = (int)((p.m + p.bm - 1) / p.bm), nts = (int)((nn + p.bn - 1) / p.bn);
+  const int mts = ((int)p.m + p.bm - 1) / p.bm, nts = ((int)nn + p.bn - 1) / p.bn;
   const int ks = (k + kStep<T> - 1) / kStep<T>;
   const mma::Deal d = mma::deal(mts * nts, ks, p.grad_blocks, kPartSteps<T>, kGradRounds);
   const float inv = p.scale ? 1.f / *p.scale : 1.f;
-  const int64_t quads = (p.hidden_size + 3) / 4;
+  const uint32_t quads = (uint32_t)((p.hidden_size + 3) / 4);
+  const int64_t all = p.out_rows * quads;
   const int64_t stride = (int64_t)d.tiles * p.bm * p.bn;  // from a split to the next
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.out_rows * quads;
-       i += (int64_t)gridDim.x * 256) {
-    const int64_t o = i / quads, m = i % quads * 4;
-    const int64_t n = DW ? o : p.row[o];
-    f32x4 sum{0.f, 0.f, 0.f, 0.f};
-    if (n >= 0 && ks > 0) {
-      constexpr int kGroup = 8;
-      const int nt = (int)(n / p.bn), mt = (int)(m / p.bm), from = nt / kGroup * kGroup;
-      const int width = nts - from < kGroup ? nts - from : kGroup;
-      const int64_t tile = (int64_t)from * mts + mt * width + (nt - from);
-      const float* at = p.seg + tile * p.bm * p.bn + (n % p.bn) * p.bm + m % p.bm;
-      for (int s0 = 0; s0 < d.splits; s0 += 8) {
-        f32x4 x[8];
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-          x[s] = s0 + s < d.splits ? *reinterpret_cast<const f32x4*>(at + (s0 + s) * stride)
-                                   : f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s < 8; ++s) sum += x[s];
-      }
+  const auto place = [&](int64_t i, int64_t& o, int& m) {
+    if (all <= UINT32_MAX) {  // a 64-bit division costs more than the rest
+      o = (uint32_t)i / quads;
+      m = (int)((uint32_t)i % quads) * 4;
+    } else {
+      o = i / quads;
+      m = (int)(i % quads) * 4;
     }
+  };
+  // parts first, first + by, ... of group i
+  const auto sum_of = [&](int64_t i, int first, int by) {
+    int64_t o;
+    int m;
+    place(i, o, m);
+    const int n = DW ? (int)o : p.row[o];
+    f32x4 sum{0.f, 0.f, 0.f, 0.f};
+    if (n < 0 || ks == 0) return sum;
+    constexpr int kGroup = 8;
+    const int nt = n / p.bn, mt = m / p.bm, from = nt / kGroup * kGroup;
+    const int width = nts - from < kGroup ? nts - from : kGroup;
+    const int64_t tile = (int64_t)from * mts + mt * width + (nt - from);
+    const float* at = p.seg + tile * p.bm * p.bn + (n % p.bn) * p.bm + m % p.bm;
+    for (int s0 = first; s0 < d.splits; s0 += 8 * by) {
+      f32x4 x[8];
+#pragma unroll
+      for (int s = 0; s < 8; ++s)
+        x[s] = s0 + s * by < d.splits ? *reinterpret_cast<const f32x4*>(at + (s0 + s * by) * stride)
+                                      : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 8; ++s) sum += x[s];
+    }
+    return sum;
+  };
+  const auto put = [&](int64_t i, f32x4 sum) {
+    int64_t o;
+    int m;
+    place(i, o, m);
     store4(static_cast<T*>(p.out) + o * p.hidden_size + m, sum * inv, p.hidden_size - m, p.out_vec);
+  };
+  if (d.splits <= 8 || all >= 32768) {
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256)
+      put(i, sum_of(i, 0, 1));
+    return;
+  }
+  const int z = (int)threadIdx.x / 32, q = (int)threadIdx.x % 32;
+  for (int64_t i0 = (int64_t)blockIdx.x * 32; i0 < all; i0 += (int64_t)gridDim.x * 32) {
+    if (i0 + q < all) s_sum[z][q] = sum_of(i0 + q, z, 8);
+    __syncthreads();
+    if (z == 0 && i0 + q < all) {
+      f32x4 sum = s_sum[0][q];
+#pragma unroll
+      for (int y = 1; y < 8; ++y) sum += s_sum[y][q];
+      put(i0 + q, sum);
+    }
+    __syncthreads();
   }
 }
 
@@ -778,7 +819,7 @@ enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTiles = 4 };
 struct TileShape {
   int bm, bn, per_cu;  // per_cu: blocks of it whose LDS fits one of the 256 CUs
 };
-constexpr TileShape kShape[kTiles] = {{256, 256, 1}, {128, 128, 2}, {128, 64, 3}, {128, 32, 3}};
+constexpr TileShape kShape[kTiles] = {{256, 256, 1}, {128, 128, 2}, {128, 64, 3}, {128, 32, 2}};
 
 // Implemented per element type by ACE_DEFINE_VOCAB in the ace_k_vocab_*.hip
 // units.
@@ -793,15 +834,22 @@ struct Launch {
   static hipError_t finish(bool dw, const FinishParams&, int blocks, hipStream_t);
 };
 
-template <typename P>
-inline hipError_t launch(void (*kern)(P), int blocks, int threads, size_t lds, hipStream_t s,
-                         const P& p) {
-  if (lds > 64 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(kern),
-                                             hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+template <auto KERNEL, typename P>
+inline hipError_t launch(int blocks, int threads, size_t lds, hipStream_t s, const P& p) {
+  if (lds > 64 * 1024) {  // asked for once per kernel and device
+    static std::atomic<uint64_t> asked{0};
+    int device = 0;
+    hipError_t e = hipGetDevice(&device);
     if (e != hipSuccess) return e;
+    const uint64_t bit = 1ull << (device & 63);
+    if (device > 63 || !(asked.load(std::memory_order_relaxed) & bit)) {
+      e = hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+      if (e != hipSuccess) return e;
+      asked.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
-  hipLaunchKernelGGL(kern, dim3((unsigned)blocks), dim3((unsigned)threads), lds, s, p);
+  hipLaunchKernelGGL(KERNEL, dim3((unsigned)blocks), dim3((unsigned)threads), lds, s, p);
   return hipGetLastError();
 }
 
@@ -818,7 +866,7 @@ inline hipError_t with_tile(int tile, F f) {
 #define ACE_DEFINE_VOCAB(T)                                                                      \
   template <>                                                                                    \
   hipError_t Launch<T>::prep(const PrepParams& p, int blocks, hipStream_t s) {                   \
-    return launch(prep_kernel<T>, blocks, 256, 0, s, p);                                         \
+    return launch<prep_kernel<T>>(blocks, 256, 0, s, p);                                         \
   }                                                                                              \
   template <>                                                                                    \
   hipError_t Launch<T>::pad(const void* src, void* dst, int64_t rows, int size, int width,       \
@@ -832,18 +880,18 @@ inline hipError_t with_tile(int tile, F f) {
   hipError_t Launch<T>::score(int tile, const ScoreParams& p, int blocks, hipStream_t s) {       \
     return with_tile<T, true, true>(tile, [&](auto t) {                                          \
       using TL = decltype(t);                                                                    \
-      return launch(score_kernel<TL>, blocks, TL::kThreads, TL::kLdsBytes, s, p);                \
+      return launch<score_kernel<TL>>(blocks, TL::kThreads, TL::kLdsBytes, s, p);                \
     });                                                                                          \
   }                                                                                              \
   template <>                                                                                    \
   hipError_t Launch<T>::upstream(const UpstreamParams& p, int blocks, hipStream_t s) {           \
-    return launch(upstream_kernel<T>, blocks, 256, 0, s, p);                                     \
+    return launch<upstream_kernel<T>>(blocks, 256, 0, s, p);                                     \
   }                                                                                              \
   template <>                                                                                    \
   hipError_t Launch<T>::dscore(int tile, const ScoreParams& p, int blocks, hipStream_t s) {      \
     return with_tile<T, true, true, true>(tile, [&](auto t) {                                    \
       using TL = decltype(t);                                                                    \
-      return launch(dscore_kernel<TL>, blocks, TL::kThreads, TL::kLdsBytes, s, p);               \
+      return launch<dscore_kernel<TL>>(blocks, TL::kThreads, TL::kLdsBytes, s, p);               \
     });                                                                                          \
   }                                                                                              \
   template <>                                                                                    \
@@ -852,17 +900,17 @@ inline hipError_t with_tile(int tile, F f) {
     if (dw)                                                                                      \
       return with_tile<T, false, false, sizeof(T) == 2>(tile, [&](auto t) {                      \
         using TL = decltype(t);                                                                  \
-        return launch(grad_kernel<TL, true>, blocks, TL::kThreads, TL::kLdsBytes, s, p);         \
+        return launch<grad_kernel<TL, true>>(blocks, TL::kThreads, TL::kLdsBytes, s, p);         \
       });                                                                                        \
     return with_tile<T, false, true>(tile, [&](auto t) {                                         \
       using TL = decltype(t);                                                                    \
-      return launch(grad_kernel<TL, false>, blocks, TL::kThreads, TL::kLdsBytes, s, p);          \
+      return launch<grad_kernel<TL, false>>(blocks, TL::kThreads, TL::kLdsBytes, s, p);          \
     });                                                                                          \
   }                                                                                              \
   template <>                                                                                    \
   hipError_t Launch<T>::finish(bool dw, const FinishParams& p, int blocks, hipStream_t s) {      \
-    return dw ? launch(finish_kernel<T, true>, blocks, 256, 0, s, p)                             \
-              : launch(finish_kernel<T, false>, blocks, 256, 0, s, p);                           \
+    return dw ? launch<finish_kernel<T, true>>(blocks, 256, 0, s, p)                             \
+              : launch<finish_kernel<T, false>>(blocks, 256, 0, s, p);                           \
   }
 
 }  // namespace vocab
