@@ -27,11 +27,11 @@
 // against 64 bits are 1.1 times those of a gradient that is only rounded at the end.
 //
 // What bounds it: the matrix cores.  8192 tokens (5 % ignored) x 4096 x 65536 words
-// in bfloat16 take 13.9 ms for four products of 4.2 TFLOP, 1.2 PFLOP/s, the rate
+// in bfloat16 take 13.4 ms for four products of 4.2 TFLOP, 1.2 PFLOP/s, the rate
 // of the library's products of this size (1.1 to 1.4 PFLOP/s); the logits are
 // formed twice because they are not kept.  With few tokens it is the weight, which
 // is read three times and whose gradient is written: 96 tokens x 2048 x 50304 words
-// in float16 take 0.28 ms for 0.83 GB.
+// in float16 take 0.27 ms for 0.83 GB.
 #pragma once
 
 #include <float.h>

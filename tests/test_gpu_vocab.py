@@ -104,11 +104,14 @@ def test_reductions(reduction, dtype) -> None:
     _compare(hidden, weight, labels, VocabConfig(reduction=reduction), go, torch.randn(n, generator=gen).cuda())
 
 
-@pytest.mark.parametrize("n,size,v", [(2100, 128, 8200), (6000, 64, 30000), (9000, 72, 1024)])
+@pytest.mark.parametrize("n,size,v", [(2100, 128, 8200), (6000, 64, 30000), (9000, 72, 1024), (70000, 40, 300),
+                                      (3, 24, 200000), (40, 1024, 60000)])
 @pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
 def test_large_tiles_and_pieces(n, size, v, dtype) -> None:
     """The 256-wide tiles; 6000 x 30000 takes two pieces of the vocabulary;
-    9000 tokens of a small head share out the tokens of the weight's gradient."""
+    9000 tokens of a small head share out the tokens of the weight's gradient; 70000
+    have more token tiles than blocks; few tokens of a long vocabulary have the
+    hidden gradient in many partial tiles."""
     hidden, weight, labels = inputs(n, size, v, dtype, seed=8, ignored=0.4)
     _compare(hidden, weight, labels, VocabConfig(), torch.tensor(1.0, device="cuda"))
 
