@@ -54,9 +54,13 @@ __device__ inline char* lds_base() {
 // it is written as assembler: the compiler waits for every load to LDS that it
 // knows of before each transposing LDS read, which takes the whole pipeline away
 // (8192 x 8192 x 4096 in bfloat16: 820 TFLOP/s instead of 1146).  Nothing here has
-// an output, the waits are landed_barrier's, and nothing else in a kernel that
-// uses it needs m0.  Where no transposing reads are,
-// the builtin leaves the compiler more freedom (1200 instead of 1140).
+// an output, and the waits for the data are landed_barrier's.  What the compiler
+// would do for an instruction of its own is done in the block: a vector memory
+// instruction may read scalar registers that a vector instruction wrote
+// (v_readfirstlane) no sooner than five wait states later, which is the move and
+// four of s_nop 3 (the load that follows a write of m0 needs one of them).  Where no
+// transposing reads are, the builtin leaves the compiler more freedom (1200 instead
+// of 1140).
 __device__ inline uint32_t lds_address(const char* p) {
   return (uint32_t)__builtin_amdgcn_readfirstlane(
       (int)(uintptr_t)(__attribute__((address_space(3))) const char*)p);
@@ -70,9 +74,10 @@ __device__ inline const char* uniform(const char* p) {
 template <bool ASM>
 __device__ inline void load_to_lds(const char* base, uint32_t off, char* dst) {
   if constexpr (ASM)
-    asm volatile(
-        "s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds_address(dst)),
-        "v"(off), "s"(uniform(base)));
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(
+                     lds_address(dst)),
+                 "v"(off), "s"(uniform(base))
+                 : "m0");
   else
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(base + off),
                                      (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
@@ -82,7 +87,8 @@ __device__ inline void load_to_lds(const char* src, char* dst) {
   if constexpr (ASM)
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(
                      lds_address(dst)),
-                 "v"(src));
+                 "v"(src)
+                 : "m0");
   else
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
                                      (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
