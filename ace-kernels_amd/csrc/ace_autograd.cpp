@@ -16,6 +16,7 @@
 // (ace_kernels/balance.py) have their calls and nodes here too, for any
 // arguments: the Python side checks them, nothing is remembered between calls.
 #include <ATen/DeviceGuard.h>
+#include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -25,6 +26,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <atomic>
+#include <initializer_list>
 #include <memory>
 #include <stdexcept>
 #include <string>
@@ -320,6 +322,15 @@ void refuse_second_derivative(variable_list& out, const variable_list& inputs, c
     if (t.defined()) torch::autograd::set_history(t, node);
 }
 
+// The nodes know no forward-mode derivative: a tensor that carries a tangent is
+// refused, as its result would come without one.
+void refuse_tangents(std::initializer_list<at::Tensor> inputs, const char* what) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const at::Tensor& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what,
+                                " has no forward-mode derivative");
+}
+
 struct VocabLossBackward : public Node {
   std::string name() const override { return "VocabLossBackward"; }
 
@@ -328,6 +339,7 @@ struct VocabLossBackward : public Node {
     const at::Tensor& gl = grads[0];
     const at::Tensor gc = grads.size() > 1 ? grads[1] : at::Tensor();
     if (!gl.defined() && !gc.defined()) return out;
+    refuse_tangents({gl, gc}, "vocab_loss's gradient");
     const at::Tensor hidden = hidden_.unpack(), weight = weight_.unpack(), saved = saved_.unpack();
     {
       const at::NoGradGuard no_grad;
@@ -369,6 +381,7 @@ std::vector<at::Tensor> vocab_loss(const at::Tensor& hidden, const at::Tensor& w
                                    const at::Tensor& labels, int64_t ignore_index, int reduction,
                                    bool scores) {
   if (!g_vocab_forward.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  refuse_tangents({hidden, weight}, "vocab_loss");
   const bool record = torch::autograd::compute_requires_grad(hidden, weight);
   const c10::DeviceGuard guard(hidden.device());
   std::vector<at::Tensor> out;
@@ -415,6 +428,7 @@ struct BalanceLossBackward : public Node {
   variable_list apply(variable_list&& grads) override {
     variable_list out(1);
     if (!grads[0].defined()) return out;
+    refuse_tangents({grads[0]}, "balance_loss's gradient");
     const at::Tensor logits = logits_.unpack(), share = share_.unpack(), mask = mask_.unpack();
     {
       const at::NoGradGuard no_grad;
@@ -449,6 +463,7 @@ std::vector<at::Tensor> balance_loss(const at::Tensor& logits, const std::option
                                      int64_t groups, int top_k, int reduction,
                                      const at::Tensor& tickets) {
   if (!g_balance_forward.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  refuse_tangents({logits}, "balance_loss");
   const bool record = torch::autograd::compute_requires_grad(logits);
   const c10::DeviceGuard guard(logits.device());
   const int64_t tokens = logits.size(-2), experts = logits.size(-1);

@@ -94,3 +94,14 @@ def test_limits_and_workspace() -> None:
     assert _forward(nbytes=need - 1) == 3 and _forward(ticket_bytes=tickets - 1) == 3
     assert lib.ace_balance_workspace_bytes(0, 10, 8) == 0 and lib.ace_balance_ticket_bytes(0, 10, 8) == 0
     assert _backward(tokens=0, logits=None, share=None, grad=None, d=None) == 0  # nothing to do
+
+
+def test_tangents_are_refused() -> None:
+    """The call itself, under the checks of the Python side: scores with a tangent
+    raise, where their loss would have had none."""
+    import torch.autograd.forward_ad as fwd
+
+    x = torch.randn(5, 8)
+    with fwd.dual_level(), pytest.raises(NotImplementedError, match="balance_loss has no forward-mode derivative"):
+        _lib.autograd().balance_loss(fwd.make_dual(x, torch.ones_like(x)), None, 1, 2, _lib.RED_MEAN,
+                                     torch.zeros(4096, dtype=torch.uint8))

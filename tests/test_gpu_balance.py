@@ -258,3 +258,18 @@ def test_second_derivative_is_refused() -> None:
     (g,) = torch.autograd.grad(balance_loss(leaf, BalanceConfig(top_k=2)).loss, leaf, create_graph=True)
     with pytest.raises(RuntimeError):
         torch.autograd.grad(g.sum(), leaf)
+
+
+def test_forward_mode_is_refused() -> None:
+    """In the call and in its backward: nothing comes back without its tangent."""
+    import torch.autograd.forward_ad as fwd
+
+    x, cfg = _scores((), 20, 8, F32), BalanceConfig(top_k=2)
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            balance_loss(fwd.make_dual(x, torch.ones_like(x)), cfg)
+        leaf = x.clone().requires_grad_(True)
+        loss = balance_loss(leaf, cfg).loss
+        up = fwd.make_dual(torch.ones_like(loss), torch.ones_like(loss))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(loss, leaf, up)

@@ -355,3 +355,18 @@ def test_captured_step_replays() -> None:
         torch.cuda.synchronize()
         for a, b in zip(got, want):
             assert torch.equal(a, b), f"replay {i}"
+
+
+def test_forward_mode_is_refused() -> None:
+    """In the call and in its backward: nothing comes back without its tangent."""
+    import torch.autograd.forward_ad as fwd
+
+    hidden, weight, labels = inputs(10, 64, 50, F32)
+    with fwd.dual_level():
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            vocab_loss_confidence(fwd.make_dual(hidden, torch.ones_like(hidden)), weight, labels)
+        h = hidden.clone().requires_grad_(True)
+        loss = vocab_loss(h, weight, labels)
+        up = fwd.make_dual(torch.ones_like(loss), torch.ones_like(loss))
+        with pytest.raises(NotImplementedError, match="forward-mode"):
+            torch.autograd.grad(loss, h, up)

@@ -115,3 +115,15 @@ def test_workspace_is_bounded() -> None:
     assert lib.ace_vocab_workspace_bytes(_lib.F64, 8, 8, 8, 0) == 0
     assert lib.ace_vocab_workspace_bytes(_lib.BF16, -1, 8, 8, 0) == 0
     assert lib.ace_vocab_saved_bytes(0) > 0 and lib.ace_vocab_saved_bytes(-1) == 0
+
+
+def test_tangents_are_refused() -> None:
+    """The call itself, under the checks of the Python side: a tensor with a
+    tangent raises, where its loss would have had none."""
+    import torch.autograd.forward_ad as fwd
+
+    h, w, y = torch.randn(6, 8), torch.randn(10, 8), torch.zeros(6, dtype=torch.int64)
+    with fwd.dual_level():
+        for a, b in ((fwd.make_dual(h, torch.ones_like(h)), w), (h, fwd.make_dual(w, torch.ones_like(w)))):
+            with pytest.raises(NotImplementedError, match="vocab_loss has no forward-mode derivative"):
+                _lib.autograd().vocab_loss(a, b, y, -100, _lib.RED_MEAN, False)
