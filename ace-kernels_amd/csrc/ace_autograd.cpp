@@ -361,7 +361,7 @@ struct VocabLossBackward : public Node {
           current_stream(hidden));
       if (rc) fail(rc, "ace_vocab_backward");
     }
-    refuse_second_derivative(out, {hidden, weight}, "vocab_loss");
+    refuse_second_derivative(out, {hidden, weight, gl, gc}, "vocab_loss");
     return out;
   }
 
@@ -443,7 +443,7 @@ struct BalanceLossBackward : public Node {
           current_stream(logits));
       if (rc) fail(rc, "ace_balance_backward");
     }
-    refuse_second_derivative(out, {logits}, "balance_loss");
+    refuse_second_derivative(out, {logits, grads[0]}, "balance_loss");
     return out;
   }
 

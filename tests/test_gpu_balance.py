@@ -273,3 +273,12 @@ def test_forward_mode_is_refused() -> None:
         up = fwd.make_dual(torch.ones_like(loss), torch.ones_like(loss))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(loss, leaf, up)
+
+
+def test_second_derivative_in_the_upstream_gradient_is_refused() -> None:
+    leaf = _scores((), 20, 8, F32).requires_grad_(True)
+    loss = balance_loss(leaf, BalanceConfig(top_k=2)).loss
+    up = torch.ones_like(loss).requires_grad_(True)
+    (g,) = torch.autograd.grad(loss, leaf, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="only once"):
+        torch.autograd.grad(g.sum(), up, allow_unused=True)

@@ -370,3 +370,13 @@ def test_forward_mode_is_refused() -> None:
         up = fwd.make_dual(torch.ones_like(loss), torch.ones_like(loss))
         with pytest.raises(NotImplementedError, match="forward-mode"):
             torch.autograd.grad(loss, h, up)
+
+
+def test_second_derivative_in_the_upstream_gradient_is_refused() -> None:
+    hidden, weight, labels = inputs(10, 64, 50, F32)
+    h = hidden.clone().requires_grad_(True)
+    loss = vocab_loss(h, weight, labels)
+    up = torch.ones_like(loss).requires_grad_(True)
+    (g,) = torch.autograd.grad(loss, h, up, create_graph=True)
+    with pytest.raises(RuntimeError, match="only once"):
+        torch.autograd.grad(g.sum(), up, allow_unused=True)
