@@ -249,7 +249,7 @@ struct ScoreParams {
   const float* g;      // row -> upstream of nll
   const float* c;      // row -> upstream of conf, times conf; null: none
   int one_g;           // g is the same for all rows
-  const float* bound;  // float16: blocks' largest |g| + |c|, and how many
+  const float* bound;  // blocks' largest |g| + |c|, and how many
   int bounds;
   float* scale;        // 16 bits: what ds is multiplied by (out)
 };
@@ -484,6 +484,10 @@ __global__ __launch_bounds__(256) void upstream_kernel(UpstreamParams p) {
 // float16 takes 2^13 of that, or for other upstream gradients a power of two that
 // takes the largest |g| + |c|, dS's bound, to 2^13..2^14: without it the
 // probabilities of a large vocabulary are below float16's smallest numbers.
+// bfloat16 has float32's range: with confidences whose upstream gradients are
+// larger by more than kMostScaled it takes none, as the products' sums would
+// leave that range.
+constexpr float kMostScaled = 0x1p40f;
 template <typename T>
 constexpr float kHalfScale = __is_same(T, _Float16) ? 8192.f : 1.f;
 
@@ -507,17 +511,22 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreP
   const int count = *p.saved.count;
   float scale = 1.f;
   if constexpr (sizeof(T) == 2) {
+    constexpr bool half = __is_same(T, _Float16);
     const float g0 = p.one_g && count > 0 ? fabsf(p.g[0]) : 0.f;
     if (g0 >= FLT_MIN * 8192.f && g0 <= FLT_MAX / 8192.f) {
       scale = kHalfScale<T> / g0;
     }
-    if (__is_same(T, _Float16) && (scale == 1.f || p.c)) {
+    if (p.c || (half && scale == 1.f)) {
       float most = 0.f;  // every wave on its own
       for (int i = lane; i < p.bounds; i += 64) most = fmaxf(most, p.bound[i]);
 #pragma unroll
       for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
       // with confidences: no more than the largest |g| + |c| allows
-      if (scale == 1.f || !(most * scale <= 32768.f)) scale = scale_of(most);
+      if constexpr (half) {
+        if (scale == 1.f || !(most * scale <= 32768.f)) scale = scale_of(most);
+      } else {
+        if (!(most * scale <= kMostScaled)) scale = 1.f;
+      }
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *p.scale = scale;
   }

@@ -380,3 +380,27 @@ def test_second_derivative_in_the_upstream_gradient_is_refused() -> None:
     (g,) = torch.autograd.grad(loss, h, up, create_graph=True)
     with pytest.raises(RuntimeError, match="only once"):
         torch.autograd.grad(g.sum(), up, allow_unused=True)
+
+
+def _compare_all(hidden, weight, labels, config=VocabConfig(), go=None, gc=None):
+    """``_compare`` with both gradients always among it: tokens whose two largest
+    logits are too close to tell which is the top label have no upstream gradient
+    of their confidence, on which the top label bears."""
+    if gc is not None:
+        gc = torch.where(exact(hidden, weight, labels, config.ignore_index, config.reduction).sure, gc, 0.0)
+    want = exact(hidden, weight, labels, config.ignore_index, config.reduction, go, gc)
+    out, (dh, dw) = _compare(hidden, weight, labels, config, go, gc)
+    _within(dh, want.d_hidden, want.tol_hidden + 1e-30, "d hidden")
+    _within(dw, want.d_weight, want.tol_weight + 1e-30, "d weight")
+    return out, (dh, dw)
+
+
+def test_tiny_upstream_of_the_loss_beside_an_ordinary_one_of_the_confidence() -> None:
+    """dS is held times the reciprocal of the loss's upstream gradient, unless that
+    takes the confidence's part out of float32's range."""
+    n, size, v = 300, 64, 500
+    hidden, weight, labels = inputs(n, size, v, BF16, seed=31, ignored=0.1)
+    gc = torch.randn(n, generator=torch.Generator().manual_seed(3)).cuda()
+    for up in (1e-34, 1e-30, 1e-12, 1.0):
+        for factor in (1.0, 1e5):
+            _compare_all(hidden, weight, labels, VocabConfig(reduction="sum"), torch.tensor(up, device="cuda"), factor * gc)
