@@ -240,8 +240,8 @@ BackwardSpace backward_space(const Plan& p) {
   BackwardSpace s{};
   const TileShape ht = kShape[p.dh_tile], wt = kShape[p.dw_tile];
   s.zeros = c.take(16);
-  s.scale = c.take(4);
-  s.bound = c.take((size_t)p.prep_blocks * 4);
+  s.scale = c.take(8);
+  s.bound = c.take((size_t)p.prep_blocks * 8);
   s.g = c.take((size_t)p.n * 4);
   s.c = c.take((size_t)p.n * 4);
   s.rows = c.take((size_t)(p.n * p.width) * p.es);
@@ -362,6 +362,9 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
     weight = ws + at.weight;
   }
   float* scale = sizeof(T) == 2 ? reinterpret_cast<float*>(ws + at.scale) : nullptr;
+  // float16: tokens' upstream gradients may be far apart (kApart)
+  const bool apart = __is_same(T, _Float16) && d_hidden && p.n > 0 &&
+                     (reduction == ACE_RED_NONE || grad_confidence);
   const TileShape ht = kShape[p.dh_tile], wt = kShape[p.dw_tile];
   const int64_t row_bytes = p.width * p.es;
   for (int64_t v0 = 0; v0 < p.v; v0 += p.piece) {
@@ -385,6 +388,7 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
     r.bound = q.bound;
     r.bounds = p.prep_blocks;
     r.scale = scale;
+    r.scaling = apart && !d_weight ? kEach : kTogether;
     ACE_TRY(Launch<T>::dscore(p.score_tile, r, p.dscore_blocks, s));
     GradParams g{};
     g.b = ws + at.ds;
@@ -422,6 +426,10 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
       }
     }
     if (d_hidden && p.n > 0) {
+      if (apart && d_weight) {
+        r.scaling = kEachOrNone;
+        ACE_TRY(Launch<T>::dscore(p.score_tile, r, p.dscore_blocks, s));
+      }
       g.a = w;
       g.a_stride = row_bytes;
       g.k = v1 - v0;
@@ -444,6 +452,10 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
         f.out = d_hidden;
         f.out_vec = p.h % 4 == 0;
         f.scale = scale;
+        if (apart) {
+          f.g = q.g;
+          f.c = q.c;
+        }
         const int64_t need = parts(p.n * parts(p.h, 4), 32);
         ACE_TRY(Launch<T>::finish(false, f, (int)(need < 4096 ? need : 4096), s));
       }

@@ -249,9 +249,12 @@ struct ScoreParams {
   const float* g;      // row -> upstream of nll
   const float* c;      // row -> upstream of conf, times conf; null: none
   int one_g;           // g is the same for all rows
-  const float* bound;  // blocks' largest |g| + |c|, and how many
+  const float* bound;  // blocks' largest |g| + |c|, then (float16) their smallest
+                       // that is not 0, and how many blocks
   int bounds;
-  float* scale;        // 16 bits: what ds is multiplied by (out)
+  int scaling;         // float16: kTogether, kEach or kEachOrNone
+  float* scale;        // 16 bits (out): what ds is multiplied by, and whether the
+                       // rows of the hidden gradient's ds have scales of their own
 };
 
 // How the score kernels deal (token tile) x (vocabulary tiles): part s of a token
@@ -435,7 +438,7 @@ struct UpstreamParams {
   const float* grad_conf;  // [n] or null
   float* g;
   float* c;
-  float* bound;            // [blocks]
+  float* bound;            // [blocks], float16: [2][blocks]
 };
 
 // The rows' upstream gradients, and the counted tokens' hidden states together
@@ -449,7 +452,7 @@ __global__ __launch_bounds__(256) void upstream_kernel(UpstreamParams p) {
   if (blockIdx.x == 0 && tid < 4) reinterpret_cast<int*>(q.zeros)[tid] = 0;
   const int64_t first = (int64_t)blockIdx.x * q.per_block;
   const int64_t last = first + q.per_block < count ? first + q.per_block : count;
-  float most = 0.f;
+  float most = 0.f, least = FLT_MAX;
   for (int64_t r0 = first; r0 < last; r0 += 256) {
     __syncthreads();
     const int64_t r = r0 + tid;
@@ -463,7 +466,9 @@ __global__ __launch_bounds__(256) void upstream_kernel(UpstreamParams p) {
       }
       if (p.c) p.c[r] = c = p.grad_conf[t] * q.saved.inv[r];
       p.g[r] = g;
-      most = fmaxf(most, fabsf(g) + fabsf(c));
+      const float bound = fabsf(g) + fabsf(c);
+      most = fmaxf(most, bound);
+      if (bound > 0.f) least = fminf(least, bound);
     }
     __syncthreads();
     if (q.rows)
@@ -475,6 +480,15 @@ __global__ __launch_bounds__(256) void upstream_kernel(UpstreamParams p) {
   if ((tid & 63) == 0) s_max[tid >> 6] = most;
   __syncthreads();
   if (tid == 0) p.bound[blockIdx.x] = fmaxf(fmaxf(s_max[0], s_max[1]), fmaxf(s_max[2], s_max[3]));
+  if constexpr (__is_same(T, _Float16)) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) least = fminf(least, __shfl_xor(least, d));
+    __syncthreads();
+    if ((tid & 63) == 0) s_max[tid >> 6] = least;
+    __syncthreads();
+    if (tid == 0)
+      p.bound[gridDim.x + blockIdx.x] = fminf(fminf(s_max[0], s_max[1]), fminf(s_max[2], s_max[3]));
+  }
 }
 
 // dS is held times a scale that its products are divided by at the end.
@@ -487,7 +501,21 @@ __global__ __launch_bounds__(256) void upstream_kernel(UpstreamParams p) {
 // bfloat16 has float32's range: with confidences whose upstream gradients are
 // larger by more than kMostScaled it takes none, as the products' sums would
 // leave that range.
+//
+// One scale serves all tokens in float16 while their |g| + |c| are within kApart
+// of each other: an entry is then off by at most half of float16's smallest step,
+// 2^-25, against a bound of 2^7, which summed over 2^18 words is below float16's
+// own rounding of the token's gradient.  Where they are further apart, the
+// probabilities of tokens with small upstream gradients would be lost, so the hidden
+// gradient has a dS of its own, each row scaled by a power of two to 2^13..2^14, which
+// finish_kernel takes out.  The weight's gradient sums over tokens, beside whose
+// largest those entries do not count.
 constexpr float kMostScaled = 0x1p40f;
+constexpr float kApart = 64.f;
+// What one launch of dscore_kernel makes: dS with one scale; dS for the hidden
+// gradient, with scales by row where they are needed; or that, and nothing where
+// they are not (the dS that is there serves).
+enum { kTogether = 0, kEach = 1, kEachOrNone = 2 };
 template <typename T>
 constexpr float kHalfScale = __is_same(T, _Float16) ? 8192.f : 1.f;
 
@@ -510,6 +538,7 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreP
   const int lane = (int)threadIdx.x & 63, n = lane & 15, g = lane >> 4;
   const int count = *p.saved.count;
   float scale = 1.f;
+  bool by_row = false;
   if constexpr (sizeof(T) == 2) {
     constexpr bool half = __is_same(T, _Float16);
     const float g0 = p.one_g && count > 0 ? fabsf(p.g[0]) : 0.f;
@@ -523,12 +552,26 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreP
       for (int d = 1; d < 64; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
       // with confidences: no more than the largest |g| + |c| allows
       if constexpr (half) {
+        if (p.scaling != kTogether) {
+          float least = FLT_MAX;
+          for (int i = lane; i < p.bounds; i += 64) least = fminf(least, p.bound[p.bounds + i]);
+#pragma unroll
+          for (int d = 1; d < 64; d *= 2) least = fminf(least, __shfl_xor(least, d));
+          by_row = least * kApart < most;
+        }
         if (scale == 1.f || !(most * scale <= 32768.f)) scale = scale_of(most);
       } else {
         if (!(most * scale <= kMostScaled)) scale = 1.f;
       }
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *p.scale = scale;
+    if (p.scaling == kEachOrNone && !by_row) {
+      if (blockIdx.x == 0 && threadIdx.x == 0) p.scale[1] = 0.f;
+      return;
+    }
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+      p.scale[0] = scale;
+      p.scale[1] = by_row ? 1.f : 0.f;
+    }
   }
   float top[NT], of_p[NT], of_label[NT], of_best[NT];
   int label[NT], best[NT];
@@ -537,8 +580,10 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void dscore_kernel(ScoreP
     for (int j = 0; j < NT; ++j) {
       const int r = tt * TL::BN + TL::wave_n() + 16 * j + n;
       const bool in = r < count;
-      const float gr = in ? p.g[r] * scale : 0.f;
-      const float cr = in && p.c ? p.c[r] * scale : 0.f;
+      float gr = in ? p.g[r] : 0.f, cr = in && p.c ? p.c[r] : 0.f;
+      const float by = by_row ? scale_of(fabsf(gr) + fabsf(cr)) : scale;
+      gr *= by;
+      cr *= by;
       top[j] = in ? p.saved.top[r] : 0.f;
       of_p[j] = in ? (gr - cr) * p.saved.inv[r] : 0.f;
       of_label[j] = gr;
@@ -744,6 +789,8 @@ struct FinishParams {
   void* out;
   int out_vec;
   const float* scale;
+  const float* g;     // dh in float16, where rows may have scales of their own: the
+  const float* c;     // rows' upstream gradients (c may be null), else null
 };
 
 // out = the sum of each tile's partial tiles in order, in the output's type.  Where
@@ -760,6 +807,7 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
   const int ks = (k + kStep<T> - 1) / kStep<T>;
   const mma::Deal d = mma::deal(mts * nts, ks, p.grad_blocks, kPartSteps<T>, kGradRounds);
   const float inv = p.scale ? 1.f / *p.scale : 1.f;
+  const bool by_row = p.g && p.scale[1] != 0.f;
   const uint32_t quads = (uint32_t)((p.hidden_size + 3) / 4);
   const int64_t all = p.out_rows * quads;
   const int64_t stride = (int64_t)d.tiles * p.bm * p.bn;  // from a split to the next
@@ -800,7 +848,14 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
     int64_t o;
     int m;
     place(i, o, m);
-    store4(static_cast<T*>(p.out) + o * p.hidden_size + m, sum * inv, p.hidden_size - m, p.out_vec);
+    float of = inv;
+    if constexpr (!DW && __is_same(T, _Float16)) {
+      if (by_row) {
+        const int r = p.row[o];
+        if (r >= 0) of = 1.f / scale_of(fabsf(p.g[r]) + (p.c ? fabsf(p.c[r]) : 0.f));
+      }
+    }
+    store4(static_cast<T*>(p.out) + o * p.hidden_size + m, sum * of, p.hidden_size - m, p.out_vec);
   };
   if (d.splits <= 8 || all >= 32768) {
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256)

@@ -404,3 +404,72 @@ def test_tiny_upstream_of_the_loss_beside_an_ordinary_one_of_the_confidence() ->
     for up in (1e-34, 1e-30, 1e-12, 1.0):
         for factor in (1.0, 1e5):
             _compare_all(hidden, weight, labels, VocabConfig(reduction="sum"), torch.tensor(up, device="cuda"), factor * gc)
+
+
+def _by_size(hidden, weight, labels, config, go, gc, size_of, head):
+    """The hidden gradient of tokens whose upstream gradients are of very different
+    size, compared group by group: each group's bound knows only its own size.  float16
+    holds dS of a token at 2^7 or more of what the group's reference allows for its
+    subnormals (2^13), so that rounding is off by half a step, 2^-25, of that."""
+    h = hidden.detach().clone().requires_grad_(True)
+    leaves = (h,)
+    w = weight.detach().clone().requires_grad_(not head)
+    if not head:
+        leaves = (h, w)
+    out = vocab_loss_confidence(h, w, labels, config)
+    grads = torch.autograd.grad((out.loss, out.confidence), leaves, (go, gc))
+    counted = int(((labels >= 0) & (labels < weight.shape[0])).sum())
+    for group in size_of.unique():
+        at = size_of == group
+        one = go[at] if config.reduction == "none" else (go / counted).expand(int(at.sum()))
+        want = exact(hidden[at], weight, labels[at], reduction="none", grad_loss=one, grad_confidence=gc[at])
+        most = float((one.abs() + gc[at].abs()).max())
+        floor = 2.0 ** -25 / 2.0 ** 7 * most * weight.double().abs().sum(0)
+        _within(grads[0][at], want.d_hidden, want.tol_hidden + floor, f"d hidden of group {int(group)}")
+    return grads
+
+
+@pytest.mark.parametrize("frozen_head", [False, True], ids=["both", "frozen head"])
+@pytest.mark.parametrize("n,v", [(160, 20000), (2500, 60000)])  # one piece of the vocabulary, and two
+def test_float16_hidden_gradients_of_tokens_with_small_upstream_gradients(n, v, frozen_head) -> None:
+    """Upstream gradients over 2^-21..1 of a loss scale: each token's own hidden
+    gradient is as good as if the token were alone.  The weight's rows share a mean,
+    to which a token's many small probabilities add up."""
+    size = 64
+    hidden, weight, labels = inputs(n, size, v, F16, seed=17, ignored=0.1)
+    hidden, weight = hidden / 8, weight + 0.5
+    group = torch.arange(n, device="cuda") % 8
+    size_of = torch.exp2(12.0 - 3 * group)
+    gen = torch.Generator().manual_seed(2)
+    sign = torch.sign(torch.randn(n, generator=gen)).cuda()
+    # per-token weights of the loss
+    grads = _by_size(hidden, weight, labels, VocabConfig(reduction="none"), size_of * sign, torch.zeros(n, device="cuda"), group,
+                     frozen_head)
+    want = exact(hidden, weight, labels, reduction="none", grad_loss=size_of * sign)
+    _within(grads[0], want.d_hidden, want.tol_hidden, "d hidden")
+    if not frozen_head:
+        _within(grads[1], want.d_weight, want.tol_weight, "d weight")
+    # and of the confidences beside a mean
+    gc = torch.where(exact(hidden, weight, labels).sure, size_of * sign, 0.0)
+    up = torch.tensor(2.0 ** -9 * n, device="cuda")
+    _by_size(hidden, weight, labels, VocabConfig(), up, gc, group, frozen_head)
+    # all alike, a few decades down, and tokens without any
+    near = torch.exp2(-5.0 * (group % 2)) * sign * (group != 3)
+    _by_size(hidden, weight, labels, VocabConfig(reduction="none"), near, torch.zeros(n, device="cuda"), group, frozen_head)
+
+
+def test_float16_infinite_upstream_gradient_stays_in_its_token() -> None:
+    n = 60
+    hidden, weight, labels = inputs(n, 64, 3000, F16, seed=18)
+    go = torch.exp2(-1.0 * (torch.arange(n, device="cuda") % 20))
+    h = hidden.clone().requires_grad_(True)
+    loss = vocab_loss(h, weight, labels, VocabConfig(reduction="none"))
+    (want,) = torch.autograd.grad(loss, h, go, retain_graph=True)
+    for wild in (float("inf"), float("nan")):
+        go[7] = wild
+        (got,) = torch.autograd.grad(loss, h, go, retain_graph=True)
+        keep = torch.arange(n, device="cuda") != 7
+        assert not torch.isfinite(got[7]).any()
+        ref = exact(hidden[keep], weight, labels[keep], reduction="none", grad_loss=go[keep])
+        _within(got[keep], ref.d_hidden, ref.tol_hidden, f"d hidden beside {wild}")
+        assert torch.isfinite(want[keep]).all()
