@@ -1,6 +1,6 @@
 // Host side of the vocabulary loss (ace_vocab_forward / ace_vocab_backward,
-// declared in include/ace_hip.h): argument checks, the choice of tiles, the
-// layout of the workspace, and the launches.  Nothing here allocates, copies
+// declared in include/ace_hip.h): argument checks and the launches; the choice of
+// tiles and the layout of the workspace are ace_vocab_plan.hpp's.  Nothing here allocates, copies
 // or synchronises.
 #include "ace_vocab.hpp"
 
@@ -103,155 +103,7 @@ __global__ __launch_bounds__(256) void join_kernel(JoinParams p) {
   if (tid == 0) *p.loss = (float)(p.reduction == 0 ? s_sum[0] / (count > 0 ? count : 1) : s_sum[0]);
 }
 
-constexpr int kCus = 256;
-constexpr int64_t kMaxTokens = (int64_t)1 << 30, kMaxVocab = (int64_t)1 << 30;
-constexpr int64_t kMaxHidden = (int64_t)1 << 20;
-// Bytes of dS that one piece of the vocabulary may take: what the last-level
-// cache holds.
-constexpr int64_t kPieceBytes = (int64_t)256 << 20;
-
-int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
-int64_t parts(int64_t x, int64_t of) { return (x + of - 1) / of; }
 int elem_size(int dtype) { return dtype == ACE_F32 ? 4 : 2; }
-
-// Rates of the tiles relative to each other, measured on large products: with 16
-// bits 1146, 870 and less (TFLOP/s), which small tiles lose to the traffic of LDS;
-// with float32 the matrix cores alone bound them (125 to 140).
-float rate_of(int es, int tile) {
-  constexpr float half[kTiles] = {1.2f, 0.85f, 0.65f, 0.4f}, single[kTiles] = {0.95f, 1.f, 0.95f, 0.85f};
-  return es == 2 ? half[tile] : single[tile];
-}
-
-// The tile for m x n results: the one that takes the least time, counting what
-// its edges waste.  `whole`: tiles are not cut, so that a round of blocks counts
-// in full however few they are.
-int pick_tile(int es, int64_t m, int64_t n, bool whole, int first = kTile256) {
-  int best = first;
-  double least = 0.0;
-  for (int t = first; t < kTiles; ++t) {
-    const TileShape s = kShape[t];
-    const double slots = (double)kCus * s.per_cu;
-    double rounds = (double)(parts(m, s.bm) * parts(n, s.bn)) / slots;
-    if (whole) rounds = (double)(int64_t)(rounds + 1.0 - 1e-9);
-    const double cost = rounds * s.per_cu * s.bm * s.bn / rate_of(es, t);
-    if (t == first || cost < least) {
-      best = t;
-      least = cost;
-    }
-  }
-  return best;
-}
-
-// Most parts that mma::deal makes of at most `tiles` tiles.
-int64_t parts_of(int blocks, int rounds, int64_t tiles) {
-  const int64_t cut = (int64_t)blocks * rounds;
-  return tiles > cut ? tiles : cut;
-}
-
-struct Cursor {  // lays out a workspace
-  size_t at = 0;
-  size_t take(size_t bytes) {
-    const size_t here = at;
-    at += (bytes + 255) / 256 * 256;
-    return here;
-  }
-};
-
-// Everything that follows from the sizes alone.
-struct Plan {
-  int64_t n, h, v, width;
-  int es;
-  bool pad;            // the weight's rows are copied to a padded width
-  int score_tile, score_blocks;
-  int prep_blocks, prep_per, join_blocks;
-  // backward
-  int64_t piece;       // words of a piece (a multiple of 256)
-  int dscore_blocks;
-  int dh_tile, dh_blocks;
-  int dw_tile, dw_blocks;
-  bool dw_seg;
-  int64_t dh_segs, dw_segs;
-};
-
-Plan make_plan(int dtype, int64_t n, int64_t h, int64_t v) {
-  Plan p{};
-  p.n = n;
-  p.h = h;
-  p.v = v;
-  p.es = elem_size(dtype);
-  p.width = up(h, 16 / p.es);
-  p.pad = p.width != h;
-  p.score_tile = pick_tile(p.es, v, n, true);
-  const auto blocks_of = [](int tile, int64_t tiles) {
-    const int64_t most = (int64_t)kCus * kShape[tile].per_cu;
-    return (int)(tiles < most ? (tiles > 0 ? tiles : 1) : most);
-  };
-  const TileShape st = kShape[p.score_tile];
-  p.score_blocks = blocks_of(p.score_tile, parts(v, st.bm) * parts(n, st.bn));
-  p.prep_per = (int)parts(n > 0 ? n : 1, kPrepBlocks);
-  p.prep_blocks = (int)parts(n > 0 ? n : 1, p.prep_per);
-  p.join_blocks = (int)(n < 4 * kPrepBlocks ? parts(n > 0 ? n : 1, 4) : kPrepBlocks);
-  // equal pieces, of no more than kPieceBytes unless a piece would be narrow
-  int64_t most = kPieceBytes / ((n > 0 ? n : 1) * p.es) / 256 * 256;
-  if (most < 2048) most = 2048;
-  p.piece = up(parts(v, parts(v, most)), 256);
-  p.dscore_blocks = blocks_of(p.score_tile, parts(p.piece, st.bm) * parts(n, st.bn));
-  p.dh_tile = pick_tile(p.es, p.width, n, false);
-  const TileShape ht = kShape[p.dh_tile];
-  const int64_t dh_tiles = parts(p.width, ht.bm) * parts(n, ht.bn);
-  p.dh_blocks = blocks_of(p.dh_tile, dh_tiles * parts(p.piece, mma::kStepBytes / p.es));
-  p.dh_segs = parts_of(p.dh_blocks, kGradRounds, dh_tiles);
-  // few tokens: what is written bounds it, and blocks that share a CU overlap
-  p.dw_tile = pick_tile(p.es, p.width, p.piece, true, n > 256 ? kTile256 : kTile128);
-  // the tokens are shared out as well where whole tiles leave half of the CUs idle
-  p.dw_seg = n >= 512 && parts(p.width, 128) * parts(p.piece, 128) < kCus;
-  if (p.dw_seg) p.dw_tile = kTile128;
-  const TileShape wt = kShape[p.dw_tile];
-  const int64_t dw_tiles = parts(p.width, wt.bm) * parts(p.piece, wt.bn);
-  p.dw_blocks = p.dw_seg ? kCus * wt.per_cu : blocks_of(p.dw_tile, dw_tiles);
-  p.dw_segs = p.dw_seg ? parts_of(p.dw_blocks, kGradRounds, dw_tiles) : 0;
-  return p;
-}
-
-struct ForwardSpace {
-  size_t zeros, ticket, rows, weight, part, label_logit, sums, bytes;
-};
-ForwardSpace forward_space(const Plan& p) {
-  Cursor c;
-  ForwardSpace s{};
-  const TileShape st = kShape[p.score_tile];
-  s.zeros = c.take(16);
-  s.ticket = c.take(4);
-  s.sums = c.take((size_t)p.join_blocks * 8);
-  s.label_logit = c.take((size_t)p.n * 4);
-  const size_t score_parts = parts_of(p.score_blocks, kScoreRounds, parts(p.n, st.bn));
-  s.part = c.take(score_parts * st.bn * sizeof(Part));
-  s.rows = c.take((size_t)(p.n * p.width) * p.es);
-  s.weight = c.take(p.pad ? (size_t)(p.v * p.width) * p.es : 0);
-  s.bytes = c.at;
-  return s;
-}
-
-struct BackwardSpace {
-  size_t zeros, scale, bound, g, c, rows, weight, ds, dh, dw, bytes;
-};
-BackwardSpace backward_space(const Plan& p) {
-  Cursor c;
-  BackwardSpace s{};
-  const TileShape ht = kShape[p.dh_tile], wt = kShape[p.dw_tile];
-  s.zeros = c.take(16);
-  s.scale = c.take(8);
-  s.bound = c.take((size_t)p.prep_blocks * 8);
-  s.g = c.take((size_t)p.n * 4);
-  s.c = c.take((size_t)p.n * 4);
-  s.rows = c.take((size_t)(p.n * p.width) * p.es);
-  s.weight = c.take(p.pad ? (size_t)(p.v * p.width) * p.es : 0);
-  s.ds = c.take((size_t)(p.n * p.piece) * p.es);
-  s.dh = c.take((size_t)p.dh_segs * ht.bm * ht.bn * 4);
-  s.dw = c.take((size_t)p.dw_segs * wt.bm * wt.bn * 4);
-  s.bytes = c.at;
-  return s;
-}
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
@@ -482,7 +334,7 @@ size_t ace_vocab_workspace_bytes(int dtype, int64_t tokens, int64_t hidden_size,
   if (tokens < 0 || hidden_size < 1 || vocab < 1 || tokens > kMaxTokens || vocab > kMaxVocab ||
       hidden_size > kMaxHidden)
     return 0;
-  const Plan p = make_plan(dtype, tokens, hidden_size, vocab);
+  const Plan p = make_plan(elem_size(dtype), tokens, hidden_size, vocab);
   return backward ? backward_space(p).bytes : forward_space(p).bytes;
 }
 
@@ -495,7 +347,7 @@ int ace_vocab_forward(const void* hidden, const void* weight, int dtype, const i
   if (bad) return bad;
   if ((!labels && tokens > 0) || (!loss && (tokens > 0 || reduction != ACE_RED_NONE)))
     return ACE_EINVAL;
-  const Plan p = make_plan(dtype, tokens, hidden_size, vocab);
+  const Plan p = make_plan(elem_size(dtype), tokens, hidden_size, vocab);
   if (workspace_bytes < forward_space(p).bytes) return ACE_EWORKSPACE;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -520,7 +372,7 @@ int ace_vocab_backward(const void* hidden, const void* weight, int dtype, int64_
       check(hidden, weight, dtype, tokens, hidden_size, vocab, reduction, saved, workspace);
   if (bad) return bad;
   if (!aligned16(d_hidden) || !aligned16(d_weight)) return ACE_EINVAL;
-  const Plan p = make_plan(dtype, tokens, hidden_size, vocab);
+  const Plan p = make_plan(elem_size(dtype), tokens, hidden_size, vocab);
   if (workspace_bytes < backward_space(p).bytes) return ACE_EWORKSPACE;
   const hipStream_t s = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);

@@ -42,6 +42,7 @@
 #include <atomic>
 
 #include "ace_mma.hpp"
+#include "ace_vocab_plan.hpp"
 
 namespace ace {
 namespace vocab {
@@ -51,7 +52,6 @@ using mma::kStep;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kNone = 0x7fffffff;  // no index
-constexpr int kPrepBlocks = 512;   // most blocks of the kernels that walk tokens
 
 // What a forward leaves for its backward, in one allocation of 4-byte words:
 // the number of counted tokens (`rows`), then n words each of
@@ -111,6 +111,7 @@ struct Part {
   float top, sum;
   int best, pad;
 };
+static_assert(sizeof(Part) == kPartBytes, "the workspace holds them");
 
 // Both take NaN along.
 __device__ inline float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
@@ -262,7 +263,6 @@ struct ScoreParams {
 // walk the same few vocabulary tiles at a time (4 to 8 of them and 4 to 8 token
 // tiles): 1250 TFLOP/s at 8192 x 4096 x 65536, against 995 where each block had a
 // run of vocabulary tiles of its own.
-constexpr int kScoreRounds = 4;
 __device__ inline mma::Deal score_deal(int tts, int vts, int blocks) {
   return mma::deal(tts, vts, blocks, 0, kScoreRounds);
 }
@@ -655,11 +655,6 @@ struct GradParams {
   const char* zeros;
 };
 
-// A part of a tile costs its partial tile's way to memory and back: about as long
-// as this many steps of k.
-template <typename T>
-constexpr int kPartSteps = sizeof(T) == 2 ? 24 : 8;
-constexpr int kGradRounds = 2;
 
 // dh (DW = false): C[h][row] = sum over words of w[v][h] ds[row][v];
 // dw (DW = true):  C[h][v] = sum over rows of rows[row][h] ds[row][v].
@@ -682,7 +677,7 @@ __global__ __launch_bounds__(TL::kThreads, TL::kWaves) void grad_kernel(GradPara
   const int ks = DW ? all : (int)((p.k_map + kStep<T> - 1) / kStep<T>);
   if (nts == 0) return;
   const int blocks = (int)gridDim.x;
-  const mma::Deal d = p.seg ? mma::deal(mts * nts, ks, blocks, kPartSteps<T>, kGradRounds)
+  const mma::Deal d = p.seg ? mma::deal(mts * nts, ks, blocks, part_steps(sizeof(T)), kGradRounds)
                             : mma::Deal{mts * nts, 1};
   const int start = mma::xcd_order((int)blockIdx.x, blocks);
 
@@ -805,7 +800,7 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
   const int k = DW ? count : (int)p.k_map;
   const int mts = ((int)p.m + p.bm - 1) / p.bm, nts = ((int)nn + p.bn - 1) / p.bn;
   const int ks = (k + kStep<T> - 1) / kStep<T>;
-  const mma::Deal d = mma::deal(mts * nts, ks, p.grad_blocks, kPartSteps<T>, kGradRounds);
+  const mma::Deal d = mma::deal(mts * nts, ks, p.grad_blocks, part_steps(sizeof(T)), kGradRounds);
   const float inv = p.scale ? 1.f / *p.scale : 1.f;
   const bool by_row = p.g && p.scale[1] != 0.f;
   const uint32_t quads = (uint32_t)((p.hidden_size + 3) / 4);
@@ -878,13 +873,6 @@ __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
 
 // ------------------------------------------------------------------ launches
 
-// The tiles that are built: vocabulary (or hidden) x tokens (or vocabulary).
-enum { kTile256 = 0, kTile128 = 1, kTile64 = 2, kTile32 = 3, kTiles = 4 };
-struct TileShape {
-  int bm, bn, per_cu;  // per_cu: blocks of it whose LDS fits one of the 256 CUs
-};
-constexpr TileShape kShape[kTiles] = {{256, 256, 1}, {128, 128, 2}, {128, 64, 3}, {128, 32, 2}};
-
 // Implemented per element type by ACE_DEFINE_VOCAB in the ace_k_vocab_*.hip
 // units.
 template <typename T>
@@ -919,8 +907,9 @@ inline hipError_t launch(int blocks, int threads, size_t lds, hipStream_t s, con
 
 template <typename T, bool AKC, bool BKC, bool PAIRED = false, typename F>
 inline hipError_t with_tile(int tile, F f) {
+  if constexpr (sizeof(T) == 2)
+    if (tile == kTile256) return f(mma::Tile<T, 256, 256, 2, 4, AKC, BKC, PAIRED>{});
   switch (tile) {
-    case kTile256: return f(mma::Tile<T, 256, 256, 2, 4, AKC, BKC, PAIRED>{});
     case kTile128: return f(mma::Tile<T, 128, 128, 2, 2, AKC, BKC, PAIRED>{});
     case kTile64: return f(mma::Tile<T, 128, 64, 4, 1, AKC, BKC, PAIRED>{});
     default: return f(mma::Tile<T, 128, 32, 4, 1, AKC, BKC, PAIRED>{});

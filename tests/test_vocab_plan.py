@@ -1,0 +1,77 @@
+"""The plan of the vocabulary loss on the CPU (``ace_vocab_plan.hpp``, compiled here
+with g++): the tiles that sizes lead to, and the workspace that they need."""
+
+from __future__ import annotations
+
+import ctypes
+import random
+import re
+import subprocess
+from collections import namedtuple
+from pathlib import Path
+from typing import Set, Tuple
+
+import pytest
+
+from ace_kernels import _lib
+from test_vocab_isa import _code_objects
+
+HERE = Path(__file__).resolve().parent
+CSRC = HERE.parent / "ace-kernels_amd" / "csrc"
+Plan = namedtuple("Plan", "score dh dw dw_parts pieces pad piece dh_blocks dh_segs dw_blocks dw_segs score_blocks "
+                          "dscore_blocks forward_bytes backward_bytes")
+
+
+@pytest.fixture(scope="module")
+def harness(tmp_path_factory) -> ctypes.CDLL:
+    out = tmp_path_factory.mktemp("vocab") / "libvocab.so"
+    subprocess.run(["g++", "-O2", "-shared", "-fPIC", "-std=c++17", f"-I{CSRC}", str(HERE / "vocab_harness.cpp"), "-o", str(out)],
+                   check=True, capture_output=True)
+    lib = ctypes.CDLL(str(out))
+    ll, i = ctypes.c_longlong, ctypes.c_int
+    lib.vocab_plan.argtypes = [i, ll, ll, ll, ctypes.POINTER(ll)]
+    lib.vocab_plan.restype = None
+    lib.vocab_parts.argtypes = [i] * 5
+    lib.vocab_parts.restype = ll
+    lib.vocab_score_parts.argtypes = [i, ll, ll, ll]
+    lib.vocab_score_parts.restype = ll
+    return lib
+
+
+def plan_of(lib, es, n, h, v) -> Plan:
+    out = (ctypes.c_longlong * 15)()
+    lib.vocab_plan(es, n, h, v, out)
+    return Plan(*out)
+
+
+def shape(lib, tile) -> Tuple[int, int]:
+    bm, bn = ctypes.c_int(), ctypes.c_int()
+    lib.vocab_tile(tile, ctypes.byref(bm), ctypes.byref(bn))
+    return bm.value, bn.value
+
+
+def _sizes():
+    """Tokens, hidden sizes and vocabularies over what a card holds."""
+    for n in sorted({int(2 ** (i / 3)) for i in range(60)}):
+        for h in (1, 8, 64, 200, 512, 1024, 4096, 16384):
+            for v in sorted({int(2 ** (i / 2)) for i in range(42)}):
+                if h * v < 2 ** 36:
+                    yield n, h, v
+
+
+def test_every_kernel_that_is_built_is_chosen_by_some_size(harness) -> None:
+    chosen: Set[Tuple[str, str, int, int]] = set()
+    for letter, es in (("f", 4), ("DF16_", 2), ("DF16b", 2)):
+        for sizes in _sizes():
+            p = plan_of(harness, es, *sizes)
+            chosen |= {("score", letter, *shape(harness, p.score)), ("dscore", letter, *shape(harness, p.score)),
+                       ("dh", letter, *shape(harness, p.dh)), ("dw", letter, *shape(harness, p.dw))}
+    built = set()
+    for elf in _code_objects(_lib.LIB_PATH):
+        for m in re.finditer(rb"_ZN3ace5vocab\d+(score|dscore|grad)_kernelINS_3mma4TileI(f|DF16_|DF16b)Li(\d+)ELi(\d+)E([^\0]*?)\.kd", elf):
+            kernel = m[1].decode()
+            if kernel == "grad":
+                kernel = "dw" if b"ELb1EEEv" in m[5] else "dh"
+            built.add((kernel, m[2].decode(), int(m[3]), int(m[4])))
+    assert built, "no kernels found"
+    assert built == chosen, f"never chosen: {sorted(built - chosen)}; not built: {sorted(chosen - built)}"
