@@ -75,3 +75,50 @@ def test_every_kernel_that_is_built_is_chosen_by_some_size(harness) -> None:
             built.add((kernel, m[2].decode(), int(m[3]), int(m[4])))
     assert built, "no kernels found"
     assert built == chosen, f"never chosen: {sorted(built - chosen)}; not built: {sorted(chosen - built)}"
+
+
+def _kernels(p: Plan) -> Set[Tuple]:
+    """What a call runs that the numerics could depend on: each kernel's tile, whether
+    the weight's gradient is cut along the tokens, in one or several pieces of the
+    vocabulary; rows padded or not."""
+    many = p.pieces > 1
+    return {("score", p.score, many), ("dh", p.dh, many), ("dw", p.dw, bool(p.dw_parts), many), ("padded", bool(p.pad), many)}
+
+
+@pytest.mark.parametrize("es", [2, 4])
+def test_gpu_cases_take_every_kernel(harness, es) -> None:
+    from test_gpu_vocab_plans import PLANS
+
+    chosen: Set[Tuple] = set()
+    for sizes in [*_sizes(), *PLANS[es]]:
+        chosen |= _kernels(plan_of(harness, es, *sizes))
+    tested: Set[Tuple] = set()
+    for sizes in PLANS[es]:
+        tested |= _kernels(plan_of(harness, es, *sizes))
+    assert tested == chosen, f"not tested: {sorted(chosen - tested, key=str)}"
+
+
+@pytest.mark.parametrize("es", [2, 4])
+def test_the_workspace_holds_the_parts(harness, es) -> None:
+    """Whatever the number of counted tokens, which the device alone knows, and in
+    the last, shorter piece of the vocabulary too."""
+    rng = random.Random(es)
+    step = 64 // es
+    for _ in range(3000):
+        n, h, v = (int(2 ** rng.uniform(0, top)) for top in (17, 13, 19))
+        p = plan_of(harness, es, n, h, v)
+        width = -(-h * es // 16) * 16 // es
+        assert p.piece % 256 == 0 and (p.pieces - 1) * p.piece < v <= p.pieces * p.piece
+        bm, bn = shape(harness, p.score)
+        assert harness.vocab_score_parts(es, n, h, v) >= -(-n // bn)
+        for count in {1, n, rng.randint(1, n), rng.randint(1, n)}:
+            tts = -(-count // bn)
+            assert harness.vocab_parts(0, es, tts, -(-v // bm), p.score_blocks) <= harness.vocab_score_parts(es, n, h, v)
+            hm, hn = shape(harness, p.dh)
+            units = -(-min(p.piece, v) // step)
+            assert harness.vocab_parts(1, es, -(-width // hm) * -(-count // hn), units, p.dh_blocks) <= p.dh_segs
+            if p.dw_parts:
+                wm, wn = shape(harness, p.dw)
+                for words in {min(p.piece, v), v - (p.pieces - 1) * p.piece}:
+                    tiles = -(-width // wm) * -(-words // wn)
+                    assert harness.vocab_parts(2, es, tiles, -(-count // step), p.dw_blocks) <= p.dw_segs
