@@ -282,3 +282,32 @@ def test_second_derivative_in_the_upstream_gradient_is_refused() -> None:
     (g,) = torch.autograd.grad(loss, leaf, up, create_graph=True)
     with pytest.raises(RuntimeError, match="only once"):
         torch.autograd.grad(g.sum(), up, allow_unused=True)
+
+
+def test_scores_past_32_bit_offsets() -> None:
+    """Five groups of 2^20 tokens and 512 experts, 2.7 G scores: each group is what it is
+    alone, the last one's elements beyond 2^31."""
+    gen = torch.Generator(device="cuda").manual_seed(1)
+    x = torch.empty(5, 1 << 20, 512, dtype=BF16, device="cuda").normal_(generator=gen)
+    mask = torch.rand(5, 1 << 20, device="cuda", generator=gen) < 0.9
+    cfg = BalanceConfig(top_k=4, reduction="none")
+    leaf = x.requires_grad_(True)
+    out = balance_loss(leaf, cfg, mask)
+    up = torch.tensor([1.0, 2.0, 3.0, 4.0, 5.0], device="cuda") * 2.0 ** 20
+    (grad,) = torch.autograd.grad(out.loss, leaf, up)
+    for g in (0, 4):
+        one = x[g].detach().requires_grad_(True)
+        alone = balance_loss(one, cfg, mask[g])
+        (want,) = torch.autograd.grad(alone.loss, one, up[g])
+        assert torch.equal(out.counts[g], alone.counts)
+        # blocks sum in another order: 4 sqrt(T) u each
+        assert abs(out.loss[g].item() - alone.loss.item()) <= 8 * 1024 * U * alone.loss.item()
+        assert torch.equal(grad[g], want)  # a token's gradient is its own: the counts are the same
+    # the last group's last tokens, from the definition
+    n, m = out.counts[4].double(), mask[4].sum().double()
+    p = torch.softmax(x[4, -1000:].detach().double(), 1)
+    q = 512 * n / (4 * m * m)
+    pull = (p * q).sum(1, keepdim=True)
+    want = float(up[4]) * p * (q - pull) * mask[4, -1000:, None]
+    tol = float(up[4]) * p * (q + pull) * (2 * 16 * U * 12 + 4 * 512 ** 0.5 * U) + 2.0 ** -8 * want.abs()
+    assert ((grad[4, -1000:].double() - want).abs() <= tol).all()

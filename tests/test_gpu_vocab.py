@@ -473,3 +473,80 @@ def test_float16_infinite_upstream_gradient_stays_in_its_token() -> None:
         ref = exact(hidden[keep], weight, labels[keep], reduction="none", grad_loss=go[keep])
         _within(got[keep], ref.d_hidden, ref.tol_hidden, f"d hidden beside {wild}")
         assert torch.isfinite(want[keep]).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32], ids=["bf16", "f32"])
+def test_weights_past_32_bit_offsets(dtype) -> None:
+    """600000 words of 4096: the last words' elements are beyond 2^31.  Labels at both
+    ends; gradients against the definition in float64, word by word at the ends."""
+    n, size, v = 5, 4096, 600000
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    weight = torch.empty(v, size, dtype=dtype, device="cuda").normal_(std=1 / 64, generator=gen)
+    hidden = torch.randn(n, size, device="cuda", generator=gen).to(dtype)
+    labels = torch.tensor([0, 1, v // 2, v - 2, v - 1], device="cuda")
+    hidden = (hidden.float() + 5 * weight[labels].float() * 8).to(dtype).requires_grad_(True)
+    w = weight.requires_grad_(True)
+    out = vocab_loss_confidence(hidden, w, labels, VocabConfig(reduction="none"))
+    up = torch.ones(n, device="cuda")
+    dh, dw = torch.autograd.grad((out.loss, out.confidence), (hidden, w), (up, -0.5 * up))
+    with torch.no_grad():
+        h = hidden.double()
+        s = torch.cat([h @ weight[i:i + 50000].double().t() for i in range(0, v, 50000)], 1)
+        most = float(torch.stack([(h.abs() @ weight[i:i + 50000].double().abs().t()).max() for i in range(0, v, 50000)]).max())
+        e = 2 * (4 * size ** 0.5 * U * most) + 16 * U * (1 + float(s.max() - s.min()))  # as in vocab_reference.py
+        lse = torch.logsumexp(s, 1)
+        here = torch.arange(n, device="cuda")
+        _within(out.loss, lse - s[here, labels], e + 2 * U * lse, "loss")
+        p = torch.exp(s - lse[:, None])
+        best = s.argmax(1)
+        conf = p[here, best]
+        _within(out.confidence, conf, e * conf, "confidence")
+        c = -0.5 * conf
+        ds, size_ds = (1 - c)[:, None] * p, (1 + c.abs())[:, None] * p
+        ds[here, labels] -= 1
+        ds[here, best] += c
+        size_ds[here, labels] += 1
+        size_ds[here, best] += c.abs()
+        half = torch.finfo(dtype).eps / 2
+        rel = 3 * e + (half if dtype != F32 else 0)
+        for words in (slice(0, 300), slice(v // 2 - 100, v // 2 + 100), slice(v - 300, v)):
+            want, tol = ds[:, words].t() @ h, rel * (size_ds[:, words].t() @ h.abs())
+            _within(dw[words], want, tol * (1 + half) + half * want.abs() + 1e-30, f"d weight {words}")
+        want, tol = torch.zeros_like(h), torch.zeros_like(h)
+        for i in range(0, v, 50000):
+            part = weight[i:i + 50000].double()
+            want += ds[:, i:i + 50000] @ part
+            tol += (rel + 4 * v ** 0.5 * U) * (size_ds[:, i:i + 50000] @ part.abs())
+        _within(dh, want, tol * (1 + half) + half * want.abs(), "d hidden")
+
+
+def test_captured_float16_step_with_upstream_gradients_near_and_far_apart() -> None:
+    """One graph: whether the rows of dS take scales of their own is the device's to
+    say, anew in every replay."""
+    n = 100
+    hidden, weight, labels = inputs(n, 64, 3000, F16, seed=41, ignored=0.1)
+    h, w = hidden.clone().requires_grad_(True), weight.clone().requires_grad_(True)
+    go = torch.ones(n, device="cuda")
+
+    def step():
+        loss = vocab_loss(h, w, labels, VocabConfig(reduction="none"))
+        return [loss, *torch.autograd.grad(loss, (h, w), go)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    far = torch.exp2(10.0 - 5.0 * (torch.arange(n, device="cuda") % 5))
+    for up in (torch.ones(n, device="cuda"), far, 0.5 * torch.ones(n, device="cuda"), far.flip(0), torch.zeros(n, device="cuda")):
+        go.copy_(up)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in held]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+        want = exact(hidden, weight, labels, reduction="none", grad_loss=up)
+        _within(got[1], want.d_hidden, want.tol_hidden, "d hidden")
