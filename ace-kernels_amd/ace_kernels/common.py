@@ -60,6 +60,19 @@ def _refuse_under_capture(device: torch.device, what: str) -> None:
         )
 
 
+def _kept(*tensors: torch.Tensor) -> None:
+    """Refuses to keep what a ``torch.func`` transform or a fake-tensor mode hands out
+    in a tensor's place: it has no memory of its own, and every later call that found
+    it here would fail."""
+    for t in tensors:
+        if type(t) is not torch.Tensor or torch._C._functorch.is_functorch_wrapped_tensor(t):
+            raise RuntimeError(
+                "ace_kernels: the call's device buffers do not exist yet and cannot be created inside a "
+                "torch.func transform or a fake-tensor mode; run one ordinary call of the same "
+                "configuration on this stream first"
+            )
+
+
 def bin_tables(num_bins: int, soft: bool, device: torch.device) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
     """(bucket table, centre table or None) as float32 tensors on ``device``.
 
@@ -82,6 +95,7 @@ def bin_tables(num_bins: int, soft: bool, device: torch.device) -> Tuple[torch.T
             sentinel = torch.full((1,), 10000.0)
             repl = torch.cat((-sentinel, half[1::2].repeat_interleave(2), sentinel))
             out = (half[1:].contiguous().to(device), repl.contiguous().to(device))
+        _kept(*(t for t in out if t is not None))
         _TABLES[key] = out
         return out
 
@@ -115,6 +129,7 @@ def class_weight_tensor(weights: Tuple[float, ...], device: torch.device,
         if hit is None:
             _refuse_under_capture(device, "the class-weight tensor")
             hit = torch.tensor(key[0], dtype=dtype, device=device)
+            _kept(hit)
             _CLASS_WEIGHTS[key] = hit
         return hit
 
@@ -150,10 +165,12 @@ def workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
             return buf
         if capturing(device):
             own = torch.zeros(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+            _kept(own)
             _RETIRED.append(own)
             return own
         size = max(int(nbytes), 1 << 16, 2 * (buf.numel() if buf is not None else 0))
         new = torch.zeros(size, dtype=torch.uint8, device=device)
+        _kept(new)
         if buf is not None:
             _RETIRED.append(buf)
         _WORKSPACES[key] = new

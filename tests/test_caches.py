@@ -66,3 +66,40 @@ def test_nothing_is_created_during_capture(monkeypatch: pytest.MonkeyPatch) -> N
         common.bin_tables(3001, False, dev)
     with pytest.raises(RuntimeError, match="graph capture"):
         common.class_weight_tensor((3.0, 4.0), dev)
+
+
+def _under(transform, call):
+    """``call`` inside a transform, or a mode, that makes tensors of its own kind."""
+    from torch._subclasses import FakeTensorMode
+
+    def f(x):
+        call()
+        return (x * 1.0).sum()
+
+    x = torch.ones(3)
+    if transform == "fake":
+        with FakeTensorMode():
+            call()
+    elif transform == "jvp":
+        torch.func.jvp(f, (x,), (x,))
+    else:
+        {"grad": torch.func.grad, "functionalize": torch.func.functionalize}[transform](f)(x)
+
+
+@pytest.mark.parametrize("transform", ["grad", "jvp", "functionalize", "fake"])
+def test_nothing_that_a_transform_made_is_kept(transform) -> None:
+    """A first call inside a transform is refused, and later ones find nothing of it."""
+    dev = torch.device("cpu")
+    n = ["grad", "jvp", "functionalize", "fake"].index(transform)
+    calls = {
+        "workspace": lambda: common.workspace(dev, 5550000 + n, 100),
+        "table": lambda: common.bin_tables(701 + n, True, dev)[0],
+        "weights": lambda: common.class_weight_tensor((0.25, 3.0 + n), dev),
+    }
+    for what, call in calls.items():
+        with pytest.raises(RuntimeError, match="ordinary call"):
+            _under(transform, call)
+        t = call()
+        assert type(t) is torch.Tensor and not torch._C._functorch.is_functorch_wrapped_tensor(t), what
+        assert t.data_ptr() and t.numel() > 0
+        _under(transform, call)  # it is there now
