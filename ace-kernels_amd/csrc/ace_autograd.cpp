@@ -297,9 +297,15 @@ int dtype_code(const at::Tensor& t) {
   }
 }
 
-// t contiguous and starting at a multiple of 16 bytes.
+// t contiguous, its memory holding its values: not their negatives, as the memory of
+// a tensor with the negative bit (the imaginary part of a conjugate) does.
+at::Tensor plain(const at::Tensor& t) {
+  return t.is_neg() ? t.resolve_neg().contiguous() : t.contiguous();
+}
+
+// That and starting at a multiple of 16 bytes.
 at::Tensor dense(const at::Tensor& t) {
-  at::Tensor c = t.contiguous();
+  at::Tensor c = plain(t);
   return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
 }
 
@@ -308,7 +314,7 @@ at::Tensor scratch(const at::Tensor& like, size_t bytes) {
 }
 
 at::Tensor float32(const at::Tensor& g) {
-  return g.defined() ? g.to(at::kFloat).contiguous() : at::Tensor();
+  return g.defined() ? plain(g.to(at::kFloat)) : at::Tensor();
 }
 
 // Gradients of a backward that is itself recorded (create_graph) refuse to be
@@ -390,7 +396,7 @@ std::vector<at::Tensor> vocab_loss(const at::Tensor& hidden, const at::Tensor& w
   {
     const at::NoGradGuard no_grad;
     const at::Tensor x = dense(hidden.reshape({-1, size})), w = dense(weight);
-    const at::Tensor y = labels.to(at::kLong).contiguous();
+    const at::Tensor y = plain(labels.to(at::kLong));
     const auto f32 = hidden.options().dtype(at::kFloat).requires_grad(false);
     const int code = dtype_code(hidden);
     out.push_back(reduction == ACE_RED_NONE ? at::empty(labels.sizes(), f32) : at::empty({}, f32));
@@ -433,7 +439,7 @@ struct BalanceLossBackward : public Node {
     {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(logits.device());
-      const at::Tensor x = logits.contiguous(), go = float32(grads[0]);
+      const at::Tensor x = plain(logits), go = float32(grads[0]);
       const at::Tensor m = mask.defined() ? mask.contiguous() : mask;
       out[0] = at::empty(logits.sizes(), logits.options().requires_grad(false));
       const int rc = g_balance_backward.load()(
@@ -470,7 +476,7 @@ std::vector<at::Tensor> balance_loss(const at::Tensor& logits, const std::option
   at::Tensor loss, counts, share;
   {
     const at::NoGradGuard no_grad;
-    const at::Tensor x = logits.contiguous();
+    const at::Tensor x = plain(logits);
     const at::Tensor m = mask ? mask->contiguous() : at::Tensor();
     const auto options = logits.options().requires_grad(false);
     std::vector<int64_t> lead(logits.sizes().begin(), logits.sizes().end() - 2);

@@ -311,3 +311,13 @@ def test_scores_past_32_bit_offsets() -> None:
     want = float(up[4]) * p * (q - pull) * mask[4, -1000:, None]
     tol = float(up[4]) * p * (q + pull) * (2 * 16 * U * 12 + 4 * 512 ** 0.5 * U) + 2.0 ** -8 * want.abs()
     assert ((grad[4, -1000:].double() - want).abs() <= tol).all()
+
+
+def test_negative_bit() -> None:
+    """Scores whose memory holds the negatives of their values."""
+    x = _scores((2,), 50, 16, F32)
+    want, grad = _compare(x, 3)
+    leaf = torch._neg_view(-x).requires_grad_(True)
+    out = balance_loss(leaf, BalanceConfig(top_k=3))
+    (got,) = torch.autograd.grad(out.loss, leaf, torch._neg_view(torch.tensor(-0.7, device="cuda")))
+    assert torch.equal(out.loss, want.loss) and torch.equal(out.counts, want.counts) and torch.equal(got, grad)

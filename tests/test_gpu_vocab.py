@@ -550,3 +550,17 @@ def test_captured_float16_step_with_upstream_gradients_near_and_far_apart() -> N
             assert torch.equal(a, b)
         want = exact(hidden, weight, labels, reduction="none", grad_loss=up)
         _within(got[1], want.d_hidden, want.tol_hidden, "d hidden")
+
+
+def test_negative_bit() -> None:
+    """Tensors whose memory holds the negatives of their values."""
+    hidden, weight, labels = inputs(40, 64, 300, F32, seed=5)
+    want, (dh, dw) = _step(hidden, weight, labels, VocabConfig(), torch.tensor(0.5, device="cuda"))
+    h, w, y = (torch._neg_view(-t) for t in (hidden, weight, labels))
+    assert h.is_neg() and h.is_contiguous() and y.is_neg()
+    h.requires_grad_(True)
+    w.requires_grad_(True)
+    loss = vocab_loss(h, w, y)
+    up = torch._neg_view(torch.tensor(-0.5, device="cuda"))
+    a, b = torch.autograd.grad(loss, (h, w), up)
+    assert torch.equal(loss, want.loss) and torch.equal(a, dh) and torch.equal(b, dw)
