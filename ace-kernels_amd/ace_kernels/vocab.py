@@ -34,7 +34,7 @@ from __future__ import annotations
 from typing import List, Literal, NamedTuple, Optional
 
 import torch
-from pydantic import BaseModel, ConfigDict
+from pydantic import BaseModel, ConfigDict, Field
 
 from ace_kernels import _lib
 
@@ -54,7 +54,7 @@ class VocabConfig(BaseModel):
 
     model_config = ConfigDict(frozen=True, extra="forbid")
 
-    ignore_index: int = -100
+    ignore_index: int = Field(default=-100, ge=-(2**63), lt=2**63)  # an int64, as the labels are
     reduction: Literal["mean", "sum", "none"] = "mean"
 
 

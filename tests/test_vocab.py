@@ -127,3 +127,11 @@ def test_tangents_are_refused() -> None:
         for a, b in ((fwd.make_dual(h, torch.ones_like(h)), w), (h, fwd.make_dual(w, torch.ones_like(w)))):
             with pytest.raises(NotImplementedError, match="vocab_loss has no forward-mode derivative"):
                 _lib.autograd().vocab_loss(a, b, y, -100, _lib.RED_MEAN, False)
+
+
+def test_ignore_index_is_an_int64() -> None:
+    for good in (-(2 ** 63), -1, 0, 2 ** 63 - 1):
+        assert VocabConfig(ignore_index=good).ignore_index == good
+    for bad in (2 ** 63, -(2 ** 63) - 1, 2 ** 70):
+        with pytest.raises(ValidationError):
+            VocabConfig(ignore_index=bad)
