@@ -128,8 +128,20 @@ inline Plan make_plan(int es, int64_t n, int64_t h, int64_t v) {
   p.dh_segs = parts_of(p.dh_blocks, kGradRounds, dh_tiles);
   // few tokens: what is written bounds it, and blocks that share a CU overlap
   p.dw_tile = pick_tile(p.es, p.width, p.piece, true, n > 256 ? kTile256 : kTile128);
-  // the tokens are shared out as well where whole tiles leave half of the CUs idle
-  p.dw_seg = n >= 512 && parts(p.width, 128) * parts(p.piece, 128) < kCus;
+  // The tokens are shared out as well (cut) where whole tiles leave CUs idle for long
+  // enough to pay for partial tiles and a launch more: 128 x 128 tiles for less than
+  // all CUs, and the more steps of k the more CUs the smallest tiles fill by themselves.
+  // Where the 128 x 128 tiles alone fill most CUs, float32, which the matrix cores
+  // bound, gains from a cut early, 16 bits late.  Backward in us, whole / cut:
+  //   bfloat16 512 x 512 x 4000 words 55 / 70, 2048: 89 / 94, 4096: 131 / 122, 9000: 248 /
+  //   202; 1500 x 64 x 1000 46 / 45, 2048: 53 / 46; 2500 x 256 x 12000 118 / 129, 9000: 306 / 310
+  //   float32 1024 x 512 x 4000 151 / 157, 2048: 252 / 247; 768 x 64 x 1000 54 / 52, 1500: 80 /
+  //   59; 512 x 256 x 12000 132 / 136, 1500: 310 / 281
+  const int64_t tiles = parts(p.width, 128) * parts(p.piece, 128);
+  const int64_t small = parts(p.width, 128) * parts(p.piece, 32), filled = small < kCus ? small : kCus;
+  const bool most_cus = p.es == 4 ? 2 * tiles > kCus : 8 * tiles > 5 * kCus;
+  const int64_t steps = most_cus ? (p.es == 4 ? 48 : 192) : 34 + filled / 4;
+  p.dw_seg = tiles < kCus && parts(n, mma::kStepBytes / p.es) >= steps;
   if (p.dw_seg) p.dw_tile = kTile128;
   const TileShape wt = kShape[p.dw_tile];
   const int64_t dw_tiles = parts(p.width, wt.bm) * parts(p.piece, wt.bn);

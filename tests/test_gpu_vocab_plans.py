@@ -35,7 +35,7 @@ PLANS = {
         (70, 24, 52061),     # all of 128
         (3, 72, 66001),      # score and dw 64, dh 32
         (2, 13, 16483),      # dw 64
-        (600, 40, 700),      # dw by tokens
+        (1300, 40, 700),     # dw by tokens
         (5, 88, 900),        # score and dw 32
     ],
     4: [
@@ -48,7 +48,7 @@ PLANS = {
         (207, 36, 331423),   # score 32, dw 128, two pieces
         (5621, 10, 11887),   # score and dh 128, two pieces
         (1111, 262, 20011),  # all of 128
-        (600, 40, 700),      # dw by tokens
+        (1300, 40, 700),     # dw by tokens
         (5, 88, 900),        # score and dw 32
         (3, 7, 33001),       # dw 64
     ],

@@ -122,3 +122,14 @@ def test_the_workspace_holds_the_parts(harness, es) -> None:
                 for words in {min(p.piece, v), v - (p.pieces - 1) * p.piece}:
                     tiles = -(-width // wm) * -(-words // wn)
                     assert harness.vocab_parts(2, es, tiles, -(-count // step), p.dw_blocks) <= p.dw_segs
+
+
+@pytest.mark.parametrize("es,n,h,v,cut", [
+    (2, 512, 512, 4000, False), (2, 768, 320, 5003, False), (2, 1024, 1024, 1000, False), (2, 2048, 512, 4000, False),
+    (2, 4096, 512, 4000, True), (2, 4096, 1024, 1000, True), (2, 9000, 320, 5003, True), (2, 2048, 64, 1000, True),
+    (2, 512, 64, 1000, False), (2, 512, 128, 2000, False), (4, 512, 512, 4000, False), (4, 1024, 320, 5003, False),
+    (4, 1024, 1024, 700, False), (4, 2048, 256, 12000, True), (4, 2048, 1024, 1000, True), (4, 1024, 64, 1000, True),
+    (4, 1024, 128, 2000, True), (4, 350, 128, 2000, False), (4, 512, 256, 12000, False), (4, 1500, 256, 12000, True),
+    (2, 2500, 256, 12000, False), (2, 5000, 1024, 3000, False), (2, 5000, 256, 9000, True), (4, 1024, 256, 9000, True)])
+def test_the_weights_gradient_is_cut_along_the_tokens_where_that_was_measured_faster(harness, es, n, h, v, cut) -> None:
+    assert bool(plan_of(harness, es, n, h, v).dw_parts) == cut
