@@ -160,7 +160,6 @@ int forward(const Plan& p, const void* hidden, const void* weight, const int64_t
     r.weight = static_cast<const char*>(weight);
     r.rows = ws + at.rows;
     r.vocab = p.v;
-    r.hidden_size = (int)p.h;
     r.width = (int)p.width;
     r.saved = q.saved;
     r.zeros = q.zeros;
@@ -226,7 +225,6 @@ int backward(const Plan& p, const void* hidden, const void* weight, int reductio
     r.weight = static_cast<const char*>(weight);
     r.rows = ws + at.rows;
     r.vocab = p.v;
-    r.hidden_size = (int)p.h;
     r.width = (int)p.width;
     r.saved = q.copy.saved;
     r.zeros = q.copy.zeros;

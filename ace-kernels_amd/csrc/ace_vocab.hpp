@@ -35,7 +35,6 @@
 #pragma once
 
 #include <float.h>
-#include <hip/hip_ext.h>
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
@@ -235,7 +234,7 @@ struct ScoreParams {
   const char* weight;  // [vocab, width]
   const char* rows;    // [n, width]
   int64_t vocab;
-  int hidden_size, width;
+  int width;
   Saved saved;
   const char* zeros;
   // forward
