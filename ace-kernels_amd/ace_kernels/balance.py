@@ -16,7 +16,9 @@ Leading dimensions are groups with a loss of their own: ``[layers, tokens, E]`` 
 every layer's router of a step, ``[batch, tokens, E]`` a balance per sequence.  A
 group without counted tokens has loss 0 and gradient 0.
 
-The call and its backward node are C++ (``csrc/ace_autograd.cpp``).
+The call and its backward node are C++ (``csrc/ace_autograd.cpp``).  They have no
+forward-mode and no second derivative, and ``torch.func`` transforms do not know them;
+``torch.compile`` breaks its graph at them.
 """
 
 from __future__ import annotations

@@ -23,8 +23,16 @@ differentiable, so the calibration loss trains the model through it.
 Tokens whose label is ``ignore_index``, or any number outside the vocabulary,
 are not counted: their loss, confidence, correctness and gradients are 0 and
 their hidden states are not read (they may be NaN).  The mean is over the counted
-tokens, and 0 where there are none.  Logits, sums and gradients accumulate in
-float32; the gradients have the inputs' type, the losses are float32.
+tokens, and 0 where there are none.  Logits and all sums are float32, and so are the
+losses; the gradients have the inputs' type.  In bfloat16 and float16 the gradient of
+each logit is rounded to that type before it is multiplied with the weight and the
+hidden states (half a step: 2^-8, 2^-11), as a product in that type does.  In float16
+it is scaled first, so that small probabilities count: for the hidden gradient by
+each token's own upstream gradient (to within a factor of 64), for the weight's by the
+tokens' largest, beside which entries below 2^-38 are lost.
+
+The calls have no forward-mode and no second derivative, and ``torch.func`` transforms
+do not know them; ``torch.compile`` breaks its graph at them.
 
 The call and its backward node are C++ (``csrc/ace_autograd.cpp``).
 """

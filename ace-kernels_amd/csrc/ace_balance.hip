@@ -19,8 +19,8 @@ struct Geometry {
 
 Geometry geometry(int64_t groups, int64_t tokens, int experts) {
   Geometry g{};
-  // one lane a token up to 16 experts, then 16 scores a lane up to 64, 32 above:
-  // fewer lanes mean fewer exchanges, more registers
+  // 8 scores a lane up to 8 experts, else 16: fewer lanes mean fewer exchanges, more
+  // registers
   g.c = experts <= 8 ? 8 : 16;
   while ((g.c << g.lanes_log2) < experts) ++g.lanes_log2;
   const int64_t at_once = kThreads >> g.lanes_log2;  // tokens of a block at a time
@@ -28,7 +28,10 @@ Geometry geometry(int64_t groups, int64_t tokens, int experts) {
   int64_t blocks = (kTarget + groups - 1) / groups;
   if (blocks > most) blocks = most;
   if (blocks > kMaxBlocks) blocks = kMaxBlocks;
-  if (blocks < 1 || most <= 4) blocks = 1;  // a few rounds cost less than joining blocks
+  // A few rounds cost less than joining blocks: forward in us with one block a group up
+  // to 1, 4 and 16 rounds, 300 x 200 tokens of 64 experts 26 / 16 / 16, 8 x 512 13 / 13 / 20, 32 x
+  // 1024 16 / 16 / 34, 4 x 1024 of 16 experts 13.7 / 14.8 / 15.1.
+  if (blocks < 1 || most <= 4) blocks = 1;
   const int64_t rounds = (most + blocks - 1) / blocks;
   g.per_block = (rounds > 0 ? rounds : 1) * at_once;
   g.blocks = (int)((tokens + g.per_block - 1) / g.per_block);

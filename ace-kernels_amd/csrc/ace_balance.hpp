@@ -7,9 +7,12 @@
 //   loss = sum_e q_e sum_t p_te,      dl_te = u p_te (q_e - sum_j q_j p_tj)
 //
 // Both directions are one pass over the scores.  The backward is bound by it (131072
-// tokens of 256 experts in float32: 45 us for 268 MB, 6 TB/s), the forward by the
-// work per score (69 us for 134 MB, top 8; 24 us for 32 x 4096 x 64 in bfloat16,
-// top 6).  L lanes share a token, each holding C = 8 (up to 8 experts) or 16 scores
+// tokens of 256 experts in float32: 45 us for 268 MB, 6 TB/s).  The forward (69 us for
+// 134 MB, top 8; 23 us for 32 x 4096 x 64 in bfloat16, top 6; 27 us for 16 x 8191 x 100, top
+// 1) waits: its vector units work for a half, a third and two fifths of that time, and
+// its waves stand still for half of theirs, for their first scores (a wave has two
+// to four rounds of them in the smaller two) and for the blocks' joins, two or three one
+// after another.  L lanes share a token, each holding C = 8 (up to 8 experts) or 16 scores
 // in registers as interleaved 16-byte pieces.  With 32 scores a lane fewer lanes
 // exchange, but half of the waves fit: 158 us instead of 69.
 //

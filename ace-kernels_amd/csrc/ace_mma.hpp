@@ -7,7 +7,7 @@
 //
 // from two operands in device memory that are each stored one of two ways:
 //
-//   k contiguous  rows of k, one per m (or n): LDS holds 128 bytes of k of
+//   k contiguous  rows of k, one per m (or n): LDS holds 64 bytes of k of
 //                 each row, read as 16-byte fragments (ds_read_b128);
 //   m contiguous  rows of m (or n), one per k: LDS holds the rows of one step
 //                 of k, read through the transposing LDS load

@@ -22,12 +22,15 @@
 // matrix cores' operand), one forms the piece's dw, and one adds its part of dh.
 //
 // All sums, the running maxima, the logits and the partial dh are float32.  The one
-// rounding beside the results' own is dS's to the inputs' type, half a step of each
-// entry (2^-9 relatively in bfloat16 at most twice that): the gradients' errors
-// against 64 bits are 1.1 times those of a gradient that is only rounded at the end.
+// rounding beside the results' own is dS's to the inputs' type, at most half a step of
+// each entry (2^-8 of it in bfloat16, 2^-11 in float16), because the matrix cores take
+// both operands of a product in one type: two products of halves of dS would keep more
+// digits for twice the time.  The gradients' errors against 64 bits are 1.15 to 1.2
+// times those of a gradient that is only rounded at the end (8192 x 4096 x 65536 in
+// bfloat16: 1.93e-3 against 1.66e-3 of the gradient's norm).
 //
 // What bounds it: the matrix cores.  8192 tokens (5 % ignored) x 4096 x 65536 words
-// in bfloat16 take 13.4 ms for four products of 4.2 TFLOP, 1.2 PFLOP/s, the rate
+// in bfloat16 take 13.2 ms for four products of 4.2 TFLOP, 1.27 PFLOP/s, the rate
 // of the library's products of this size (1.1 to 1.4 PFLOP/s); the logits are
 // formed twice because they are not kept.  With few tokens it is the weight, which
 // is read three times and whose gradient is written: 96 tokens x 2048 x 50304 words
@@ -790,7 +793,9 @@ struct FinishParams {
 // out = the sum of each tile's partial tiles in order, in the output's type.  Where
 // there are many for few results (few tokens, a long vocabulary), eight threads share
 // a group of four values: 20 tokens of a hidden size of 256 have 1280 such groups
-// of up to 384 parts, which took one thread each 29 us, and takes eight 7 us.
+// of up to 384 parts, which took one thread each 29 us, and takes eight 7 us.  Backward
+// in us with the rule, always one thread, always eight: 4 x 256 x 40000 38 / 45 / 38, 60 x 512
+// x 11000 38 / 43 / 38, 1000 x 256 x 4000 69 / 68 / 79, 2048 x 1024 x 32768 411 / 409 / 431.
 template <typename T, bool DW>
 __global__ __launch_bounds__(256) void finish_kernel(FinishParams p) {
   __shared__ f32x4 s_sum[8][32];

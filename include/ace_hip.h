@@ -273,6 +273,12 @@ int ace_forward_noalloc(const void* x, int x_dtype, const void* target,
  * confidence or correct); either may be NULL, for 0.  It may be called any
  * number of times on one `saved`.
  *
+ * Sums are float32.  In ACE_BF16 and ACE_F16 the gradient of each logit is rounded
+ * to that type (half a step) before its products with weight and hidden.  ACE_F16
+ * scales it first: for d_hidden by each token's own upstream gradient (to within a
+ * factor of 64), for d_weight by the tokens' largest, of which entries below 2^-38 are
+ * lost.
+ *
  * The workspace (ace_vocab_workspace_bytes, backward 0 or 1, 16-byte aligned)
  * needs no clearing and holds nothing between calls; calls that overlap need
  * one each.  Both calls are asynchronous on `stream`, allocate nothing and can
