@@ -14,7 +14,7 @@ from pathlib import Path
 
 LIB_PATH = Path(os.environ.get("ACE_HIP_LIB", Path(__file__).resolve().with_name("libace_hip.so")))
 
-ABI_VERSION = 9
+ABI_VERSION = 10
 
 # enums of include/ace_hip.h
 F32, BF16, F16, F64 = 0, 1, 2, 3
@@ -51,6 +51,18 @@ EXPORTS = (
     "ace_balance_ticket_bytes",
     "ace_balance_forward",
     "ace_balance_backward",
+    "ace_logprob_saved_bytes",
+    "ace_logprob_workspace_bytes",
+    "ace_logprob_ticket_bytes",
+    "ace_logprob_forward",
+    "ace_logprob_backward",
+    "ace_route_forward",
+    "ace_route_backward",
+    "ace_expert_order_workspace_bytes",
+    "ace_expert_order",
+    "ace_to_experts",
+    "ace_from_experts",
+    "ace_from_experts_backward",
 )
 
 # ace_forward_noalloc's scratch (ACE_NOALLOC_SCRATCH_BYTES) and its error code
@@ -206,6 +218,38 @@ def lib() -> ctypes.CDLL:
         _i64, _i64, _i64,          # groups, tokens, experts
         _i, _p, _p, _p, _p,        # reduction, share, grad_loss, d_logits, stream
     ]
+    handle.ace_logprob_saved_bytes.restype = _sz
+    handle.ace_logprob_saved_bytes.argtypes = [_i64]
+    handle.ace_logprob_workspace_bytes.restype = _sz
+    handle.ace_logprob_workspace_bytes.argtypes = [_i, _i64, _i64, _i]
+    handle.ace_logprob_ticket_bytes.restype = _sz
+    handle.ace_logprob_ticket_bytes.argtypes = [_i, _i64, _i64]
+    handle.ace_logprob_forward.restype = _i
+    handle.ace_logprob_forward.argtypes = [
+        _p, _i, _i64, _p,          # logits, dtype, stride, tokens
+        _i64, _i64, _i64, _f, _i,  # rows, vocab, ignore_index, temperature, top
+        _p, _p, _p, _p, _p,        # saved, logprob, entropy, top_logprobs, top_tokens
+        _p, _sz, _p, _sz, _p,      # tickets, bytes, workspace, bytes, stream
+    ]
+    handle.ace_logprob_backward.restype = _i
+    handle.ace_logprob_backward.argtypes = [
+        _p, _i, _i64, _i64, _i64,  # logits, dtype, stride, rows, vocab
+        _f, _p, _p, _p, _p, _p,    # temperature, saved, grads, d_logits, stream
+    ]
+    handle.ace_route_forward.restype = _i
+    handle.ace_route_forward.argtypes = [_p, _i, _p, _i64, _i64, _i, _i, _p, _p, _p]
+    handle.ace_route_backward.restype = _i
+    handle.ace_route_backward.argtypes = [_p, _i, _i64, _i64, _i, _i, _p, _p, _p, _p, _p]
+    handle.ace_expert_order_workspace_bytes.restype = _sz
+    handle.ace_expert_order_workspace_bytes.argtypes = [_i64, _i64]
+    handle.ace_expert_order.restype = _i
+    handle.ace_expert_order.argtypes = [_p, _i64, _i64, _p, _p, _p, _p, _sz, _p]
+    handle.ace_to_experts.restype = _i
+    handle.ace_to_experts.argtypes = [_p, _i, _i64, _i64, _i64, _p, _p, _p, _p]
+    handle.ace_from_experts.restype = _i
+    handle.ace_from_experts.argtypes = [_p, _i, _i64, _i64, _i64, _p, _p, _p, _p]
+    handle.ace_from_experts_backward.restype = _i
+    handle.ace_from_experts_backward.argtypes = [_p, _p, _i, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]
     handle.ace_set_launch_events.restype = _i
     handle.ace_set_launch_events.argtypes = [_p, _p]
     handle.ace_set_test_hooks.restype = _i
@@ -249,6 +293,12 @@ def autograd():
                             addr(handle.ace_vocab_forward), addr(handle.ace_vocab_backward),
                             addr(handle.ace_balance_workspace_bytes), addr(handle.ace_balance_forward),
                             addr(handle.ace_balance_backward))
+    mod.set_expert_entry_points(addr(handle.ace_route_forward), addr(handle.ace_route_backward),
+                                addr(handle.ace_expert_order_workspace_bytes), addr(handle.ace_expert_order),
+                                addr(handle.ace_to_experts), addr(handle.ace_from_experts),
+                                addr(handle.ace_from_experts_backward))
+    mod.set_logprob_entry_points(addr(handle.ace_logprob_saved_bytes), addr(handle.ace_logprob_workspace_bytes),
+                                 addr(handle.ace_logprob_forward), addr(handle.ace_logprob_backward))
     return mod
 
 

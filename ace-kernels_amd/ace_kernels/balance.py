@@ -31,7 +31,7 @@ import torch
 from pydantic import BaseModel, ConfigDict, Field
 
 from ace_kernels import _lib
-from ace_kernels.common import capturing, workspace
+from ace_kernels.common import tickets
 from ace_kernels.impls.hip_mi355x import _stream
 
 _DTYPES = (torch.float32, torch.bfloat16, torch.float16)
@@ -89,15 +89,6 @@ def _ticket_bytes(groups: int, tokens: int, experts: int) -> int:
     return _lib.lib().ace_balance_ticket_bytes(groups, tokens, experts)
 
 
-def _tickets(device: torch.device, nbytes: int) -> torch.Tensor:
-    """Zeroed counters that the call leaves zero: the stream's workspace, or in a
-    capture counters of its own, cleared by the graph, so that replays of
-    different graphs share none."""
-    if capturing(device):
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return workspace(device, _stream(device), nbytes)
-
-
 def balance_loss(logits: torch.Tensor, config: BalanceConfig,
                  mask: Optional[torch.Tensor] = None) -> BalanceLoss:
     """The balance loss of router scores ``[..., tokens, E]`` (float32, bfloat16
@@ -108,6 +99,6 @@ def balance_loss(logits: torch.Tensor, config: BalanceConfig,
     dev = logits.device
     tokens, experts = logits.shape[-2:]
     groups = math.prod(logits.shape[:-2])
-    tickets = _tickets(dev, _ticket_bytes(groups, tokens, experts))
+    zeros = tickets(dev, _stream(dev), _ticket_bytes(groups, tokens, experts))
     return BalanceLoss(*_lib.autograd().balance_loss(logits, mask, groups, config.top_k,
-                                                     _REDUCTIONS[config.reduction], tickets))
+                                                     _REDUCTIONS[config.reduction], zeros))

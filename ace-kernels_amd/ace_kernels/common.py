@@ -175,3 +175,12 @@ def workspace(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
             _RETIRED.append(buf)
         _WORKSPACES[key] = new
         return new
+
+
+def tickets(device: torch.device, stream: int, nbytes: int) -> torch.Tensor:
+    """Zeroed counters that the call leaves zero: the stream's workspace, or in a
+    capture counters of its own, cleared by the graph, so that replays of
+    different graphs share none."""
+    if capturing(device):
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return workspace(device, stream, nbytes)

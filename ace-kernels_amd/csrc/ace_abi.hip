@@ -509,7 +509,7 @@ using namespace ace;
 
 extern "C" {
 
-int ace_abi_version(void) { return 9; }
+int ace_abi_version(void) { return 10; }
 
 const char* ace_error_string(int code) {
   switch (code) {

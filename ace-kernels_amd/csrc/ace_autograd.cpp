@@ -12,9 +12,11 @@
 // module and the ctypes binding drive the same loaded library.  Host code
 // only: it builds with g++ against torch's headers.
 //
-// The vocabulary losses (ace_kernels/vocab.py) and the balance loss
-// (ace_kernels/balance.py) have their calls and nodes here too, for any
-// arguments: the Python side checks them, nothing is remembered between calls.
+// The vocabulary losses (ace_kernels/vocab.py), the balance loss
+// (ace_kernels/balance.py), the token log probabilities (ace_kernels/logprobs.py) and
+// the experts' operators (ace_kernels/experts.py) have their calls and nodes here
+// too, for any arguments: the Python side checks them, nothing is remembered between
+// calls.
 #include <ATen/DeviceGuard.h>
 #include <c10/core/AutogradState.h>
 #include <torch/csrc/autograd/function.h>
@@ -523,6 +525,374 @@ void set_lm_entry_points(uintptr_t vocab_saved, uintptr_t vocab_workspace, uintp
   g_balance_backward.store(reinterpret_cast<decltype(&ace_balance_backward)>(balance_backward));
 }
 
+// ------------------------------------------------ token log probabilities
+std::atomic<decltype(&ace_logprob_saved_bytes)> g_logprob_saved{nullptr};
+std::atomic<decltype(&ace_logprob_workspace_bytes)> g_logprob_workspace{nullptr};
+std::atomic<decltype(&ace_logprob_forward)> g_logprob_forward{nullptr};
+std::atomic<decltype(&ace_logprob_backward)> g_logprob_backward{nullptr};
+
+// t as rows of its last dimension, whose elements are neighbours: a view wherever the
+// strides allow one.
+at::Tensor as_rows(const at::Tensor& t) {
+  at::Tensor r = (t.is_neg() ? t.resolve_neg() : t).reshape({-1, t.size(-1)});
+  return r.size(1) == 1 || r.stride(1) == 1 ? r : r.contiguous();
+}
+
+struct TokenLogprobsBackward : public Node {
+  std::string name() const override { return "TokenLogprobsBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(1);
+    const at::Tensor &gl = grads[0], &ge = grads[1];
+    if (!gl.defined() && !ge.defined()) return out;
+    refuse_tangents({gl, ge}, "token_logprobs's gradient");
+    const at::Tensor logits = logits_.unpack(), saved = saved_.unpack();
+    {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(logits.device());
+      const at::Tensor x = as_rows(logits), l = float32(gl), e = float32(ge);
+      out[0] = at::empty(logits.sizes(), logits.options().requires_grad(false));
+      const int rc = g_logprob_backward.load()(
+          x.data_ptr(), dtype_code(logits), x.stride(0), x.size(0), x.size(1), temperature,
+          saved.data_ptr(), l.defined() ? l.data_ptr<float>() : nullptr,
+          e.defined() ? e.data_ptr<float>() : nullptr, out[0].data_ptr(), current_stream(logits));
+      if (rc) fail(rc, "ace_logprob_backward");
+    }
+    refuse_second_derivative(out, {logits, gl, ge}, "token_logprobs");
+    return out;
+  }
+
+  void release_variables() override {
+    logits_.reset_data();
+    saved_.reset_data();
+  }
+
+  float temperature = 1.f;
+  SavedVariable logits_, saved_;
+};
+
+// (logprob, entropy), and with top > 0 (.., top_logprobs, top_tokens), of checked
+// arguments; `tickets`: zero, left zero, where the sizes need them.
+std::vector<at::Tensor> token_logprobs(const at::Tensor& logits, const at::Tensor& tokens,
+                                       int64_t ignore_index, float temperature, int top,
+                                       const std::optional<at::Tensor>& tickets) {
+  if (!g_logprob_forward.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  refuse_tangents({logits}, "token_logprobs");
+  const bool record = torch::autograd::compute_requires_grad(logits);
+  const c10::DeviceGuard guard(logits.device());
+  std::vector<at::Tensor> out;
+  at::Tensor saved;
+  {
+    const at::NoGradGuard no_grad;
+    const at::Tensor x = as_rows(logits), y = plain(tokens.to(at::kLong));
+    const int64_t rows = x.size(0), vocab = x.size(1);
+    const int code = dtype_code(logits);
+    const auto f32 = logits.options().dtype(at::kFloat).requires_grad(false);
+    for (int i = 0; i < 2; ++i) out.push_back(at::empty(tokens.sizes(), f32));
+    if (top > 0) {
+      std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+      shape.push_back(top);
+      out.push_back(at::empty(shape, f32));
+      out.push_back(at::empty(shape, f32.dtype(at::kLong)));
+    }
+    saved = scratch(logits, g_logprob_saved.load()(rows));
+    const size_t need = g_logprob_workspace.load()(code, rows, vocab, top);
+    const at::Tensor ws = need ? scratch(logits, need) : at::Tensor();
+    const int rc = g_logprob_forward.load()(
+        x.data_ptr(), code, x.stride(0), y.data_ptr<int64_t>(), rows, vocab, ignore_index,
+        temperature, top, saved.data_ptr(), out[0].data_ptr<float>(), out[1].data_ptr<float>(),
+        top > 0 ? out[2].data_ptr<float>() : nullptr,
+        top > 0 ? out[3].data_ptr<int64_t>() : nullptr, tickets ? tickets->data_ptr() : nullptr,
+        tickets ? (size_t)tickets->numel() : 0, ws.defined() ? ws.data_ptr() : nullptr, need,
+        current_stream(logits));
+    if (rc) fail(rc, "ace_logprob_forward");
+  }
+  if (record) {
+    auto node = std::shared_ptr<TokenLogprobsBackward>(new TokenLogprobsBackward(),
+                                                       torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->temperature = temperature;
+    node->logits_ = SavedVariable(logits, false);
+    node->saved_ = SavedVariable(saved, false);
+    for (int i = 0; i < 2; ++i) torch::autograd::set_history(out[i], node);
+  }
+  return out;
+}
+
+void set_logprob_entry_points(uintptr_t saved, uintptr_t workspace, uintptr_t forward,
+                              uintptr_t backward) {
+  g_logprob_saved.store(reinterpret_cast<decltype(&ace_logprob_saved_bytes)>(saved));
+  g_logprob_workspace.store(reinterpret_cast<decltype(&ace_logprob_workspace_bytes)>(workspace));
+  g_logprob_forward.store(reinterpret_cast<decltype(&ace_logprob_forward)>(forward));
+  g_logprob_backward.store(reinterpret_cast<decltype(&ace_logprob_backward)>(backward));
+}
+
+// ------------------------------------------------------------------ experts
+std::atomic<decltype(&ace_route_forward)> g_route_forward{nullptr};
+std::atomic<decltype(&ace_route_backward)> g_route_backward{nullptr};
+std::atomic<decltype(&ace_expert_order_workspace_bytes)> g_order_workspace{nullptr};
+std::atomic<decltype(&ace_expert_order)> g_order{nullptr};
+std::atomic<decltype(&ace_to_experts)> g_to_experts{nullptr};
+std::atomic<decltype(&ace_from_experts)> g_from_experts{nullptr};
+std::atomic<decltype(&ace_from_experts_backward)> g_from_experts_backward{nullptr};
+
+struct RouteTokensBackward : public Node {
+  std::string name() const override { return "RouteTokensBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(1);
+    if (!grads[0].defined()) return out;
+    refuse_tangents({grads[0]}, "route_tokens's gradient");
+    const at::Tensor logits = logits_.unpack(), chosen = chosen_.unpack(),
+                     weights = weights_.unpack();
+    {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(logits.device());
+      // normalised weights' gradient reads no score
+      const at::Tensor x = normalize ? logits : plain(logits), g = float32(grads[0]);
+      out[0] = at::empty(logits.sizes(), logits.options().requires_grad(false));
+      const int rc = g_route_backward.load()(
+          x.data_ptr(), dtype_code(logits), tokens, logits.size(-1), top_k, normalize,
+          chosen.data_ptr<int64_t>(), weights.data_ptr<float>(), g.data_ptr<float>(),
+          out[0].data_ptr(), current_stream(logits));
+      if (rc) fail(rc, "ace_route_backward");
+    }
+    refuse_second_derivative(out, {logits, grads[0]}, "route_tokens");
+    return out;
+  }
+
+  void release_variables() override {
+    logits_.reset_data();
+    chosen_.reset_data();
+    weights_.reset_data();
+  }
+
+  int64_t tokens = 0;
+  int top_k = 0, normalize = 0;
+  SavedVariable logits_, chosen_, weights_;
+};
+
+// (experts, weights) of checked arguments.
+std::vector<at::Tensor> route_tokens(const at::Tensor& logits, const std::optional<at::Tensor>& mask,
+                                     int top_k, bool normalize) {
+  if (!g_route_forward.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  refuse_tangents({logits}, "route_tokens");
+  const bool record = torch::autograd::compute_requires_grad(logits);
+  const c10::DeviceGuard guard(logits.device());
+  at::Tensor chosen, weights;
+  int64_t tokens = 0;
+  {
+    const at::NoGradGuard no_grad;
+    const at::Tensor x = plain(logits);
+    const at::Tensor m = mask ? mask->contiguous() : at::Tensor();
+    std::vector<int64_t> shape(logits.sizes().begin(), logits.sizes().end());
+    shape.back() = top_k;
+    const auto options = logits.options().requires_grad(false);
+    chosen = at::empty(shape, options.dtype(at::kLong));
+    weights = at::empty(shape, options.dtype(at::kFloat));
+    tokens = weights.numel() / top_k;
+    const int rc = g_route_forward.load()(
+        x.data_ptr(), dtype_code(logits),
+        m.defined() ? static_cast<const uint8_t*>(m.data_ptr()) : nullptr, tokens, logits.size(-1),
+        top_k, normalize, chosen.data_ptr<int64_t>(), weights.data_ptr<float>(),
+        current_stream(logits));
+    if (rc) fail(rc, "ace_route_forward");
+  }
+  if (record) {
+    auto node = std::shared_ptr<RouteTokensBackward>(new RouteTokensBackward(),
+                                                     torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(logits));
+    node->tokens = tokens;
+    node->top_k = top_k;
+    node->normalize = normalize;
+    node->logits_ = SavedVariable(logits, false);
+    node->chosen_ = SavedVariable(chosen, false);
+    // not the result itself, which will hold the node; it shares the version that
+    // tells of changes in place
+    node->weights_ = SavedVariable(weights.detach(), false);
+    torch::autograd::set_history(weights, node);
+  }
+  return {chosen, weights};
+}
+
+// (offsets, source, place) of checked arguments.
+std::vector<at::Tensor> expert_order(const at::Tensor& experts, int64_t num_experts) {
+  if (!g_order.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(experts.device());
+  const at::Tensor chosen = plain(experts.to(at::kLong));
+  const auto options = chosen.options();
+  const int64_t slots = chosen.numel();
+  const at::Tensor offsets = at::empty({num_experts + 1}, options);
+  const at::Tensor source = at::empty({slots}, options), place = at::empty(experts.sizes(), options);
+  const size_t need = g_order_workspace.load()(slots, num_experts);
+  const at::Tensor ws = need ? scratch(chosen, need) : at::Tensor();
+  const int rc = g_order.load()(chosen.data_ptr<int64_t>(), slots, num_experts,
+                                offsets.data_ptr<int64_t>(), source.data_ptr<int64_t>(),
+                                place.data_ptr<int64_t>(), ws.defined() ? ws.data_ptr() : nullptr,
+                                need, current_stream(chosen));
+  if (rc) fail(rc, "ace_expert_order");
+  return {offsets, source, place};
+}
+
+const int64_t* last_offset(const at::Tensor& offsets) {
+  return offsets.data_ptr<int64_t>() + offsets.numel() - 1;
+}
+
+struct ToExpertsBackward : public Node {
+  std::string name() const override { return "ToExpertsBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(1);
+    const at::Tensor& g = grads[0];
+    if (!g.defined()) return out;
+    refuse_tangents({g}, "to_experts's gradient");
+    const at::Tensor place = place_.unpack();
+    {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(g.device());
+      const at::Tensor rows = plain(g);
+      out[0] = at::empty(shape, g.options().requires_grad(false));
+      const int64_t top_k = place.size(-1);
+      const int rc = g_from_experts.load()(rows.data_ptr(), dtype_code(g), place.numel() / top_k,
+                                           shape.back(), top_k, place.data_ptr<int64_t>(), nullptr,
+                                           out[0].data_ptr(), current_stream(g));
+      if (rc) fail(rc, "ace_from_experts");
+    }
+    refuse_second_derivative(out, {g}, "to_experts");
+    return out;
+  }
+
+  void release_variables() override { place_.reset_data(); }
+
+  std::vector<int64_t> shape;
+  SavedVariable place_;
+};
+
+// The rows of checked arguments.
+at::Tensor to_experts(const at::Tensor& x, const at::Tensor& offsets, const at::Tensor& place) {
+  if (!g_to_experts.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  refuse_tangents({x}, "to_experts");
+  const bool record = torch::autograd::compute_requires_grad(x);
+  const c10::DeviceGuard guard(x.device());
+  at::Tensor rows, at;
+  {
+    const at::NoGradGuard no_grad;
+    const at::Tensor in = plain(x), ends = offsets.contiguous();
+    at = place.contiguous();
+    const int64_t top_k = at.size(-1), width = x.size(-1);
+    rows = at::empty({at.numel(), width}, x.options().requires_grad(false));
+    const int rc = g_to_experts.load()(in.data_ptr(), dtype_code(x), at.numel() / top_k, width,
+                                       top_k, at.data_ptr<int64_t>(), last_offset(ends),
+                                       rows.data_ptr(), current_stream(x));
+    if (rc) fail(rc, "ace_to_experts");
+  }
+  if (record) {
+    auto node = std::shared_ptr<ToExpertsBackward>(new ToExpertsBackward(),
+                                                   torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(x));
+    node->shape.assign(x.sizes().begin(), x.sizes().end());
+    node->place_ = SavedVariable(at, false);
+    torch::autograd::set_history(rows, node);
+  }
+  return rows;
+}
+
+struct FromExpertsBackward : public Node {
+  std::string name() const override { return "FromExpertsBackward"; }
+
+  variable_list apply(variable_list&& grads) override {
+    variable_list out(2);
+    const at::Tensor& g = grads[0];
+    if (!g.defined()) return out;
+    refuse_tangents({g}, "from_experts's gradient");
+    const at::Tensor place = place_.unpack(), offsets = offsets_.unpack(), rows = rows_.unpack(),
+                     weights = weights_.unpack();
+    {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(g.device());
+      const at::Tensor up = plain(g), w = weights.defined() ? plain(weights) : weights;
+      const int64_t top_k = place.size(-1), slots = place.numel(), width = g.size(-1);
+      if (task_should_compute_output(0))
+        out[0] = at::empty({slots, width}, g.options().requires_grad(false));
+      at::Tensor in;
+      if (rows.defined() && task_should_compute_output(1)) {
+        in = plain(rows);
+        out[1] = at::empty(place.sizes(), g.options().dtype(at::kFloat).requires_grad(false));
+      }
+      const int rc = g_from_experts_backward.load()(
+          in.defined() ? in.data_ptr() : nullptr, up.data_ptr(), dtype_code(g), slots / top_k,
+          width, top_k, place.data_ptr<int64_t>(), last_offset(offsets),
+          w.defined() ? w.data_ptr<float>() : nullptr,
+          out[0].defined() ? out[0].data_ptr() : nullptr,
+          out[1].defined() ? out[1].data_ptr<float>() : nullptr, current_stream(g));
+      if (rc) fail(rc, "ace_from_experts_backward");
+    }
+    refuse_second_derivative(out, {rows, weights, g}, "from_experts");
+    return out;
+  }
+
+  void release_variables() override {
+    rows_.reset_data();
+    weights_.reset_data();
+    place_.reset_data();
+    offsets_.reset_data();
+  }
+
+  SavedVariable rows_, weights_, place_, offsets_;
+};
+
+// The tokens' rows of checked arguments.
+at::Tensor from_experts(const at::Tensor& rows, const at::Tensor& offsets, const at::Tensor& place,
+                        const std::optional<at::Tensor>& weights) {
+  if (!g_from_experts.load()) throw std::runtime_error("ace_autograd: entry points not set");
+  const at::Tensor factor = weights ? *weights : at::Tensor();
+  refuse_tangents({rows, factor}, "from_experts");
+  const bool record = torch::autograd::compute_requires_grad(rows, factor);
+  const c10::DeviceGuard guard(rows.device());
+  at::Tensor out, at;
+  {
+    const at::NoGradGuard no_grad;
+    const at::Tensor in = plain(rows), w = factor.defined() ? plain(factor) : factor;
+    at = place.contiguous();
+    const int64_t top_k = at.size(-1), width = rows.size(-1);
+    std::vector<int64_t> shape(at.sizes().begin(), at.sizes().end());
+    shape.back() = width;
+    out = at::empty(shape, rows.options().requires_grad(false));
+    const int rc = g_from_experts.load()(in.data_ptr(), dtype_code(rows), at.numel() / top_k, width,
+                                         top_k, at.data_ptr<int64_t>(),
+                                         w.defined() ? w.data_ptr<float>() : nullptr,
+                                         out.data_ptr(), current_stream(rows));
+    if (rc) fail(rc, "ace_from_experts");
+  }
+  if (record) {
+    auto node = std::shared_ptr<FromExpertsBackward>(new FromExpertsBackward(),
+                                                     torch::autograd::deleteNode);
+    node->set_next_edges(torch::autograd::collect_next_edges(rows, factor));
+    // the rows only for the weights' gradient
+    if (factor.defined() && factor.requires_grad()) node->rows_ = SavedVariable(rows, false);
+    if (factor.defined()) node->weights_ = SavedVariable(factor, false);
+    node->place_ = SavedVariable(at, false);
+    node->offsets_ = SavedVariable(offsets.contiguous(), false);
+    torch::autograd::set_history(out, node);
+  }
+  return out;
+}
+
+void set_expert_entry_points(uintptr_t route_forward, uintptr_t route_backward,
+                             uintptr_t order_workspace, uintptr_t order, uintptr_t to,
+                             uintptr_t from, uintptr_t from_backward) {
+  g_route_forward.store(reinterpret_cast<decltype(&ace_route_forward)>(route_forward));
+  g_route_backward.store(reinterpret_cast<decltype(&ace_route_backward)>(route_backward));
+  g_order_workspace.store(
+      reinterpret_cast<decltype(&ace_expert_order_workspace_bytes)>(order_workspace));
+  g_order.store(reinterpret_cast<decltype(&ace_expert_order)>(order));
+  g_to_experts.store(reinterpret_cast<decltype(&ace_to_experts)>(to));
+  g_from_experts.store(reinterpret_cast<decltype(&ace_from_experts)>(from));
+  g_from_experts_backward.store(
+      reinterpret_cast<decltype(&ace_from_experts_backward)>(from_backward));
+}
+
 std::shared_ptr<LevelSignature> make_level_signature(
     int x_dtype, int64_t batch, int64_t channels, int num_bins, int binning, int include_background,
     int ignore_empty, int reduction, int right, float empty_weight, uintptr_t class_weight,
@@ -618,4 +988,14 @@ PYBIND11_MODULE(_ace_autograd, m) {
   m.def("vocab_loss", &vocab_loss);
   m.def("balance_loss", &balance_loss, pybind11::arg(), pybind11::arg().none(true), pybind11::arg(),
         pybind11::arg(), pybind11::arg(), pybind11::arg());
+  m.def("set_logprob_entry_points", &set_logprob_entry_points);
+  m.def("token_logprobs", &token_logprobs, pybind11::arg(), pybind11::arg(), pybind11::arg(),
+        pybind11::arg(), pybind11::arg(), pybind11::arg().none(true));
+  m.def("set_expert_entry_points", &set_expert_entry_points);
+  m.def("route_tokens", &route_tokens, pybind11::arg(), pybind11::arg().none(true), pybind11::arg(),
+        pybind11::arg());
+  m.def("expert_order", &expert_order);
+  m.def("to_experts", &to_experts);
+  m.def("from_experts", &from_experts, pybind11::arg(), pybind11::arg(), pybind11::arg(),
+        pybind11::arg().none(true));
 }

@@ -43,7 +43,6 @@ namespace balance {
 
 constexpr int kFan = 32;             // partial sums that one block adds
 constexpr int kMaxBlocks = kFan * kFan;  // blocks of a group
-constexpr int kTicketStride = 64;    // words: a counter has a 256-byte line of its own
 constexpr int kMaxExperts = 512;
 constexpr int kMaxTopK = 16;
 
@@ -185,14 +184,12 @@ __device__ inline uint32_t median(uint32_t a, uint32_t b, uint32_t c) {
   return max(min(a, b), min(max(a, b), c));  // v_med3_u32
 }
 
-// The scores' keys and the threshold that the k largest reach: score i is taken
-// where key[i] >= the result.  `on`: the token is counted, its scores are there;
-// others take nothing.  `nans`: some score of the wave may be NaN.
+// The scores' keys, and the K largest of all of a token's in order.  `nans`: some
+// score of the wave may be NaN.
 template <typename T, int C, int K>
-__device__ inline uint32_t choose(const Row<T, C>& row, const T (&x)[C], int lanes, int top_k,
-                                  bool on, bool nans, uint32_t (&key)[C]) {
+__device__ inline void largest(const Row<T, C>& row, const T (&x)[C], int lanes, bool nans,
+                               uint32_t (&key)[C], uint32_t (&list)[K]) {
   constexpr bool numbered = sizeof(T) == 2;
-  uint32_t list[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) list[k] = 0;
 #pragma unroll
@@ -239,6 +236,17 @@ __device__ inline uint32_t choose(const Row<T, C>& row, const T (&x)[C], int lan
   if (lanes > 4) merge(std::integral_constant<int, 4>{});
   if (lanes > 8) merge(std::integral_constant<int, 8>{});
   if (lanes > 16) merge(std::integral_constant<int, 16>{});
+}
+
+// The scores' keys and the threshold that the k largest reach: score i is taken
+// where key[i] >= the result.  `on`: the token is counted, its scores are there;
+// others take nothing.
+template <typename T, int C, int K>
+__device__ inline uint32_t choose(const Row<T, C>& row, const T (&x)[C], int lanes, int top_k,
+                                  bool on, bool nans, uint32_t (&key)[C]) {
+  constexpr bool numbered = sizeof(T) == 2;
+  uint32_t list[K];
+  largest<T, C, K>(row, x, lanes, nans, key, list);
   uint32_t least = list[0];
 #pragma unroll
   for (int k = 1; k < K; ++k) least = k < top_k ? list[k] : least;
@@ -301,23 +309,6 @@ __device__ inline float exponentials(const Row<T, C>& row, const T (&x)[C], int 
     for (int i = 0; i < C; ++i) sum += e[i];
   }
   return 1.f / over_lanes(sum, lanes, kAdd);
-}
-
-// Whether this is the last of `n` blocks to come here; it then sees what the
-// others wrote (device-coherently) before they came, and leaves the counter zero.
-// All threads of the block call it.
-__device__ inline bool last_of(int* counter, int n) {
-  __shared__ int s_last;
-  wait_own_writes();
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    s_last = ticket(counter) == n - 1;
-    if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  }
-  __syncthreads();
-  const bool last = s_last;
-  __syncthreads();
-  return last;
 }
 
 __device__ inline void store_dev(double* p, double v) {

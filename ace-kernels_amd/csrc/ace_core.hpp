@@ -532,6 +532,29 @@ __device__ __forceinline__ unsigned long long xchg_dev(unsigned long long* p, un
 __device__ __forceinline__ int ticket(int* ctr) {
   return __hip_atomic_fetch_add(ctr, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// Orders a wave's own LDS accesses: what its lanes wrote before, they read after.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+constexpr int kTicketStride = 64;  // words: a counter has a 256-byte line of its own
+
+// Whether this is the last of `n` blocks to come here; it then sees what the
+// others wrote (device-coherently) before they came, and leaves the counter zero.
+// All threads of the block call it.
+__device__ inline bool last_of(int* counter, int n) {
+  __shared__ int s_last;
+  wait_own_writes();
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s_last = ticket(counter) == n - 1;
+    if (s_last) __hip_atomic_store(counter, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  const bool last = s_last;
+  __syncthreads();
+  return last;
+}
 
 // Copies the bucket table (padded with -inf / +inf) and the centre table into
 // LDS.

@@ -1,0 +1,175 @@
+// The entry points of tokens sorted by expert and back (declared in
+// include/ace_hip.h): argument checks, launch geometry, instantiations.
+#include "ace_experts.hpp"
+
+#include "ace_hip.h"
+
+namespace ace {
+namespace experts {
+namespace {
+
+constexpr int64_t kMaxSlots = (int64_t)1 << 30;
+constexpr int64_t kMaxWidth = (int64_t)1 << 20;
+constexpr int64_t kMaxWaves = (int64_t)1 << 26;  // a launch has fewer than 2^32 threads
+
+int launched() {
+  const hipError_t e = hipGetLastError();
+  return e == hipSuccess ? ACE_OK : ACE_EHIP + (int)e;
+}
+
+int64_t order_blocks(int64_t slots, int64_t* per_block) {
+  // 4096 slots a block: 16 rounds of a wave; at most kMaxBlocks
+  int64_t each = 4096;
+  if (slots > each * kMaxBlocks) each = (slots + kMaxBlocks - 1) / kMaxBlocks;
+  *per_block = (each + kBlock - 1) / kBlock * kBlock;
+  const int64_t blocks = (slots + *per_block - 1) / *per_block;
+  return blocks < 1 ? 1 : blocks;
+}
+
+int span_of(int dtype) { return dtype == ACE_F32 ? kSpan<float> : kSpan<__bf16>; }
+
+int check(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_k,
+          const int64_t* place) {
+  if (dtype != ACE_F32 && dtype != ACE_BF16 && dtype != ACE_F16) return ACE_EINVAL;
+  if (tokens < 0 || width < 1 || top_k < 1) return ACE_EINVAL;
+  if (tokens > 0 && (!in || !place)) return ACE_EINVAL;
+  if (width > kMaxWidth || top_k > kMaxSlots || tokens > kMaxSlots || tokens * top_k > kMaxSlots)
+    return ACE_EUNSUPPORTED;
+  const int64_t span = span_of(dtype), pieces = (width + span - 1) / span;
+  if (tokens * pieces >= kMaxWaves || tokens * top_k >= kMaxWaves) return ACE_EUNSUPPORTED;
+  return ACE_OK;
+}
+
+RowsParams params(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_k,
+                  const int64_t* place, const float* weights) {
+  RowsParams p{};
+  p.in = in;
+  p.tokens = tokens;
+  p.slots = tokens * top_k;
+  p.width = (int)width;
+  p.top_k = (int)top_k;
+  p.place = place;
+  p.weights = weights;
+  p.pieces = (int)((width + span_of(dtype) - 1) / span_of(dtype));
+  return p;
+}
+
+dim3 grid_of(int64_t waves) { return dim3((unsigned)((waves + kWaves - 1) / kWaves)); }
+
+template <typename T>
+void launch_backward(const RowsParams& p, hipStream_t s) {
+  const dim3 grid = grid_of(p.slots), block(kBlock);
+  if (p.out && p.d_weights)
+    hipLaunchKernelGGL((from_backward_kernel<T, true, true>), grid, block, 0, s, p);
+  else if (p.out)
+    hipLaunchKernelGGL((from_backward_kernel<T, true, false>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((from_backward_kernel<T, false, true>), grid, block, 0, s, p);
+}
+
+}  // namespace
+}  // namespace experts
+}  // namespace ace
+
+using namespace ace::experts;
+
+extern "C" {
+
+size_t ace_expert_order_workspace_bytes(int64_t slots, int64_t experts) {
+  if (slots < 0 || slots > kMaxSlots || experts < 1 || experts > kMaxExperts) return 0;
+  int64_t per_block;
+  const int64_t blocks = order_blocks(slots, &per_block);
+  return blocks > 1 ? (size_t)blocks * (size_t)experts * 4 : 0;
+}
+
+int ace_expert_order(const int64_t* chosen, int64_t slots, int64_t experts, int64_t* offsets,
+                     int64_t* source, int64_t* place, void* workspace, size_t workspace_bytes,
+                     void* stream) {
+  if (slots < 0 || experts < 1 || !offsets) return ACE_EINVAL;
+  if (slots > kMaxSlots || experts > kMaxExperts) return ACE_EUNSUPPORTED;
+  if (slots > 0 && (!chosen || !source || !place)) return ACE_EINVAL;
+  OrderParams p{};
+  p.blocks = (int)order_blocks(slots, &p.per_block);
+  if (p.blocks > 1) {
+    if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 4) return ACE_EINVAL;
+    if (workspace_bytes < ace_expert_order_workspace_bytes(slots, experts)) return ACE_EWORKSPACE;
+  }
+  p.chosen = chosen;
+  p.slots = slots;
+  p.experts = (int)experts;
+  p.counts = static_cast<int*>(workspace);
+  p.offsets = offsets;
+  p.source = source;
+  p.place = place;
+  const dim3 grid((unsigned)p.blocks), block(kBlock);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  if (p.blocks > 1) {
+    hipLaunchKernelGGL(count_kernel, grid, block, 0, s, p);
+    const int rc = launched();
+    if (rc) return rc;
+  }
+  hipLaunchKernelGGL(place_kernel, grid, block, 0, s, p);
+  return launched();
+}
+
+int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width, int64_t top_k,
+                   const int64_t* place, const int64_t* routed, void* rows, void* stream) {
+  const int bad = check(x, dtype, tokens, width, top_k, place);
+  if (bad) return bad;
+  if (tokens == 0) return ACE_OK;
+  if (!routed || !rows) return ACE_EINVAL;
+  RowsParams p = params(x, dtype, tokens, width, top_k, place, nullptr);
+  p.offsets = routed;
+  p.out = rows;
+  const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case ACE_F32: hipLaunchKernelGGL((to_kernel<float>), grid, block, 0, s, p); break;
+    case ACE_BF16: hipLaunchKernelGGL((to_kernel<__bf16>), grid, block, 0, s, p); break;
+    default: hipLaunchKernelGGL((to_kernel<_Float16>), grid, block, 0, s, p);
+  }
+  return launched();
+}
+
+int ace_from_experts(const void* rows, int dtype, int64_t tokens, int64_t width, int64_t top_k,
+                     const int64_t* place, const float* weights, void* out, void* stream) {
+  const int bad = check(rows, dtype, tokens, width, top_k, place);
+  if (bad) return bad;
+  if (tokens == 0) return ACE_OK;
+  if (!out) return ACE_EINVAL;
+  RowsParams p = params(rows, dtype, tokens, width, top_k, place, weights);
+  p.out = out;
+  const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case ACE_F32: hipLaunchKernelGGL((from_kernel<float>), grid, block, 0, s, p); break;
+    case ACE_BF16: hipLaunchKernelGGL((from_kernel<__bf16>), grid, block, 0, s, p); break;
+    default: hipLaunchKernelGGL((from_kernel<_Float16>), grid, block, 0, s, p);
+  }
+  return launched();
+}
+
+int ace_from_experts_backward(const void* rows, const void* grad, int dtype, int64_t tokens,
+                              int64_t width, int64_t top_k, const int64_t* place,
+                              const int64_t* routed, const float* weights, void* d_rows,
+                              float* d_weights, void* stream) {
+  // without the weights' gradient the rows are not read
+  const int bad = check(d_weights ? rows : grad, dtype, tokens, width, top_k, place);
+  if (bad) return bad;
+  if (tokens == 0 || (!d_rows && !d_weights)) return ACE_OK;
+  if (!grad || !routed) return ACE_EINVAL;
+  RowsParams p = params(rows, dtype, tokens, width, top_k, place, weights);
+  p.grad = grad;
+  p.offsets = routed;
+  p.out = d_rows;
+  p.d_weights = d_weights;
+  const hipStream_t s = static_cast<hipStream_t>(stream);
+  switch (dtype) {
+    case ACE_F32: launch_backward<float>(p, s); break;
+    case ACE_BF16: launch_backward<__bf16>(p, s); break;
+    default: launch_backward<_Float16>(p, s);
+  }
+  return launched();
+}
+
+}  // extern "C"

@@ -1,0 +1,462 @@
+// Log probabilities of given tokens from logits, with the entropy and the largest
+// alternatives, and their gradient (ace_logprob_forward / ace_logprob_backward,
+// declared in include/ace_hip.h).  For a row x of V logits, temperature t, token y:
+//
+//   z_v = (x_v - max x) / t,   l = log sum_v exp z_v,   lp_v = z_v - l,   p_v = exp lp_v
+//   logprob = lp_y,            H = -sum_v p_v lp_v = l - sum_v p_v z_v
+//   dx_v = (g [v = y] - p_v (g + h (lp_v + H))) / t
+//
+// with g and h the upstream gradients of logprob and H.  Both directions are one
+// pass over the logits.
+//
+// Forward: a team of one wave (short rows) or four reads a row, or a part of one
+// where there are few rows.  Each lane keeps a running maximum, sum of exp z and sum
+// of z exp z; these are joined across lanes, waves and, through the workspace, the
+// row's parts, by the part that ends last.  Sums are float32 over at most V / 64
+// words a lane.
+//
+// Alternatives: a word's key is its logit's bits in their order above its number's
+// complement, so keys differ and equal logits rank by number, lowest first.  The
+// k-th largest of the lanes' maxima over the team's first words bounds the k-th
+// largest of all from below; only words that reach it are kept as candidates, in
+// LDS, a few dozen in a usual row.  At the end every candidate counts those above
+// it, which is its place.  A wave whose candidates outgrow its LDS (words in
+// ascending order, say) keeps its k best and raises the bound.
+#pragma once
+
+#include <float.h>
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "ace_balance.hpp"  // keys in the scores' order
+#include "ace_core.hpp"     // device-coherent accesses
+
+namespace ace {
+namespace logprob {
+
+using balance::key_of;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr int kBlock = 256;
+constexpr int kPieces = 4;    // of 16 bytes that a lane reads at a time
+constexpr int kMaxTop = 32;
+constexpr int kMaxParts = 32;
+constexpr int kRoom = 256;    // candidates of a wave
+constexpr float kFar = 200.f;  // 2^-200 is 0 in float32: exponents beyond it count as it
+static_assert(kMaxParts * kMaxTop <= kBlock / 64 * kRoom, "the last part has room for all lists");
+
+template <typename T>
+constexpr int kV = 16 / (int)sizeof(T);  // words of a piece
+template <typename T>
+constexpr int kTile = 64 * kV<T>;        // words a wave reads with one piece a lane
+template <typename T>
+constexpr int kGroup = kPieces * kTile<T>;
+
+// What the backward needs of a row: 16 bytes.  label -1: not counted, or no logit
+// above -inf; its gradient is 0.
+struct Saved {
+  float top, log_sum, entropy;
+  int label;
+};
+
+struct Params {
+  const void* logits;    // rows of `stride` elements
+  int64_t stride;
+  const int64_t* tokens;
+  int64_t rows, vocab, ignore;
+  float inv_t, scale;    // 1 / t, log2(e) / t
+  int top;
+  int parts;             // of a row
+  int64_t per_part;      // words, whole tiles
+  Saved* saved;
+  float* logprob;
+  float* entropy;
+  float* top_logprobs;   // [rows, top]
+  int64_t* top_tokens;
+  unsigned long long* part;  // [rows][parts][2 + top]: a part's sums, and its best keys in order
+  int* tickets;          // [rows], zero, left zero
+  // backward
+  const float* grad_logprob;
+  const float* grad_entropy;
+  void* d_logits;        // [rows, vocab]
+  int tiles;             // groups of a row
+};
+
+// Takes NaN along.
+__device__ inline float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// Running maximum of x, sum of e = 2^((x - top) scale), sum of e (x - top) scale.
+struct Sums {
+  float top, sum, pull;
+
+  __device__ void clear() {
+    top = -FLT_MAX;  // not -inf: e of a logit of -inf is then 0
+    sum = pull = 0.f;
+  }
+  // moved to another, larger maximum
+  __device__ void raise(float to, float scale) {
+    const float d = fminf((to - top) * scale, kFar), f = exp2_of(-d);
+    pull = f * (pull - d * sum);
+    sum *= f;
+    top = to;
+  }
+  __device__ void join(Sums o, float scale) {
+    const float t = max_of(top, o.top);
+    raise(t, scale);
+    o.raise(t, scale);
+    sum += o.sum;
+    pull += o.pull;
+  }
+  __device__ void over_wave(float scale) {
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2)
+      join(Sums{__shfl_xor(top, d), __shfl_xor(sum, d), __shfl_xor(pull, d)}, scale);
+  }
+};
+
+// The lane's pieces of the group of words that begins at `first`; words from `end`
+// on are -inf.
+template <typename T>
+__device__ inline void load_group(const T* row, int64_t first, int64_t end,
+                                  T (&x)[kPieces][kV<T>]) {
+  constexpr int V = kV<T>;
+  const int lane = (int)threadIdx.x & 63;
+  if (first + kGroup<T> <= end) {
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u)
+      __builtin_memcpy(x[u], row + first + u * kTile<T> + lane * V, 16);
+    return;
+  }
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) {
+    const int64_t at = first + u * kTile<T> + lane * V;
+#pragma unroll
+    for (int e = 0; e < V; ++e) x[u][e] = (T)-INFINITY;
+    if (at + V <= end) {
+      __builtin_memcpy(x[u], row + at, 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (at + e < end) x[u][e] = row[at + e];
+    }
+  }
+}
+
+// Order among all of a row's words: the larger logit, then the lower number; NaN
+// above all.  0 is no word's.
+__device__ inline uint32_t order_of(float x) { return x != x ? 0xffffffffu : key_of(x); }
+__device__ inline float logit_of(uint32_t order) {
+  const uint32_t b = order & 0x80000000u ? order ^ 0x80000000u : ~order;
+  return order == 0xffffffffu ? NAN : __uint_as_float(b);
+}
+__device__ inline uint64_t word_key(uint32_t order, uint32_t word) {
+  return (uint64_t)order << 32 | (0xffffffffu - word);
+}
+
+// A wave's candidates, in its part of LDS.
+struct Candidates {
+  uint64_t* keys;   // [kRoom]
+  int count;        // uniform
+  uint64_t least;   // what a key has to reach; uniform
+
+  // How many of n keys at `at` are above `key`; all lanes read the same ones.
+  __device__ static int above(const uint64_t* at, int n, uint64_t key) {
+    int r = 0;
+    for (int i = 0; i < n; ++i) r += at[i] > key;
+    return r;
+  }
+  // Keeps the `top` best, in order.
+  __device__ void shrink(int top) {
+    const int lane = (int)threadIdx.x & 63;
+    uint64_t mine[kRoom / 64];
+    int rank[kRoom / 64];
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < kRoom / 64; ++i) {
+      const bool in = i * 64 + lane < count;
+      mine[i] = in ? keys[i * 64 + lane] : 0;
+      rank[i] = in ? above(keys, count, mine[i]) : kRoom;
+    }
+    wave_sync();
+#pragma unroll
+    for (int i = 0; i < kRoom / 64; ++i)
+      if (rank[i] < top) keys[rank[i]] = mine[i];
+    wave_sync();
+    if (count > top) count = top;
+    if (count == top) least = keys[top - 1];
+  }
+  // One key a lane, where `on`.
+  __device__ void push(uint64_t key, bool on, int top) {
+    on = on && key >= least;
+    unsigned long long m = __ballot(on);
+    if (!m) return;
+    if (count + __popcll(m) > kRoom) {
+      shrink(top);
+      on = on && key >= least;
+      m = __ballot(on);
+    }
+    const int lane = (int)threadIdx.x & 63;
+    if (on) keys[count + __popcll(m & ((1ull << lane) - 1))] = key;
+    count += __popcll(m);
+  }
+};
+
+// The k-th largest of the wave's N values a lane, from below: exact in the bits from
+// `low` on.
+template <int N>
+__device__ inline uint32_t kth_largest(const uint32_t (&x)[N], int k, int low) {
+  uint32_t found = 0;
+  for (int b = 31; b >= low; --b) {
+    const uint32_t next = found | 1u << b;
+    int reach = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) reach += __popcll(__ballot(x[i] >= next));
+    if (reach >= k) found = next;
+    if (reach == k) break;
+  }
+  return found;
+}
+
+// W waves share a row or a part of one.
+template <typename T, int W, bool TOP>
+__global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
+  constexpr int V = kV<T>, kTeams = kBlock / 64 / W;
+  __shared__ uint64_t s_keys[TOP ? kBlock / 64 * kRoom : 1];
+  __shared__ uint32_t s_max[TOP && W > 1 ? kBlock : 1];
+  __shared__ int s_count[TOP ? kBlock / 64 : 1];
+  __shared__ Sums s_sums[W > 1 ? W : 1];
+  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x / 64;
+  const int team = wave / W, mate = wave % W, thread = mate * 64 + lane;
+  const auto team_sync = [] {
+    if constexpr (W > 1)
+      __syncthreads();
+    else
+      wave_sync();
+  };
+  const int64_t row = W > 1 ? (int64_t)blockIdx.x / p.parts : (int64_t)blockIdx.x * kTeams + team;
+  const int part = W > 1 ? (int)((int64_t)blockIdx.x % p.parts) : 0;
+  if (row >= p.rows) return;  // a whole team
+  const int64_t y = p.tokens[row];
+  if (y < 0 || y >= p.vocab || y == p.ignore) {
+    if (part == 0) {
+      if (TOP && thread < p.top) {
+        p.top_logprobs[row * p.top + thread] = 0.f;
+        p.top_tokens[row * p.top + thread] = -1;
+      }
+      if (thread == 0) {
+        p.logprob[row] = p.entropy[row] = 0.f;
+        p.saved[row] = Saved{0.f, 0.f, 0.f, -1};
+      }
+    }
+    return;
+  }
+  const T* logits = static_cast<const T*>(p.logits) + row * p.stride;
+  const float x_y = (float)logits[y];
+  const int64_t v0 = part * p.per_part;
+  const int64_t v1 = v0 + p.per_part < p.vocab ? v0 + p.per_part : p.vocab;
+
+  Sums sums;
+  sums.clear();
+  Candidates best{s_keys + (TOP ? wave * kRoom : 0), 0, 0};
+  uint32_t reach = 0;  // what a group's largest order must reach to hold a candidate
+  bool first = true;
+  for (int64_t v = v0; v < v1; v += W * kGroup<T>) {
+    T x[kPieces][V];
+    const int64_t mine = v + mate * kGroup<T>;
+    load_group<T>(logits, mine, v1, x);
+    float t = -INFINITY;
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+      for (int e = 0; e < V; e += 2) t = max_of(max_of(t, (float)x[u][e]), (float)x[u][e + 1]);
+    if constexpr (TOP) {
+      const uint32_t order = order_of(t);
+      if (first) {
+        constexpr int low = sizeof(T) == 2 ? 16 : 0;
+        if constexpr (W > 1) {
+          s_max[threadIdx.x] = order;
+          __syncthreads();
+          uint32_t all[W];
+#pragma unroll
+          for (int i = 0; i < W; ++i) all[i] = s_max[i * 64 + lane];
+          reach = kth_largest<W>(all, p.top, low);
+        } else {
+          const uint32_t all[1] = {order};
+          reach = kth_largest<1>(all, p.top, low);
+        }
+        best.least = (uint64_t)reach << 32;
+      }
+      if (__ballot(order >= reach)) {
+#pragma unroll
+        for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+          for (int e = 0; e < V; ++e) {
+            const int64_t word = mine + u * kTile<T> + lane * V + e;
+            const uint32_t o = order_of((float)x[u][e]);
+            best.push(word_key(o, (uint32_t)word), word < v1, p.top);
+          }
+        // words that follow have higher numbers: an equal logit is no candidate
+        reach = (uint32_t)(best.least >> 32);
+        if ((uint32_t)best.least && reach != 0xffffffffu) ++reach;
+      }
+    }
+    sums.raise(max_of(sums.top, t), p.scale);
+    float sum = 0.f, pull = 0.f;
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float z = fmaxf(((float)x[u][e] - sums.top) * p.scale, -kFar);
+        const float ex = exp2_of(z);
+        sum += ex;
+        pull = fmaf(ex, z, pull);
+      }
+    sums.sum += sum;
+    sums.pull += pull;
+    first = false;
+  }
+  sums.over_wave(p.scale);
+  if constexpr (W > 1) {
+    if (lane == 0) s_sums[mate] = sums;
+  }
+  if constexpr (TOP) {
+    if (lane == 0) s_count[wave] = best.count;
+  }
+  team_sync();
+  if constexpr (W > 1) {
+    sums = s_sums[0];
+#pragma unroll
+    for (int i = 1; i < W; ++i) sums.join(s_sums[i], p.scale);
+  }
+
+  // Every candidate's place among the team's: `put(place, key)` for the first `top`.
+  const auto rank = [&](auto put) {
+    const uint64_t* keys = s_keys + team * W * kRoom;
+    const int* count = s_count + team * W;
+    for (int w = 0; w < W; ++w)
+      for (int i = thread; i < count[w]; i += W * 64) {
+        const uint64_t key = keys[w * kRoom + i];
+        int place = 0;
+        for (int o = 0; o < W; ++o) place += Candidates::above(keys + o * kRoom, count[o], key);
+        if (place < p.top) put(place, key);
+      }
+  };
+
+  if constexpr (W > 1) {
+    if (p.parts > 1) {
+      unsigned long long* all = p.part + row * p.parts * (2 + p.top);
+      unsigned long long* own = all + part * (2 + p.top);
+      if (thread == 0) {
+        ace::store_dev(own, (unsigned long long)__float_as_uint(sums.top) << 32 |
+                                __float_as_uint(sums.sum));
+        ace::store_dev(own + 1, (unsigned long long)__float_as_uint(sums.pull));
+      }
+      if constexpr (TOP) {
+        int held = 0;
+        for (int w = 0; w < W; ++w) held += s_count[w];
+        rank([&](int place, uint64_t key) { ace::store_dev(own + 2 + place, (unsigned long long)key); });
+        if (thread >= held && thread < p.top) ace::store_dev(own + 2 + thread, 0ull);
+      }
+      if (!ace::last_of(p.tickets + row * kTicketStride, p.parts)) return;
+      sums.clear();
+      if (lane < p.parts) {
+        const unsigned long long* at = all + lane * (2 + p.top);
+        const unsigned long long a = ace::load_dev(at), b = ace::load_dev(at + 1);
+        sums = Sums{__uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)a),
+                    __uint_as_float((uint32_t)b)};
+      }
+      sums.over_wave(p.scale);
+      if constexpr (TOP) {
+        // each part's d-th best, of which the m-th largest has at least d m >= top
+        // words that reach it
+        const int d = (p.top + p.parts - 1) / p.parts, m = (p.top + d - 1) / d;
+        const uint64_t key =
+            lane < p.parts ? ace::load_dev(all + lane * (2 + p.top) + 1 + d) : 0ull;
+        const uint32_t orders[1] = {(uint32_t)(key >> 32)};
+        best.count = 0;
+        best.least = (uint64_t)kth_largest<1>(orders, m, 0) << 32;
+        const int n = p.parts * p.top;
+        for (int i = 0; i < n; i += kBlock) {
+          const int at = i + thread;
+          const uint64_t k =
+              at < n ? ace::load_dev(all + at / p.top * (2 + p.top) + 2 + at % p.top) : 0ull;
+          best.push(k, k != 0, p.top);
+        }
+        __syncthreads();
+        if (lane == 0) s_count[wave] = best.count;
+        __syncthreads();
+      }
+    }
+  }
+
+  const bool defined = sums.top < INFINITY;  // not NaN, not +inf
+  const bool dead = sums.sum == 0.f;         // every logit is -inf
+  const float log_sum = logf(sums.sum);
+  const auto logprob_of = [&](float x) {
+    return !defined ? NAN : dead ? -INFINITY : (x - sums.top) * p.inv_t - log_sum;
+  };
+  if (thread == 0) {
+    const float entropy = !defined ? NAN : dead ? 0.f : log_sum - kLn2 * (sums.pull / sums.sum);
+    p.logprob[row] = logprob_of(x_y);
+    p.entropy[row] = entropy;
+    p.saved[row] = Saved{defined ? sums.top : NAN, log_sum, entropy, dead && defined ? -1 : (int)y};
+  }
+  if constexpr (TOP)
+    rank([&](int place, uint64_t key) {
+      p.top_logprobs[row * p.top + place] = logprob_of(logit_of((uint32_t)(key >> 32)));
+      p.top_tokens[row * p.top + place] = (int64_t)(0xffffffffu - (uint32_t)key);
+    });
+}
+
+// A wave does one group of a row.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void backward_kernel(Params p) {
+  constexpr int V = kV<T>;
+  const int lane = (int)threadIdx.x & 63;
+  // fewer than 2^28 of them, and one for the wave: a 32-bit scalar division
+  const uint32_t task = (uint32_t)__builtin_amdgcn_readfirstlane(
+      (int)(blockIdx.x * (kBlock / 64) + threadIdx.x / 64));
+  const int64_t row = task / (uint32_t)p.tiles;
+  const int64_t first = (int64_t)(task % (uint32_t)p.tiles) * kGroup<T>;
+  if (row >= p.rows) return;
+  const Saved s = p.saved[row];
+  T* out = static_cast<T*>(p.d_logits) + row * p.vocab;
+  T x[kPieces][V];
+  if (s.label >= 0) {
+    load_group<T>(static_cast<const T*>(p.logits) + row * p.stride, first, p.vocab, x);
+    float g = (p.grad_logprob ? p.grad_logprob[row] : 0.f) * p.inv_t;
+    const float h = (p.grad_entropy ? p.grad_entropy[row] : 0.f) * p.inv_t;
+    const float whole = s.top == s.top ? g : NAN;  // NaN anywhere in the row: everywhere
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        // at most kFar below: p is 0 there, and lp times it too
+        const float lp = fmaxf(((float)x[u][e] - s.top) * p.inv_t - s.log_sum, -kFar);
+        const float pr = exp2_of(lp * kLog2e);
+        float d = -pr * fmaf(h, lp + s.entropy, whole);
+        if (first + u * kTile<T> + lane * V + e == s.label) d += g;
+        x[u][e] = (T)d;
+      }
+  } else {
+#pragma unroll
+    for (int u = 0; u < kPieces; ++u)
+#pragma unroll
+      for (int e = 0; e < V; ++e) x[u][e] = (T)0.f;
+  }
+#pragma unroll
+  for (int u = 0; u < kPieces; ++u) {
+    const int64_t at = first + u * kTile<T> + lane * V;
+    if (at + V <= p.vocab) {
+      __builtin_memcpy(out + at, x[u], 16);
+    } else {
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (at + e < p.vocab) out[at + e] = x[u][e];
+    }
+  }
+}
+
+}  // namespace logprob
+}  // namespace ace

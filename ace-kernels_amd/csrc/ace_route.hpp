@@ -1,0 +1,180 @@
+// A router's choice of experts with their weights, and the gradient
+// (ace_route_forward / ace_route_backward, declared in include/ace_hip.h).  For a
+// token with scores x [experts], of which it takes the k largest, c_1 .. c_k in order:
+//
+//   p = softmax(x),   w_r = p_c_r              or, normalised, p_c_r / sum_s p_c_s
+//   dx_e = [e = c_r] w_r g_r - p_e sum_s w_s g_s              (normalised: p is w)
+//
+// As in the balance loss (ace_balance.hpp), whose choice this is: L lanes share a
+// token, each holds C of its scores in registers, and the k largest are a sorted
+// list that lanes merge by exchanges.  A 16-bit score's key holds its expert, so the
+// list is the answer; in float32 each entry's expert is looked up among the scores.
+// Normalised weights need the chosen scores only, and their gradient no score at all.
+#pragma once
+
+#include "ace_balance.hpp"
+
+namespace ace {
+namespace route {
+
+using balance::across;
+using balance::kAdd;
+using balance::kMin;
+using balance::over_lanes;
+using balance::Row;
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct Params {
+  const void* logits;   // [tokens, experts]
+  const uint8_t* mask;  // [tokens] or null
+  int64_t tokens;
+  int experts, top_k;
+  int lanes_log2;       // L
+  int64_t per_block;    // tokens of a block
+  int normalize;
+  int64_t* chosen;      // [tokens, top_k]
+  float* weights;       // [tokens, top_k]
+  // backward
+  const float* grad;    // [tokens, top_k]
+  void* d_logits;
+};
+
+// The score of a key.
+__device__ inline float score_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+}
+template <typename T>
+__device__ inline float key_score(uint32_t key) {
+  if constexpr (sizeof(T) == 4) return key == 0xffffffffu ? NAN : score_of(key);
+  if (key >= 0xffff0000u) return NAN;
+  // a 16-bit score is the upper half (of a negative key the lower half's complement is 0)
+  const uint32_t b = key & 0x80000000u ? (key & 0xffff0000u) ^ 0x80000000u : ~(key | 0xffffu);
+  if constexpr (std::is_same_v<T, __bf16>)
+    return __uint_as_float(b);
+  else
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(b >> 16));
+}
+
+template <typename T, int C, int K>
+__global__ __launch_bounds__(kThreads, 4) void forward_kernel(Params p) {
+  constexpr bool numbered = sizeof(T) == 2;
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lanes = 1 << p.lanes_log2, j = lane & (lanes - 1);
+  const int E = p.experts;
+  const int64_t t0 = blockIdx.x * p.per_block;
+  const int64_t t1 = t0 + p.per_block < p.tokens ? t0 + p.per_block : p.tokens;
+  const int per_wave = 64 >> p.lanes_log2;
+  Row<T, C> row;
+  row.init(E, j, lanes);
+  const T* logits = static_cast<const T*>(p.logits);
+  for (int64_t t = t0 + wave * per_wave; t < t1; t += kThreads / 64 * per_wave) {
+    const int64_t mine = t + (lane >> p.lanes_log2);
+    const bool in = mine < t1, counted = in && (!p.mask || p.mask[mine]);
+    T x[C];
+#pragma unroll
+    for (int i = 0; i < C; ++i) x[i] = (T)0.f;
+    if (counted) row.load(logits + mine * E, E, x);
+    bool nan = false;
+#pragma unroll
+    for (int i = 0; i < C; ++i) nan |= x[i] != x[i];
+    uint32_t key[C], list[K];
+    balance::largest<T, C, K>(row, x, lanes, __ballot(nan) != 0, key, list);
+    int expert[K];
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+      expert[r] = (int)(0xffffu ^ (list[r] & 0xffffu));
+      if (!numbered && r < p.top_k) {
+        int found = balance::kMaxExperts;
+#pragma unroll
+        for (int i = C - 1; i >= 0; --i) found = key[i] == list[r] ? row.expert(i) : found;
+        const bool again = r > 0 && list[r] == list[r > 0 ? r - 1 : 0];
+        if (__ballot(again && counted)) {  // equal scores: the lowest number above the last
+          const int last = again ? expert[r > 0 ? r - 1 : 0] : -1;
+          found = balance::kMaxExperts;
+#pragma unroll
+          for (int i = C - 1; i >= 0; --i)
+            if (key[i] == list[r] && row.expert(i) > last) found = row.expert(i);
+        }
+        expert[r] = over_lanes(found, lanes, kMin);
+      }
+    }
+    const float top = key_score<T>(list[0]);
+    const bool dead = top == -INFINITY;  // every expert is closed
+    float weight[K], total = 0.f;
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+      weight[r] = r >= p.top_k || dead
+                      ? 0.f
+                      : __builtin_amdgcn_exp2f((key_score<T>(list[r]) - top) * kLog2e);
+      total += weight[r];
+    }
+    float by = 1.f / total;
+    if (!p.normalize) {
+      float e[C];
+      by = balance::exponentials<T, C>(row, x, lanes, e);
+    }
+    if (dead) by = 0.f;
+    if (in) {
+#pragma unroll
+      for (int r = 0; r < K; ++r)
+        if (r < p.top_k && (r & (lanes - 1)) == j) {
+          p.chosen[mine * p.top_k + r] = counted ? expert[r] : -1;
+          p.weights[mine * p.top_k + r] = counted ? weight[r] * by : 0.f;
+        }
+    }
+  }
+}
+
+template <typename T, int C>
+__global__ __launch_bounds__(kThreads, 4) void backward_kernel(Params p) {
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int lanes = 1 << p.lanes_log2, j = lane & (lanes - 1);
+  const int E = p.experts;
+  const int64_t t0 = blockIdx.x * p.per_block;
+  const int64_t t1 = t0 + p.per_block < p.tokens ? t0 + p.per_block : p.tokens;
+  const int per_wave = 64 >> p.lanes_log2;
+  Row<T, C> row;
+  row.init(E, j, lanes);
+  const T* logits = static_cast<const T*>(p.logits);
+  T* out = static_cast<T*>(p.d_logits);
+  for (int64_t t = t0 + wave * per_wave; t < t1; t += kThreads / 64 * per_wave) {
+    const int64_t mine = t + (lane >> p.lanes_log2);
+    const bool in = mine < t1;
+    const int64_t at = in ? mine * p.top_k : 0;
+    float pull = 0.f, total = 0.f;
+    for (int r = 0; r < p.top_k; ++r) {
+      const float w = p.weights[at + r];
+      pull = fmaf(w, p.grad[at + r], pull);
+      total += w;
+    }
+    // a token that is masked, or whose experts are all closed, has weights of 0
+    const bool on = in && p.chosen[at] >= 0 && total != 0.f;
+    T x[C];
+    float d[C];
+    if (!p.normalize) {
+#pragma unroll
+      for (int i = 0; i < C; ++i) x[i] = (T)0.f;
+      if (on) row.load(logits + mine * E, E, x);
+      const float inv = balance::exponentials<T, C>(row, x, lanes, d);
+#pragma unroll
+      for (int i = 0; i < C; ++i) d[i] *= -inv * pull;
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) d[i] = 0.f;
+    }
+    for (int r = 0; r < p.top_k; ++r) {
+      const int expert = (int)p.chosen[at + r];
+      const float w = p.weights[at + r], g = p.grad[at + r];
+      const float more = w * (p.normalize ? g - pull : g);
+#pragma unroll
+      for (int i = 0; i < C; ++i) d[i] += row.expert(i) == expert ? more : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < C; ++i) x[i] = on ? (T)d[i] : (T)0.f;
+    if (in) row.store(out + mine * E, E, x);
+  }
+}
+
+}  // namespace route
+}  // namespace ace

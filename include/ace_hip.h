@@ -342,6 +342,127 @@ int ace_balance_backward(const void* logits, int dtype, const uint8_t* mask,
                          const float* grad_loss, void* d_logits, void* stream);
 
 /*
+ * Log probabilities of given tokens from logits, with the entropy and the largest
+ * alternatives.  No counterpart in the reference.  logits: `rows` rows of `vocab`
+ * neighbouring elements (ACE_F32, ACE_BF16 or ACE_F16), one every `stride` elements.
+ * With s = logits / temperature:
+ *
+ *   logprob_r = s_r,token - log(sum_v exp s_rv)
+ *   entropy_r = -sum_v p_rv log p_rv,   p = softmax(s)
+ *   top_tokens [rows, top]: the words of the `top` largest logits in order, the
+ *   lowest first where they are equal (NaN is above all, -0 equals 0), and their log
+ *   probabilities in top_logprobs (both may be NULL with top 0)
+ *
+ * A row whose token is `ignore_index` or outside [0, vocab) is not counted: its
+ * results and its gradient are 0, its top_tokens -1, its logits are not read.
+ * Logits of -inf have probability 0 and add nothing to the entropy.  A row of nothing
+ * else has log probabilities of -inf, entropy 0 and gradient 0; one with NaN or +inf
+ * has NaN throughout.
+ * ace_logprob_forward: `saved` (ace_logprob_saved_bytes, 16-byte aligned) goes to the
+ * backward.  Where the tickets' size (ace_logprob_ticket_bytes) is not 0, `tickets` is
+ * zero when a call starts and left zero, and calls that overlap need one each and a
+ * workspace (ace_logprob_workspace_bytes, 8-byte aligned) each.
+ * ace_logprob_backward: d_logits [rows, vocab], contiguous, in the logits' type, for
+ * upstream gradients of logprob and entropy (either may be NULL, for 0); the top
+ * alternatives are constants.  d_logits may not overlap logits.
+ * Both calls are one launch on `stream`, allocate nothing and can be captured; results
+ * do not vary from run to run.  Returns ACE_EINVAL (temperature outside [1e-3, 1e3]
+ * among others), ACE_EUNSUPPORTED (top above 32, vocab above 2^30, 2^24 rows or more,
+ * 2^26 pieces of 4096 bytes of rows or more), ACE_EWORKSPACE or a HIP error.
+ */
+size_t ace_logprob_saved_bytes(int64_t rows);
+size_t ace_logprob_workspace_bytes(int dtype, int64_t rows, int64_t vocab,
+                                   int top);
+size_t ace_logprob_ticket_bytes(int dtype, int64_t rows, int64_t vocab);
+int ace_logprob_forward(const void* logits, int dtype, int64_t stride,
+                        const int64_t* tokens, int64_t rows, int64_t vocab,
+                        int64_t ignore_index, float temperature, int top,
+                        void* saved, float* logprob, float* entropy,
+                        float* top_logprobs, int64_t* top_tokens, void* tickets,
+                        size_t ticket_bytes, void* workspace,
+                        size_t workspace_bytes, void* stream);
+int ace_logprob_backward(const void* logits, int dtype, int64_t stride,
+                         int64_t rows, int64_t vocab, float temperature,
+                         const void* saved, const float* grad_logprob,
+                         const float* grad_entropy, void* d_logits,
+                         void* stream);
+
+/*
+ * A router's choice of experts with their weights.  No counterpart in the reference.
+ * logits [tokens, experts] (ACE_F32, ACE_BF16 or ACE_F16, contiguous): a token whose
+ * byte of `mask` ([tokens], NULL: all) is not 0 takes its top_k largest logits, as
+ * ace_balance_forward counts them: the lowest expert first where they are equal, NaN
+ * above all.  chosen [tokens, top_k] in that order; weights [tokens, top_k]: the
+ * softmax over all experts, or with `normalize` over the chosen ones.  A masked
+ * token has -1 and 0, and its logits are not read.  An expert at -inf has weight 0,
+ * also where all of a token's are.
+ * ace_route_backward: the gradient of logits for an upstream gradient of weights, from
+ * the forward's chosen and weights; the choice is a constant.
+ * Both calls are one launch on `stream`, allocate nothing and can be captured.
+ * Returns ACE_EINVAL, ACE_EUNSUPPORTED (experts above 512, top_k above 16, tokens above
+ * 2^30) or a HIP error.
+ */
+int ace_route_forward(const void* logits, int dtype, const uint8_t* mask,
+                      int64_t tokens, int64_t experts, int top_k,
+                      int normalize, int64_t* chosen, float* weights,
+                      void* stream);
+int ace_route_backward(const void* logits, int dtype, int64_t tokens,
+                       int64_t experts, int top_k, int normalize,
+                       const int64_t* chosen, const float* weights,
+                       const float* grad_weights, void* d_logits,
+                       void* stream);
+
+/*
+ * Tokens sorted by expert.  No counterpart in the reference.  chosen [slots]: the
+ * expert of each choice; a number outside [0, experts) is none.
+ *
+ *   offsets [experts + 1]  expert e has the places offsets[e] .. offsets[e + 1] - 1
+ *   source [slots]         the slot at each place, slots of one expert in ascending
+ *                          order; -1 from offsets[experts] on
+ *   place [slots]          the place of each slot; -1: none
+ *
+ * The workspace (ace_expert_order_workspace_bytes, 4-byte aligned, may be 0 bytes)
+ * needs no clearing; calls that overlap need one each.  One or two launches on
+ * `stream`, no allocation, can be captured.  Returns ACE_EINVAL, ACE_EUNSUPPORTED
+ * (experts above 512, slots above 2^30), ACE_EWORKSPACE or a HIP error.
+ */
+size_t ace_expert_order_workspace_bytes(int64_t slots, int64_t experts);
+int ace_expert_order(const int64_t* chosen, int64_t slots, int64_t experts,
+                     int64_t* offsets, int64_t* source, int64_t* place,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Rows of tokens in expert order, and back.  No counterpart in the reference.  Tokens
+ * have `width` elements (ACE_F32, ACE_BF16 or ACE_F16) and top_k slots each; place
+ * [tokens, top_k] is ace_expert_order's, `routed` its last offset (device memory).  A
+ * place outside [0, tokens top_k) is none.  All tensors are contiguous; outputs may not
+ * overlap inputs.
+ *
+ * ace_to_experts: rows [tokens top_k, width], rows[place[t, j]] = x[t]; rows from
+ * `routed` on are 0.
+ * ace_from_experts: out[t] = sum_j weights[t, j] rows[place[t, j]] over its placed
+ * slots, summed in float32 and rounded once; weights [tokens, top_k] float32 or NULL,
+ * for 1 (the gradient of ace_to_experts).  Rows that nothing is placed at are not read.
+ * ace_from_experts_backward: from the gradient of out, d_rows (0 from `routed` on) and
+ * d_weights (0 without a place), either skipped if NULL; `rows` may be NULL without
+ * d_weights.
+ * One launch each on `stream`, no allocation, can be captured; results do not vary
+ * from run to run.  Returns ACE_EINVAL, ACE_EUNSUPPORTED (width above 2^20, 2^26 slots or
+ * pieces of 4096 bytes of tokens or more) or a HIP error.
+ */
+int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width,
+                   int64_t top_k, const int64_t* place, const int64_t* routed,
+                   void* rows, void* stream);
+int ace_from_experts(const void* rows, int dtype, int64_t tokens,
+                     int64_t width, int64_t top_k, const int64_t* place,
+                     const float* weights, void* out, void* stream);
+int ace_from_experts_backward(const void* rows, const void* grad, int dtype,
+                              int64_t tokens, int64_t width, int64_t top_k,
+                              const int64_t* place, const int64_t* routed,
+                              const float* weights, void* d_rows,
+                              float* d_weights, void* stream);
+
+/*
  * Kernel timing.  This has no counterpart in the reference, whose benchmark
  * brackets each call with events recorded on the stream
  * (src/ace_bench/timing.py:48-77); on HIP such events also time the dispatch
