@@ -18,15 +18,18 @@ int launched() {
 }
 
 int64_t order_blocks(int64_t slots, int64_t* per_block) {
-  // 4096 slots a block: 16 rounds of a wave; at most kMaxBlocks
-  int64_t each = 4096;
+  // 1024 slots a block: four rounds of a wave; at most kMaxBlocks
+  int64_t each = 1024;
   if (slots > each * kMaxBlocks) each = (slots + kMaxBlocks - 1) / kMaxBlocks;
   *per_block = (each + kBlock - 1) / kBlock * kBlock;
   const int64_t blocks = (slots + *per_block - 1) / *per_block;
   return blocks < 1 ? 1 : blocks;
 }
 
-int span_of(int dtype) { return dtype == ACE_F32 ? kSpan<float> : kSpan<__bf16>; }
+int64_t pieces_of(int64_t width, int dtype, int deep) {
+  const int64_t span = 64 * deep * (dtype == ACE_F32 ? kV<float> : kV<__bf16>);
+  return (width + span - 1) / span;
+}
 
 int check(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_k,
           const int64_t* place) {
@@ -35,13 +38,13 @@ int check(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_
   if (tokens > 0 && (!in || !place)) return ACE_EINVAL;
   if (width > kMaxWidth || top_k > kMaxSlots || tokens > kMaxSlots || tokens * top_k > kMaxSlots)
     return ACE_EUNSUPPORTED;
-  const int64_t span = span_of(dtype), pieces = (width + span - 1) / span;
-  if (tokens * pieces >= kMaxWaves || tokens * top_k >= kMaxWaves) return ACE_EUNSUPPORTED;
+  if (tokens * pieces_of(width, dtype, kDeepFrom) >= kMaxWaves || tokens * top_k >= kMaxWaves)
+    return ACE_EUNSUPPORTED;
   return ACE_OK;
 }
 
-RowsParams params(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_k,
-                  const int64_t* place, const float* weights) {
+RowsParams params(const void* in, int64_t tokens, int64_t width, int64_t top_k, const int64_t* place,
+                  const float* weights) {
   RowsParams p{};
   p.in = in;
   p.tokens = tokens;
@@ -50,7 +53,6 @@ RowsParams params(const void* in, int dtype, int64_t tokens, int64_t width, int6
   p.top_k = (int)top_k;
   p.place = place;
   p.weights = weights;
-  p.pieces = (int)((width + span_of(dtype) - 1) / span_of(dtype));
   return p;
 }
 
@@ -118,9 +120,10 @@ int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width, int6
   if (bad) return bad;
   if (tokens == 0) return ACE_OK;
   if (!routed || !rows) return ACE_EINVAL;
-  RowsParams p = params(x, dtype, tokens, width, top_k, place, nullptr);
+  RowsParams p = params(x, tokens, width, top_k, place, nullptr);
   p.offsets = routed;
   p.out = rows;
+  p.pieces = (int)pieces_of(width, dtype, kDeepTo);
   const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
@@ -137,8 +140,9 @@ int ace_from_experts(const void* rows, int dtype, int64_t tokens, int64_t width,
   if (bad) return bad;
   if (tokens == 0) return ACE_OK;
   if (!out) return ACE_EINVAL;
-  RowsParams p = params(rows, dtype, tokens, width, top_k, place, weights);
+  RowsParams p = params(rows, tokens, width, top_k, place, weights);
   p.out = out;
+  p.pieces = (int)pieces_of(width, dtype, kDeepFrom);
   const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
@@ -158,7 +162,7 @@ int ace_from_experts_backward(const void* rows, const void* grad, int dtype, int
   if (bad) return bad;
   if (tokens == 0 || (!d_rows && !d_weights)) return ACE_OK;
   if (!grad || !routed) return ACE_EINVAL;
-  RowsParams p = params(rows, dtype, tokens, width, top_k, place, weights);
+  RowsParams p = params(rows, tokens, width, top_k, place, weights);
   p.grad = grad;
   p.offsets = routed;
   p.out = d_rows;

@@ -23,6 +23,7 @@
 #include <stdint.h>
 
 #include "ace_core.hpp"  // wave_sync
+#include "ace_piece.hpp"
 
 namespace ace {
 namespace experts {
@@ -74,34 +75,50 @@ __global__ __launch_bounds__(kBlock) void count_kernel(OrderParams p) {
 // ballots over the bits of its number.
 __global__ __launch_bounds__(kBlock) void place_kernel(OrderParams p) {
   __shared__ int s_next[kWaves][kMaxExperts];
+  __shared__ int s_all[kMaxExperts], s_before[kMaxExperts];
   __shared__ int s_sum[kWaves];
   __shared__ int64_t s_total;
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int64_t per_wave = p.per_block / kWaves;
   const int64_t s0 = blockIdx.x * p.per_block + wave * per_wave;
   const int64_t s1 = s0 + per_wave < p.slots ? s0 + per_wave : p.slots;
-  for (int i = tid; i < kWaves * kMaxExperts; i += kBlock) (&s_next[0][0])[i] = 0;
+  for (int i = tid; i < kMaxExperts; i += kBlock) {
+    s_all[i] = s_before[i] = 0;
+#pragma unroll
+    for (int w = 0; w < kWaves; ++w) s_next[w][i] = 0;
+  }
   __syncthreads();
   for (int64_t s = s0 + lane; s < s1; s += 64) {
     const int e = choice(p, s, s1);
     if (e >= 0) atomicAdd(&s_next[wave][e], 1);
   }
   __syncthreads();
+  if (p.blocks > 1) {  // the blocks' counts, added up over all and over those before
+    uint32_t e = (uint32_t)tid % (uint32_t)p.experts, b = (uint32_t)tid / (uint32_t)p.experts;
+    const uint32_t step_e = kBlock % (uint32_t)p.experts, step_b = kBlock / (uint32_t)p.experts;
+    const int n = p.blocks * p.experts;
+    for (int i = tid; i < n; i += kBlock) {
+      const int c = p.counts[i];
+      atomicAdd(&s_all[e], c);
+      if (b < blockIdx.x) atomicAdd(&s_before[e], c);
+      e += step_e;
+      b += step_b;
+      if (e >= (uint32_t)p.experts) {
+        e -= (uint32_t)p.experts;
+        ++b;
+      }
+    }
+    __syncthreads();
+  }
   // thread t has experts 2 t and 2 t + 1
   static_assert(2 * kBlock == kMaxExperts, "all experts have a thread");
   int before[2], all[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int e = 2 * tid + i;
-    before[i] = all[i] = 0;
-    if (e >= p.experts) continue;
-    if (p.blocks > 1) {
-      for (int b = 0; b < p.blocks; ++b) {
-        const int n = p.counts[(int64_t)b * p.experts + e];
-        all[i] += n;
-        if (b < (int)blockIdx.x) before[i] += n;
-      }
-    } else {
+    before[i] = s_before[e];
+    all[i] = s_all[e];
+    if (p.blocks == 1) {
 #pragma unroll
       for (int w = 0; w < kWaves; ++w) all[i] += s_next[w][e];
     }
@@ -179,145 +196,171 @@ struct RowsParams {
 
 template <typename T>
 constexpr int kV = 16 / (int)sizeof(T);
-constexpr int kDeep = 4;  // pieces of 16 bytes a lane holds
-template <typename T>
-constexpr int kSpan = 64 * kDeep * kV<T>;  // elements of a row that a wave takes at once
+// Pieces of 16 bytes that a lane holds of a row: a wave takes spans of 64 of them.
+constexpr int kDeepTo = 4, kDeepFrom = 2, kDeepBack = 4;
+constexpr int kAtOnce = 4;  // rows that a wave has on the way
 
-// A wave's span of a row from element `first` on; what is behind the row's end
-// reads as 0 and is not written.
-template <typename T>
-__device__ inline void load_span(const T* row, int first, int width, T (&x)[kDeep][kV<T>]) {
-  constexpr int V = kV<T>;
-  const int lane = (int)threadIdx.x & 63;
+template <typename T, int D>
+struct Span {
+  static constexpr int V = kV<T>, kWidth = 64 * D * V;
+  Piece<T> x[D];
+
+  __device__ void clear() {
 #pragma unroll
-  for (int u = 0; u < kDeep; ++u) {
-    const int at = first + (u * 64 + lane) * V;
-    if (at + V <= width) {
-      __builtin_memcpy(x[u], row + at, 16);
-    } else {
+    for (int u = 0; u < D; ++u) x[u].fill((T)0.f);
+  }
+  // From element `first` of a row; what is behind the row's end reads as 0 and is
+  // not written.
+  __device__ void load(const T* row, int first, int width) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[u][e] = at + e < width ? row[at + e] : (T)0.f;
+    for (int u = 0; u < D; ++u) {
+      const int at = first + (u * 64 + ((int)threadIdx.x & 63)) * V;
+      if (at + V <= width)
+        x[u].load(row + at);
+      else
+        x[u].load_some(row + at, width - at, (T)0.f);
     }
   }
-}
-template <typename T>
-__device__ inline void store_span(T* row, int first, int width, const T (&x)[kDeep][kV<T>]) {
-  constexpr int V = kV<T>;
-  const int lane = (int)threadIdx.x & 63;
+  __device__ void store(T* row, int first, int width) const {
 #pragma unroll
-  for (int u = 0; u < kDeep; ++u) {
-    const int at = first + (u * 64 + lane) * V;
-    if (at + V <= width) {
-      __builtin_memcpy(row + at, x[u], 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (at + e < width) row[at + e] = x[u][e];
+    for (int u = 0; u < D; ++u) {
+      const int at = first + (u * 64 + ((int)threadIdx.x & 63)) * V;
+      if (at + V <= width)
+        x[u].store(row + at);
+      else
+        x[u].store_some(row + at, width - at);
     }
   }
-}
+};
 
 // The same for the whole wave, in a scalar register.
 __device__ inline int wave_number() {
   return __builtin_amdgcn_readfirstlane((int)(blockIdx.x * kWaves + threadIdx.x / 64));
 }
-// A slot's place, -1: none (or none that exists).
-__device__ inline int64_t place_of(const RowsParams& p, int64_t slot) {
+__device__ inline float lane_value(float x, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
+}
+// A slot's place (below 2^26), -1: none, or none that exists.
+__device__ inline int place_of(const RowsParams& p, int64_t slot) {
   const int64_t at = p.place[slot];
-  return at >= 0 && at < p.slots ? at : -1;
+  return at >= 0 && at < p.slots ? (int)at : -1;
 }
 
 // A wave copies one span of a token's row to its places.  Of the rows behind the
 // last, each belongs to the wave of the slot with its number.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void to_kernel(RowsParams p) {
-  const int task = wave_number();
+  using S = Span<T, kDeepTo>;
+  const int task = wave_number(), lane = (int)threadIdx.x & 63;
   const int64_t token = task / p.pieces;
-  const int first = task % p.pieces * kSpan<T>;
+  const int first = task % p.pieces * S::kWidth;
   if (token >= p.tokens) return;
-  T x[kDeep][kV<T>], none[kDeep][kV<T>];
-  load_span<T>(static_cast<const T*>(p.in) + token * p.width, first, p.width, x);
-#pragma unroll
-  for (int u = 0; u < kDeep; ++u)
-#pragma unroll
-    for (int e = 0; e < kV<T>; ++e) none[u][e] = (T)0.f;
+  S x, none;
+  x.load(static_cast<const T*>(p.in) + token * p.width, first, p.width);
+  none.clear();
   T* rows = static_cast<T*>(p.out);
   const int64_t routed = *p.offsets;
-  for (int j = 0; j < p.top_k; ++j) {
-    const int64_t slot = token * p.top_k + j, at = place_of(p, slot);
-    if (at >= 0) store_span<T>(rows + at * p.width, first, p.width, x);
-    if (slot >= routed) store_span<T>(rows + slot * p.width, first, p.width, none);
+  for (int j0 = 0; j0 < p.top_k; j0 += 64) {
+    const int64_t slot0 = token * p.top_k + j0;  // lane j has choice j0 + j
+    const int n = p.top_k - j0 < 64 ? p.top_k - j0 : 64;
+    const int place = lane < n ? place_of(p, slot0 + lane) : -1;
+    for (int j = 0; j < n; ++j) {
+      const int at = __builtin_amdgcn_readlane(place, j);
+      if (at >= 0) x.store(rows + (int64_t)at * p.width, first, p.width);
+      if (slot0 + j >= routed) none.store(rows + (slot0 + j) * p.width, first, p.width);
+    }
   }
 }
 
 // A wave adds up one span of a token's rows.
 template <typename T>
 __global__ __launch_bounds__(kBlock) void from_kernel(RowsParams p) {
-  const int task = wave_number();
+  using S = Span<T, kDeepFrom>;
+  const int task = wave_number(), lane = (int)threadIdx.x & 63;
   const int64_t token = task / p.pieces;
-  const int first = task % p.pieces * kSpan<T>;
+  const int first = task % p.pieces * S::kWidth;
   if (token >= p.tokens) return;
   const T* rows = static_cast<const T*>(p.in);
-  float sum[kDeep][kV<T>];
+  float sum[kDeepFrom][S::V];
 #pragma unroll
-  for (int u = 0; u < kDeep; ++u)
+  for (int u = 0; u < kDeepFrom; ++u)
 #pragma unroll
-    for (int e = 0; e < kV<T>; ++e) sum[u][e] = 0.f;
-  for (int j = 0; j < p.top_k; ++j) {
-    const int64_t slot = token * p.top_k + j, at = place_of(p, slot);
-    if (at < 0) continue;
-    const float w = p.weights ? p.weights[slot] : 1.f;
-    T x[kDeep][kV<T>];
-    load_span<T>(rows + at * p.width, first, p.width, x);
+    for (int e = 0; e < S::V; ++e) sum[u][e] = 0.f;
+  for (int j0 = 0; j0 < p.top_k; j0 += 64) {
+    const int64_t slot = token * p.top_k + j0 + lane;  // lane j has choice j0 + j
+    int place = -1;
+    float weight = 1.f;
+    if (j0 + lane < p.top_k) {
+      place = place_of(p, slot);
+      if (p.weights) weight = p.weights[slot];
+    }
+    for (unsigned long long left = __ballot(place >= 0); left;) {
+      S x[kAtOnce];
+      int from[kAtOnce], n = 0;
 #pragma unroll
-    for (int u = 0; u < kDeep; ++u)
+      for (int i = 0; i < kAtOnce; ++i) {
+        from[i] = 0;
+        if (!left) continue;
+        from[i] = __builtin_ctzll(left);
+        left &= left - 1;
+        n = i + 1;
+        x[i].load(rows + (int64_t)__builtin_amdgcn_readlane(place, from[i]) * p.width, first, p.width);
+      }
 #pragma unroll
-      for (int e = 0; e < kV<T>; ++e) sum[u][e] = fmaf(w, (float)x[u][e], sum[u][e]);
+      for (int i = 0; i < kAtOnce; ++i) {
+        if (i >= n) continue;
+        const float w = lane_value(weight, from[i]);
+#pragma unroll
+        for (int u = 0; u < kDeepFrom; ++u)
+#pragma unroll
+          for (int e = 0; e < S::V; ++e) sum[u][e] = fmaf(w, x[i].x[u][e], sum[u][e]);
+      }
+    }
   }
-  T out[kDeep][kV<T>];
+  S out;
 #pragma unroll
-  for (int u = 0; u < kDeep; ++u)
-#pragma unroll
-    for (int e = 0; e < kV<T>; ++e) out[u][e] = (T)sum[u][e];
-  store_span<T>(static_cast<T*>(p.out) + token * p.width, first, p.width, out);
+  for (int u = 0; u < kDeepFrom; ++u) out.x[u].set(sum[u]);
+  out.store(static_cast<T*>(p.out) + token * p.width, first, p.width);
 }
 
 // A wave takes a slot: its row's gradient and its weight's.
 template <typename T, bool ROWS, bool WEIGHTS>
 __global__ __launch_bounds__(kBlock) void from_backward_kernel(RowsParams p) {
+  using S = Span<T, kDeepBack>;
   const int64_t slot = wave_number();
   if (slot >= p.slots) return;
+  const T* grad = static_cast<const T*>(p.grad) + (int64_t)((int)slot / p.top_k) * p.width;
   const int64_t at = place_of(p, slot), routed = *p.offsets;
-  const T* grad = static_cast<const T*>(p.grad) + slot / p.top_k * p.width;
   const float w = p.weights ? p.weights[slot] : 1.f;
   float dot = 0.f;
-  T x[kDeep][kV<T>], y[kDeep][kV<T>];
-  for (int first = 0; first < p.width; first += kSpan<T>) {
+  for (int first = 0; first < p.width; first += S::kWidth) {
+    S x;
+    x.load(grad, first, p.width);
     if (at >= 0) {
-      load_span<T>(grad, first, p.width, x);
       if (WEIGHTS) {
-        load_span<T>(static_cast<const T*>(p.in) + at * p.width, first, p.width, y);
+        S y;
+        y.load(static_cast<const T*>(p.in) + at * p.width, first, p.width);
         float more = 0.f;
 #pragma unroll
-        for (int u = 0; u < kDeep; ++u)
+        for (int u = 0; u < kDeepBack; ++u)
 #pragma unroll
-          for (int e = 0; e < kV<T>; ++e) more = fmaf((float)x[u][e], (float)y[u][e], more);
+          for (int e = 0; e < S::V; ++e) more = fmaf(x.x[u][e], y.x[u][e], more);
         dot += more;
       }
       if (ROWS) {
 #pragma unroll
-        for (int u = 0; u < kDeep; ++u)
+        for (int u = 0; u < kDeepBack; ++u) {
+          float d[S::V];
 #pragma unroll
-          for (int e = 0; e < kV<T>; ++e) x[u][e] = (T)(w * (float)x[u][e]);
-        store_span<T>(static_cast<T*>(p.out) + at * p.width, first, p.width, x);
+          for (int e = 0; e < S::V; ++e) d[e] = w * x.x[u][e];
+          x.x[u].set(d);
+        }
+        x.store(static_cast<T*>(p.out) + at * p.width, first, p.width);
       }
     }
     if (ROWS && slot >= routed) {
-#pragma unroll
-      for (int u = 0; u < kDeep; ++u)
-#pragma unroll
-        for (int e = 0; e < kV<T>; ++e) x[u][e] = (T)0.f;
-      store_span<T>(static_cast<T*>(p.out) + slot * p.width, first, p.width, x);
+      x.clear();
+      x.store(static_cast<T*>(p.out) + slot * p.width, first, p.width);
     }
   }
   if (WEIGHTS) {

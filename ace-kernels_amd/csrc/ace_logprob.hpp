@@ -30,6 +30,7 @@
 
 #include "ace_balance.hpp"  // keys in the scores' order
 #include "ace_core.hpp"     // device-coherent accesses
+#include "ace_piece.hpp"
 
 namespace ace {
 namespace logprob {
@@ -42,6 +43,7 @@ constexpr int kPieces = 4;    // of 16 bytes that a lane reads at a time
 constexpr int kMaxTop = 32;
 constexpr int kMaxParts = 32;
 constexpr int kRoom = 256;    // candidates of a wave
+constexpr int kHeld = kRoom + kMaxTop;  // keys of its LDS
 constexpr float kFar = 200.f;  // 2^-200 is 0 in float32: exponents beyond it count as it
 static_assert(kMaxParts * kMaxTop <= kBlock / 64 * kRoom, "the last part has room for all lists");
 
@@ -101,54 +103,48 @@ struct Sums {
     sum *= f;
     top = to;
   }
-  __device__ void join(Sums o, float scale) {
-    const float t = max_of(top, o.top);
-    raise(t, scale);
-    o.raise(t, scale);
-    sum += o.sum;
-    pull += o.pull;
-  }
-  __device__ void over_wave(float scale) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2)
-      join(Sums{__shfl_xor(top, d), __shfl_xor(sum, d), __shfl_xor(pull, d)}, scale);
-  }
+  __device__ void over_wave(float scale);
 };
 
-// The lane's pieces of the group of words that begins at `first`; words from `end`
-// on are -inf.
+// x joined over the wave's lanes by `op`, in every lane.
+template <typename Op>
+__device__ inline float over_lanes(float x, Op op) {
+  x = balance::over_lanes(x, 32, op);
+  return op(x, __shfl_xor(x, 32));
+}
+__device__ inline void Sums::over_wave(float scale) {
+  raise(over_lanes(top, [](float a, float b) { return max_of(a, b); }), scale);
+  sum = over_lanes(sum, balance::kAdd);
+  pull = over_lanes(pull, balance::kAdd);
+}
+
+// The piece of words that begins at `at`; words from `end` on are -inf.
+template <typename T>
+__device__ inline void load_piece(const T* row, int64_t at, int64_t end, Piece<T>& x) {
+  if (at + kV<T> <= end)
+    x.load(row + at);
+  else
+    x.load_some(row + at, end - at, (T)-INFINITY);
+}
+// The lane's pieces of the group that begins at `first`.
 template <typename T>
 __device__ inline void load_group(const T* row, int64_t first, int64_t end,
-                                  T (&x)[kPieces][kV<T>]) {
-  constexpr int V = kV<T>;
-  const int lane = (int)threadIdx.x & 63;
+                                  Piece<T> (&x)[kPieces]) {
+  const int64_t mine = first + ((int)threadIdx.x & 63) * kV<T>;
   if (first + kGroup<T> <= end) {
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
-      __builtin_memcpy(x[u], row + first + u * kTile<T> + lane * V, 16);
-    return;
-  }
+    for (int u = 0; u < kPieces; ++u) x[u].load(row + mine + u * kTile<T>);
+  } else {
 #pragma unroll
-  for (int u = 0; u < kPieces; ++u) {
-    const int64_t at = first + u * kTile<T> + lane * V;
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[u][e] = (T)-INFINITY;
-    if (at + V <= end) {
-      __builtin_memcpy(x[u], row + at, 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (at + e < end) x[u][e] = row[at + e];
-    }
+    for (int u = 0; u < kPieces; ++u) load_piece<T>(row, mine + u * kTile<T>, end, x[u]);
   }
 }
 
 // Order among all of a row's words: the larger logit, then the lower number; NaN
 // above all.  0 is no word's.
 __device__ inline uint32_t order_of(float x) { return x != x ? 0xffffffffu : key_of(x); }
-__device__ inline float logit_of(uint32_t order) {
-  const uint32_t b = order & 0x80000000u ? order ^ 0x80000000u : ~order;
-  return order == 0xffffffffu ? NAN : __uint_as_float(b);
+__device__ inline float logit_of(uint32_t order) {  // NaN also where it is no logit's
+  return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
 __device__ inline uint64_t word_key(uint32_t order, uint32_t word) {
   return (uint64_t)order << 32 | (0xffffffffu - word);
@@ -156,34 +152,30 @@ __device__ inline uint64_t word_key(uint32_t order, uint32_t word) {
 
 // A wave's candidates, in its part of LDS.
 struct Candidates {
-  uint64_t* keys;   // [kRoom]
+  uint64_t* keys;   // [kRoom], and room for the best of them
   int count;        // uniform
   uint64_t least;   // what a key has to reach; uniform
 
   // How many of n keys at `at` are above `key`; all lanes read the same ones.
   __device__ static int above(const uint64_t* at, int n, uint64_t key) {
     int r = 0;
+#pragma unroll 4
     for (int i = 0; i < n; ++i) r += at[i] > key;
     return r;
   }
   // Keeps the `top` best, in order.
   __device__ void shrink(int top) {
     const int lane = (int)threadIdx.x & 63;
-    uint64_t mine[kRoom / 64];
-    int rank[kRoom / 64];
     wave_sync();
-#pragma unroll
-    for (int i = 0; i < kRoom / 64; ++i) {
-      const bool in = i * 64 + lane < count;
-      mine[i] = in ? keys[i * 64 + lane] : 0;
-      rank[i] = in ? above(keys, count, mine[i]) : kRoom;
+    for (int i = lane; i < count; i += 64) {
+      const uint64_t key = keys[i];
+      const int place = above(keys, count, key);
+      if (place < top) keys[kRoom + place] = key;
     }
     wave_sync();
-#pragma unroll
-    for (int i = 0; i < kRoom / 64; ++i)
-      if (rank[i] < top) keys[rank[i]] = mine[i];
-    wave_sync();
     if (count > top) count = top;
+    if (lane < count) keys[lane] = keys[kRoom + lane];
+    wave_sync();
     if (count == top) least = keys[top - 1];
   }
   // One key a lane, where `on`.
@@ -222,7 +214,7 @@ __device__ inline uint32_t kth_largest(const uint32_t (&x)[N], int k, int low) {
 template <typename T, int W, bool TOP>
 __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
   constexpr int V = kV<T>, kTeams = kBlock / 64 / W;
-  __shared__ uint64_t s_keys[TOP ? kBlock / 64 * kRoom : 1];
+  __shared__ uint64_t s_keys[TOP ? kBlock / 64 * kHeld : 1];
   __shared__ uint32_t s_max[TOP && W > 1 ? kBlock : 1];
   __shared__ int s_count[TOP ? kBlock / 64 : 1];
   __shared__ Sums s_sums[W > 1 ? W : 1];
@@ -258,48 +250,21 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
 
   Sums sums;
   sums.clear();
-  Candidates best{s_keys + (TOP ? wave * kRoom : 0), 0, 0};
-  uint32_t reach = 0;  // what a group's largest order must reach to hold a candidate
+  Candidates best{s_keys + (TOP ? wave * kHeld : 0), 0, 0};
+  float reach = 0.f;  // what a logit has to reach to be a candidate; NaN: nothing
   bool first = true;
   for (int64_t v = v0; v < v1; v += W * kGroup<T>) {
-    T x[kPieces][V];
+    Piece<T> x[kPieces];
     const int64_t mine = v + mate * kGroup<T>;
     load_group<T>(logits, mine, v1, x);
-    float t = -INFINITY;
+    float tops[kPieces], t = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
+    for (int u = 0; u < kPieces; ++u) {
+      tops[u] = max_of(x[u][0], x[u][1]);
 #pragma unroll
-      for (int e = 0; e < V; e += 2) t = max_of(max_of(t, (float)x[u][e]), (float)x[u][e + 1]);
-    if constexpr (TOP) {
-      const uint32_t order = order_of(t);
-      if (first) {
-        constexpr int low = sizeof(T) == 2 ? 16 : 0;
-        if constexpr (W > 1) {
-          s_max[threadIdx.x] = order;
-          __syncthreads();
-          uint32_t all[W];
-#pragma unroll
-          for (int i = 0; i < W; ++i) all[i] = s_max[i * 64 + lane];
-          reach = kth_largest<W>(all, p.top, low);
-        } else {
-          const uint32_t all[1] = {order};
-          reach = kth_largest<1>(all, p.top, low);
-        }
-        best.least = (uint64_t)reach << 32;
-      }
-      if (__ballot(order >= reach)) {
-#pragma unroll
-        for (int u = 0; u < kPieces; ++u)
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const int64_t word = mine + u * kTile<T> + lane * V + e;
-            const uint32_t o = order_of((float)x[u][e]);
-            best.push(word_key(o, (uint32_t)word), word < v1, p.top);
-          }
-        // words that follow have higher numbers: an equal logit is no candidate
-        reach = (uint32_t)(best.least >> 32);
-        if ((uint32_t)best.least && reach != 0xffffffffu) ++reach;
-      }
+      for (int e = 2; e < V; e += 2)
+        tops[u] = max_of(max_of(tops[u], x[u][e]), x[u][e + 1]);
+      t = max_of(t, tops[u]);
     }
     sums.raise(max_of(sums.top, t), p.scale);
     float sum = 0.f, pull = 0.f;
@@ -307,13 +272,60 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
     for (int u = 0; u < kPieces; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float z = fmaxf(((float)x[u][e] - sums.top) * p.scale, -kFar);
+        const float z = fmaxf((x[u][e] - sums.top) * p.scale, -kFar);
         const float ex = exp2_of(z);
         sum += ex;
         pull = fmaf(ex, z, pull);
       }
     sums.sum += sum;
     sums.pull += pull;
+    if constexpr (TOP) {
+      if (first) {
+        constexpr int low = sizeof(T) == 2 ? 16 : 0;
+        const uint32_t order = order_of(t);
+        uint32_t least;
+        if constexpr (W > 1) {
+          s_max[threadIdx.x] = order;
+          __syncthreads();
+          uint32_t all[W];
+#pragma unroll
+          for (int i = 0; i < W; ++i) all[i] = s_max[i * 64 + lane];
+          least = kth_largest<W>(all, p.top, low);
+        } else {
+          const uint32_t all[1] = {order};
+          least = kth_largest<1>(all, p.top, low);
+        }
+        best.least = (uint64_t)least << 32;
+        reach = logit_of(least);
+      }
+      if (__ballot(!(t < reach))) {
+        // seldom, so it reads its words again (from a cache): with all pieces still in
+        // registers half as many waves would fit
+#pragma unroll 1
+        for (int u = 0; u < kPieces; ++u) {
+          float tile = tops[0];
+#pragma unroll
+          for (int i = 1; i < kPieces; ++i) tile = u == i ? tops[i] : tile;
+          if (!__ballot(!(tile < reach))) continue;
+          Piece<T> y;
+          load_piece<T>(logits, mine + u * kTile<T> + lane * V, v1, y);
+          uint32_t mask = 0;
+#pragma unroll
+          for (int e = 0; e < V; ++e) mask |= !(y[e] < reach) ? 1u << e : 0u;
+          const int64_t word = mine + u * kTile<T> + lane * V;
+          while (__ballot(mask != 0)) {
+            const int at = __builtin_ctz(mask | 1u << V);
+            float l = y[0];
+#pragma unroll
+            for (int e = 1; e < V; ++e) l = at == e ? y[e] : l;
+            best.push(word_key(order_of(l), (uint32_t)(word + at)), mask && word + at < v1, p.top);
+            mask &= mask - 1;
+          }
+        }
+        // words that follow have higher numbers: an equal logit is no candidate
+        if ((uint32_t)best.least) reach = logit_of((uint32_t)(best.least >> 32) + 1);
+      }
+    }
     first = false;
   }
   sums.over_wave(p.scale);
@@ -325,20 +337,29 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
   }
   team_sync();
   if constexpr (W > 1) {
-    sums = s_sums[0];
+    float t = s_sums[0].top;
 #pragma unroll
-    for (int i = 1; i < W; ++i) sums.join(s_sums[i], p.scale);
+    for (int i = 1; i < W; ++i) t = max_of(t, s_sums[i].top);
+    sums.sum = sums.pull = 0.f;
+    sums.top = t;
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      Sums o = s_sums[i];
+      o.raise(t, p.scale);
+      sums.sum += o.sum;
+      sums.pull += o.pull;
+    }
   }
 
   // Every candidate's place among the team's: `put(place, key)` for the first `top`.
   const auto rank = [&](auto put) {
-    const uint64_t* keys = s_keys + team * W * kRoom;
+    const uint64_t* keys = s_keys + team * W * kHeld;
     const int* count = s_count + team * W;
     for (int w = 0; w < W; ++w)
       for (int i = thread; i < count[w]; i += W * 64) {
-        const uint64_t key = keys[w * kRoom + i];
+        const uint64_t key = keys[w * kHeld + i];
         int place = 0;
-        for (int o = 0; o < W; ++o) place += Candidates::above(keys + o * kRoom, count[o], key);
+        for (int o = 0; o < W; ++o) place += Candidates::above(keys + o * kHeld, count[o], key);
         if (place < p.top) put(place, key);
       }
   };
@@ -359,34 +380,37 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
         if (thread >= held && thread < p.top) ace::store_dev(own + 2 + thread, 0ull);
       }
       if (!ace::last_of(p.tickets + row * kTicketStride, p.parts)) return;
+      // each part's d-th best, of which the m-th largest has at least d m >= top words
+      // that reach it
+      const int d = TOP ? (p.top + p.parts - 1) / p.parts : 0;
+      const unsigned long long* at = all + (lane < p.parts ? lane : 0) * (2 + p.top);
+      const unsigned long long a = ace::load_dev(at), b = ace::load_dev(at + 1);
+      const uint64_t key = TOP ? ace::load_dev(at + 1 + d) : 0ull;
       sums.clear();
-      if (lane < p.parts) {
-        const unsigned long long* at = all + lane * (2 + p.top);
-        const unsigned long long a = ace::load_dev(at), b = ace::load_dev(at + 1);
+      if (lane < p.parts)
         sums = Sums{__uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)a),
                     __uint_as_float((uint32_t)b)};
-      }
-      sums.over_wave(p.scale);
       if constexpr (TOP) {
-        // each part's d-th best, of which the m-th largest has at least d m >= top
-        // words that reach it
-        const int d = (p.top + p.parts - 1) / p.parts, m = (p.top + d - 1) / d;
-        const uint64_t key =
-            lane < p.parts ? ace::load_dev(all + lane * (2 + p.top) + 1 + d) : 0ull;
-        const uint32_t orders[1] = {(uint32_t)(key >> 32)};
+        const int m = (p.top + d - 1) / d, n = p.parts * p.top;
+        uint64_t held[kMaxParts * kMaxTop / kBlock];
+#pragma unroll
+        for (int i = 0; i < kMaxParts * kMaxTop / kBlock; ++i) {
+          const uint32_t word = (uint32_t)(i * kBlock + thread);
+          held[i] = (int)word < n ? ace::load_dev(all + word / (uint32_t)p.top * (2 + p.top) + 2 +
+                                                  word % (uint32_t)p.top)
+                                  : 0ull;
+        }
+        const uint32_t orders[1] = {lane < p.parts ? (uint32_t)(key >> 32) : 0u};
         best.count = 0;
         best.least = (uint64_t)kth_largest<1>(orders, m, 0) << 32;
-        const int n = p.parts * p.top;
-        for (int i = 0; i < n; i += kBlock) {
-          const int at = i + thread;
-          const uint64_t k =
-              at < n ? ace::load_dev(all + at / p.top * (2 + p.top) + 2 + at % p.top) : 0ull;
-          best.push(k, k != 0, p.top);
-        }
+#pragma unroll
+        for (int i = 0; i < kMaxParts * kMaxTop / kBlock; ++i)
+          best.push(held[i], held[i] != 0, p.top);
         __syncthreads();
         if (lane == 0) s_count[wave] = best.count;
         __syncthreads();
       }
+      sums.over_wave(p.scale);
     }
   }
 
@@ -422,39 +446,35 @@ __global__ __launch_bounds__(kBlock) void backward_kernel(Params p) {
   if (row >= p.rows) return;
   const Saved s = p.saved[row];
   T* out = static_cast<T*>(p.d_logits) + row * p.vocab;
-  T x[kPieces][V];
+  Piece<T> x[kPieces];
   if (s.label >= 0) {
     load_group<T>(static_cast<const T*>(p.logits) + row * p.stride, first, p.vocab, x);
-    float g = (p.grad_logprob ? p.grad_logprob[row] : 0.f) * p.inv_t;
+    const float g = (p.grad_logprob ? p.grad_logprob[row] : 0.f) * p.inv_t;
     const float h = (p.grad_entropy ? p.grad_entropy[row] : 0.f) * p.inv_t;
     const float whole = s.top == s.top ? g : NAN;  // NaN anywhere in the row: everywhere
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
+    for (int u = 0; u < kPieces; ++u) {
+      float d[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         // at most kFar below: p is 0 there, and lp times it too
-        const float lp = fmaxf(((float)x[u][e] - s.top) * p.inv_t - s.log_sum, -kFar);
-        const float pr = exp2_of(lp * kLog2e);
-        float d = -pr * fmaf(h, lp + s.entropy, whole);
-        if (first + u * kTile<T> + lane * V + e == s.label) d += g;
-        x[u][e] = (T)d;
+        const float lp = fmaxf((x[u][e] - s.top) * p.inv_t - s.log_sum, -kFar);
+        d[e] = -exp2_of(lp * kLog2e) * fmaf(h, lp + s.entropy, whole);
+        if (first + u * kTile<T> + lane * V + e == s.label) d[e] += g;
       }
+      x[u].set(d);
+    }
   } else {
 #pragma unroll
-    for (int u = 0; u < kPieces; ++u)
-#pragma unroll
-      for (int e = 0; e < V; ++e) x[u][e] = (T)0.f;
+    for (int u = 0; u < kPieces; ++u) x[u].fill((T)0.f);
   }
 #pragma unroll
   for (int u = 0; u < kPieces; ++u) {
     const int64_t at = first + u * kTile<T> + lane * V;
-    if (at + V <= p.vocab) {
-      __builtin_memcpy(out + at, x[u], 16);
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        if (at + e < p.vocab) out[at + e] = x[u][e];
-    }
+    if (at + V <= p.vocab)
+      x[u].store(out + at);
+    else
+      x[u].store_some(out + at, p.vocab - at);
   }
 }
 

@@ -448,7 +448,7 @@ int ace_expert_order(const int64_t* chosen, int64_t slots, int64_t experts,
  * d_weights.
  * One launch each on `stream`, no allocation, can be captured; results do not vary
  * from run to run.  Returns ACE_EINVAL, ACE_EUNSUPPORTED (width above 2^20, 2^26 slots or
- * pieces of 4096 bytes of tokens or more) or a HIP error.
+ * pieces of 2048 bytes of tokens or more) or a HIP error.
  */
 int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width,
                    int64_t top_k, const int64_t* place, const int64_t* routed,
