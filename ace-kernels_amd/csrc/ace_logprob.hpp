@@ -15,13 +15,16 @@
 // row's parts, by the part that ends last.  Sums are float32 over at most V / 64
 // words a lane.
 //
-// Alternatives: a word's key is its logit's bits in their order above its number's
-// complement, so keys differ and equal logits rank by number, lowest first.  The
-// k-th largest of the lanes' maxima over the team's first words bounds the k-th
-// largest of all from below; only words that reach it are kept as candidates, in
-// LDS, a few dozen in a usual row.  At the end every candidate counts those above
-// it, which is its place.  A wave whose candidates outgrow its LDS (words in
-// ascending order, say) keeps its k best and raises the bound.
+// Alternatives: a key is a logit's bits in their order above the complement of its
+// number, so keys differ and equal logits rank by number, lowest first.  The k
+// largest words are among the k pieces (16 bytes of words) with the largest maxima:
+// each piece before a word's own has a word before it.  The maxima are there anyway, so
+// pieces are what is looked for.  The k-th largest of the lanes' maxima over the
+// team's first words bounds the k-th largest from below; pieces that reach it are
+// kept as candidates, in LDS, a few dozen in a usual row.  At the end every
+// candidate counts those above it, which is its place; then the same for the words
+// of the k best.  A wave whose candidates outgrow its LDS (logits in ascending
+// order, say) keeps its k best and raises the bound.
 #pragma once
 
 #include <float.h>
@@ -42,11 +45,9 @@ constexpr int kBlock = 256;
 constexpr int kPieces = 4;    // of 16 bytes that a lane reads at a time
 constexpr int kMaxTop = 32;
 constexpr int kMaxParts = 32;
-constexpr int kRoom = 256;    // candidates of a wave
+constexpr int kRoom = 128;    // candidates of a wave
 constexpr int kHeld = kRoom + kMaxTop;  // keys of its LDS
 constexpr float kFar = 200.f;  // 2^-200 is 0 in float32: exponents beyond it count as it
-static_assert(kMaxParts * kMaxTop <= kBlock / 64 * kRoom, "the last part has room for all lists");
-
 template <typename T>
 constexpr int kV = 16 / (int)sizeof(T);  // words of a piece
 template <typename T>
@@ -146,13 +147,15 @@ __device__ inline uint32_t order_of(float x) { return x != x ? 0xffffffffu : key
 __device__ inline float logit_of(uint32_t order) {  // NaN also where it is no logit's
   return __uint_as_float(order & 0x80000000u ? order ^ 0x80000000u : ~order);
 }
-__device__ inline uint64_t word_key(uint32_t order, uint32_t word) {
-  return (uint64_t)order << 32 | (0xffffffffu - word);
+__device__ inline uint64_t number_key(uint32_t order, uint32_t number) {
+  return (uint64_t)order << 32 | (0xffffffffu - number);
 }
 
 // A wave's candidates, in its part of LDS.
 struct Candidates {
+  typedef uint32_t Words __attribute__((ext_vector_type(4)));
   uint64_t* keys;   // [kRoom], and room for the best of them
+  Words* pieces;    // what belongs to a key
   int count;        // uniform
   uint64_t least;   // what a key has to reach; uniform
 
@@ -164,42 +167,54 @@ struct Candidates {
     return r;
   }
   // Keeps the `top` best, in order.
+  template <bool PIECES>
   __device__ void shrink(int top) {
     const int lane = (int)threadIdx.x & 63;
     wave_sync();
     for (int i = lane; i < count; i += 64) {
       const uint64_t key = keys[i];
       const int place = above(keys, count, key);
-      if (place < top) keys[kRoom + place] = key;
+      if (place < top) {
+        keys[kRoom + place] = key;
+        if (PIECES) pieces[kRoom + place] = pieces[i];
+      }
     }
     wave_sync();
     if (count > top) count = top;
-    if (lane < count) keys[lane] = keys[kRoom + lane];
+    if (lane < count) {
+      keys[lane] = keys[kRoom + lane];
+      if (PIECES) pieces[lane] = pieces[kRoom + lane];
+    }
     wave_sync();
     if (count == top) least = keys[top - 1];
   }
-  // One key a lane, where `on`.
-  __device__ void push(uint64_t key, bool on, int top) {
+  // One key a lane, where `on`, with its piece.
+  template <bool PIECES>
+  __device__ void push(uint64_t key, Words piece, bool on, int top) {
     on = on && key >= least;
     unsigned long long m = __ballot(on);
     if (!m) return;
     if (count + __popcll(m) > kRoom) {
-      shrink(top);
+      shrink<PIECES>(top);
       on = on && key >= least;
       m = __ballot(on);
     }
     const int lane = (int)threadIdx.x & 63;
-    if (on) keys[count + __popcll(m & ((1ull << lane) - 1))] = key;
+    if (on) {
+      const int at = count + __popcll(m & ((1ull << lane) - 1));
+      keys[at] = key;
+      if (PIECES) pieces[at] = piece;
+    }
     count += __popcll(m);
   }
 };
 
-// The k-th largest of the wave's N values a lane, from below: exact in the bits from
-// `low` on.
+// A bound of the k-th largest of the wave's N values a lane, from below: its upper
+// half, which 16 bits have all of and a float 7 bits behind the exponent.
 template <int N>
-__device__ inline uint32_t kth_largest(const uint32_t (&x)[N], int k, int low) {
+__device__ inline uint32_t kth_largest(const uint32_t (&x)[N], int k) {
   uint32_t found = 0;
-  for (int b = 31; b >= low; --b) {
+  for (int b = 31; b >= 16; --b) {
     const uint32_t next = found | 1u << b;
     int reach = 0;
 #pragma unroll
@@ -215,6 +230,8 @@ template <typename T, int W, bool TOP>
 __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
   constexpr int V = kV<T>, kTeams = kBlock / 64 / W;
   __shared__ uint64_t s_keys[TOP ? kBlock / 64 * kHeld : 1];
+  __shared__ Candidates::Words s_pieces[TOP ? kBlock / 64 * kHeld : 1];
+  __shared__ int s_slot[TOP ? kTeams * kMaxTop : 1];
   __shared__ uint32_t s_max[TOP && W > 1 ? kBlock : 1];
   __shared__ int s_count[TOP ? kBlock / 64 : 1];
   __shared__ Sums s_sums[W > 1 ? W : 1];
@@ -250,7 +267,7 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
 
   Sums sums;
   sums.clear();
-  Candidates best{s_keys + (TOP ? wave * kHeld : 0), 0, 0};
+  Candidates best{s_keys + (TOP ? wave * kHeld : 0), s_pieces + (TOP ? wave * kHeld : 0), 0, 0};
   float reach = 0.f;  // what a logit has to reach to be a candidate; NaN: nothing
   bool first = true;
   for (int64_t v = v0; v < v1; v += W * kGroup<T>) {
@@ -265,6 +282,9 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
       for (int e = 2; e < V; e += 2)
         tops[u] = max_of(max_of(tops[u], x[u][e]), x[u][e + 1]);
       t = max_of(t, tops[u]);
+      // unpacked again for the exponentials: with all floats kept beside the pieces,
+      // four waves fit a SIMD instead of seven (4096 x 32000, top 20: 68 us instead of 61)
+      if constexpr (TOP) asm volatile("" : "+v"(x[u].words));
     }
     sums.raise(max_of(sums.top, t), p.scale);
     float sum = 0.f, pull = 0.f;
@@ -281,7 +301,6 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
     sums.pull += pull;
     if constexpr (TOP) {
       if (first) {
-        constexpr int low = sizeof(T) == 2 ? 16 : 0;
         const uint32_t order = order_of(t);
         uint32_t least;
         if constexpr (W > 1) {
@@ -290,39 +309,23 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
           uint32_t all[W];
 #pragma unroll
           for (int i = 0; i < W; ++i) all[i] = s_max[i * 64 + lane];
-          least = kth_largest<W>(all, p.top, low);
+          least = kth_largest<W>(all, p.top);
         } else {
           const uint32_t all[1] = {order};
-          least = kth_largest<1>(all, p.top, low);
+          least = kth_largest<1>(all, p.top);
         }
         best.least = (uint64_t)least << 32;
         reach = logit_of(least);
       }
       if (__ballot(!(t < reach))) {
-        // seldom, so it reads its words again (from a cache): with all pieces still in
-        // registers half as many waves would fit
-#pragma unroll 1
+#pragma unroll
         for (int u = 0; u < kPieces; ++u) {
-          float tile = tops[0];
-#pragma unroll
-          for (int i = 1; i < kPieces; ++i) tile = u == i ? tops[i] : tile;
-          if (!__ballot(!(tile < reach))) continue;
-          Piece<T> y;
-          load_piece<T>(logits, mine + u * kTile<T> + lane * V, v1, y);
-          uint32_t mask = 0;
-#pragma unroll
-          for (int e = 0; e < V; ++e) mask |= !(y[e] < reach) ? 1u << e : 0u;
-          const int64_t word = mine + u * kTile<T> + lane * V;
-          while (__ballot(mask != 0)) {
-            const int at = __builtin_ctz(mask | 1u << V);
-            float l = y[0];
-#pragma unroll
-            for (int e = 1; e < V; ++e) l = at == e ? y[e] : l;
-            best.push(word_key(order_of(l), (uint32_t)(word + at)), mask && word + at < v1, p.top);
-            mask &= mask - 1;
-          }
+          if (!__ballot(!(tops[u] < reach))) continue;
+          const int64_t at = mine + u * kTile<T> + lane * V;
+          best.push<true>(number_key(order_of(tops[u]), (uint32_t)(at / V)), x[u].words, at < v1,
+                          p.top);
         }
-        // words that follow have higher numbers: an equal logit is no candidate
+        // pieces that follow have higher numbers: an equal logit is no candidate
         if ((uint32_t)best.least) reach = logit_of((uint32_t)(best.least >> 32) + 1);
       }
     }
@@ -351,18 +354,47 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
     }
   }
 
-  // Every candidate's place among the team's: `put(place, key)` for the first `top`.
+  // Every candidate's place among the team's: `put(place, key, slot)` for the first
+  // `top`.
   const auto rank = [&](auto put) {
     const uint64_t* keys = s_keys + team * W * kHeld;
     const int* count = s_count + team * W;
-    for (int w = 0; w < W; ++w)
-      for (int i = thread; i < count[w]; i += W * 64) {
-        const uint64_t key = keys[w * kHeld + i];
-        int place = 0;
-        for (int o = 0; o < W; ++o) place += Candidates::above(keys + o * kHeld, count[o], key);
-        if (place < p.top) put(place, key);
-      }
+    for (int i = lane; i < best.count; i += 64) {  // each wave its own
+      const uint64_t key = best.keys[i];
+      int place = 0;
+      for (int o = 0; o < W; ++o) place += Candidates::above(keys + o * kHeld, count[o], key);
+      if (place < p.top) put(place, key, mate * kHeld + i);
+    }
   };
+  if constexpr (TOP) {  // pieces are ranked, then the words of the best
+    constexpr int kRounds = (kMaxTop * V + W * 64 - 1) / (W * 64);
+    const uint64_t* keys = s_keys + team * W * kHeld;
+    const Candidates::Words* pieces = s_pieces + team * W * kHeld;
+    int* slots = s_slot + team * kMaxTop;
+    int held = 0;
+    for (int w = 0; w < W; ++w) held += s_count[team * W + w];
+    if (held > p.top) held = p.top;
+    rank([&](int place, uint64_t, int slot) { slots[place] = slot; });
+    team_sync();
+    uint64_t words[kRounds];
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) {
+      const int i = r * W * 64 + thread;
+      words[r] = 0;
+      if (i >= held * V) continue;
+      const int slot = slots[i / V];
+      const int64_t word = (int64_t)(0xffffffffu - (uint32_t)keys[slot]) * V + i % V;
+      const float l = (float)reinterpret_cast<const T*>(pieces + slot)[i % V];
+      if (word < v1) words[r] = number_key(order_of(l), (uint32_t)word);
+    }
+    best.least = held == p.top ? keys[slots[p.top - 1]] & 0xffffffff00000000u : 0;
+    team_sync();
+    best.count = 0;
+#pragma unroll
+    for (int r = 0; r < kRounds; ++r) best.push<false>(words[r], {}, words[r] != 0, p.top);
+    if (lane == 0) s_count[wave] = best.count;
+    team_sync();
+  }
 
   if constexpr (W > 1) {
     if (p.parts > 1) {
@@ -376,7 +408,9 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
       if constexpr (TOP) {
         int held = 0;
         for (int w = 0; w < W; ++w) held += s_count[w];
-        rank([&](int place, uint64_t key) { ace::store_dev(own + 2 + place, (unsigned long long)key); });
+        rank([&](int place, uint64_t key, int) {
+          ace::store_dev(own + 2 + place, (unsigned long long)key);
+        });
         if (thread >= held && thread < p.top) ace::store_dev(own + 2 + thread, 0ull);
       }
       if (!ace::last_of(p.tickets + row * kTicketStride, p.parts)) return;
@@ -402,10 +436,10 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
         }
         const uint32_t orders[1] = {lane < p.parts ? (uint32_t)(key >> 32) : 0u};
         best.count = 0;
-        best.least = (uint64_t)kth_largest<1>(orders, m, 0) << 32;
+        best.least = (uint64_t)kth_largest<1>(orders, m) << 32;
 #pragma unroll
         for (int i = 0; i < kMaxParts * kMaxTop / kBlock; ++i)
-          best.push(held[i], held[i] != 0, p.top);
+          best.push<false>(held[i], {}, held[i] != 0, p.top);
         __syncthreads();
         if (lane == 0) s_count[wave] = best.count;
         __syncthreads();
@@ -427,7 +461,7 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
     p.saved[row] = Saved{defined ? sums.top : NAN, log_sum, entropy, dead && defined ? -1 : (int)y};
   }
   if constexpr (TOP)
-    rank([&](int place, uint64_t key) {
+    rank([&](int place, uint64_t key, int) {
       p.top_logprobs[row * p.top + place] = logprob_of(logit_of((uint32_t)(key >> 32)));
       p.top_tokens[row * p.top + place] = (int64_t)(0xffffffffu - (uint32_t)key);
     });
