@@ -247,7 +247,7 @@ def lib() -> ctypes.CDLL:
     handle.ace_to_experts.restype = _i
     handle.ace_to_experts.argtypes = [_p, _i, _i64, _i64, _i64, _p, _p, _p, _p]
     handle.ace_from_experts.restype = _i
-    handle.ace_from_experts.argtypes = [_p, _i, _i64, _i64, _i64, _p, _p, _p, _p]
+    handle.ace_from_experts.argtypes = [_p, _i, _i64, _i64, _i64, _p, _p, _p, _p, _p]
     handle.ace_from_experts_backward.restype = _i
     handle.ace_from_experts_backward.argtypes = [_p, _p, _i, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p]
     handle.ace_set_launch_events.restype = _i

@@ -18,9 +18,15 @@ the softmax over them, or with ``normalize=False`` over all experts.  A masked t
 takes none: its experts are -1, its weights 0, its scores are not read, and its output
 is 0.  Experts at -inf have weight 0.
 
-Rows of ``to_experts`` behind the last routed one (``order.offsets[-1]``) are 0; those
-of ``from_experts``'s input are not read (they may be NaN) and get a gradient of 0.
-Copies are exact; sums are float32, rounded once.
+A choice is dropped by a ``place`` of -1, for instance those beyond an expert's capacity
+(without masked tokens, whose -1 is no index)::
+
+    late = order.place - order.offsets[routes.experts] >= capacity
+    order = order._replace(place=order.place.masked_fill(late, -1))
+
+Rows without a choice, those behind the last (``order.offsets[-1]``) among them, are 0
+in ``to_experts``; in ``from_experts`` they are not read (they may be NaN) and get a
+gradient of 0.  Copies are exact; sums are float32, rounded once.
 
 The calls and their backward nodes are C++ (``csrc/ace_autograd.cpp``).  They have no
 forward-mode and no second derivative, and ``torch.func`` transforms do not know them;
@@ -118,28 +124,27 @@ def expert_order(experts: torch.Tensor, num_experts: int) -> ExpertOrder:
 
 
 def _check_rows(what: str, rows: torch.Tensor, order: ExpertOrder) -> None:
-    offsets, source, place = order
+    _, source, place = order
     if rows.device.type != "cuda":
         raise ValueError(f"{what} needs HIP ('cuda') tensors, got {rows.device}")
     if rows.dtype not in _DTYPES:
         raise TypeError(f"{what} takes float32, bfloat16 or float16 rows, got {rows.dtype}")
-    if offsets.dtype != torch.int64 or place.dtype != torch.int64:
-        raise TypeError(f"the order must be int64, as expert_order gives it, got {offsets.dtype} and {place.dtype}")
-    if offsets.device != rows.device or place.device != rows.device:
-        raise ValueError(f"the rows are on {rows.device}, the order on {offsets.device} and {place.device}")
-    if offsets.dim() != 1 or offsets.shape[0] < 2 or place.dim() < 1 or place.shape[-1] < 1 \
-            or source.shape != (place.numel(),):
-        raise ValueError("the order must be expert_order's: offsets [E + 1], source [slots] and place [..., top_k], got "
-                         f"{tuple(offsets.shape)}, {tuple(source.shape)} and {tuple(place.shape)}")
+    if source.dtype != torch.int64 or place.dtype != torch.int64:
+        raise TypeError(f"the order must be int64, as expert_order gives it, got {source.dtype} and {place.dtype}")
+    if source.device != rows.device or place.device != rows.device:
+        raise ValueError(f"the rows are on {rows.device}, the order on {source.device} and {place.device}")
+    if place.dim() < 1 or place.shape[-1] < 1 or source.shape != (place.numel(),):
+        raise ValueError("the order must be expert_order's: source [slots] and place [..., top_k], got "
+                         f"{tuple(source.shape)} and {tuple(place.shape)}")
 
 
 def to_experts(x: torch.Tensor, order: ExpertOrder) -> torch.Tensor:
     """Rows of tokens ``x`` ``[..., W]`` in expert order, ``[slots, W]``: each token's row at
-    its ``top_k`` places, 0 behind the last.  Differentiable once in ``x``."""
+    its ``top_k`` places, 0 where nothing is.  Differentiable once in ``x``."""
     _check_rows("to_experts", x, order)
     if x.dim() < 1 or x.shape[-1] < 1 or x.shape[:-1] != order.place.shape[:-1]:
         raise ValueError(f"x must be {(*order.place.shape[:-1], 'W')}, a row per token of the order, got {tuple(x.shape)}")
-    return _lib.autograd().to_experts(x, order.offsets, order.place)
+    return _lib.autograd().to_experts(x, order.source, order.place)
 
 
 def from_experts(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -157,4 +162,4 @@ def from_experts(rows: torch.Tensor, order: ExpertOrder, weights: Optional[torch
             raise TypeError(f"weights must be float32, bfloat16 or float16, got {weights.dtype}")
         if weights.dtype != torch.float32:
             weights = weights.float()
-    return _lib.autograd().from_experts(rows, order.offsets, order.place, weights)
+    return _lib.autograd().from_experts(rows, order.source, order.place, weights)

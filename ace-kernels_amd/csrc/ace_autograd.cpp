@@ -735,10 +735,6 @@ std::vector<at::Tensor> expert_order(const at::Tensor& experts, int64_t num_expe
   return {offsets, source, place};
 }
 
-const int64_t* last_offset(const at::Tensor& offsets) {
-  return offsets.data_ptr<int64_t>() + offsets.numel() - 1;
-}
-
 struct ToExpertsBackward : public Node {
   std::string name() const override { return "ToExpertsBackward"; }
 
@@ -747,7 +743,7 @@ struct ToExpertsBackward : public Node {
     const at::Tensor& g = grads[0];
     if (!g.defined()) return out;
     refuse_tangents({g}, "to_experts's gradient");
-    const at::Tensor place = place_.unpack();
+    const at::Tensor source = source_.unpack(), place = place_.unpack();
     {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(g.device());
@@ -755,35 +751,40 @@ struct ToExpertsBackward : public Node {
       out[0] = at::empty(shape, g.options().requires_grad(false));
       const int64_t top_k = place.size(-1);
       const int rc = g_from_experts.load()(rows.data_ptr(), dtype_code(g), place.numel() / top_k,
-                                           shape.back(), top_k, place.data_ptr<int64_t>(), nullptr,
-                                           out[0].data_ptr(), current_stream(g));
+                                           shape.back(), top_k, source.data_ptr<int64_t>(),
+                                           place.data_ptr<int64_t>(), nullptr, out[0].data_ptr(),
+                                           current_stream(g));
       if (rc) fail(rc, "ace_from_experts");
     }
     refuse_second_derivative(out, {g}, "to_experts");
     return out;
   }
 
-  void release_variables() override { place_.reset_data(); }
+  void release_variables() override {
+    source_.reset_data();
+    place_.reset_data();
+  }
 
   std::vector<int64_t> shape;
-  SavedVariable place_;
+  SavedVariable source_, place_;
 };
 
 // The rows of checked arguments.
-at::Tensor to_experts(const at::Tensor& x, const at::Tensor& offsets, const at::Tensor& place) {
+at::Tensor to_experts(const at::Tensor& x, const at::Tensor& source, const at::Tensor& place) {
   if (!g_to_experts.load()) throw std::runtime_error("ace_autograd: entry points not set");
   refuse_tangents({x}, "to_experts");
   const bool record = torch::autograd::compute_requires_grad(x);
   const c10::DeviceGuard guard(x.device());
-  at::Tensor rows, at;
+  at::Tensor rows, of, at;
   {
     const at::NoGradGuard no_grad;
-    const at::Tensor in = plain(x), ends = offsets.contiguous();
+    const at::Tensor in = plain(x);
+    of = source.contiguous();
     at = place.contiguous();
     const int64_t top_k = at.size(-1), width = x.size(-1);
     rows = at::empty({at.numel(), width}, x.options().requires_grad(false));
     const int rc = g_to_experts.load()(in.data_ptr(), dtype_code(x), at.numel() / top_k, width,
-                                       top_k, at.data_ptr<int64_t>(), last_offset(ends),
+                                       top_k, of.data_ptr<int64_t>(), at.data_ptr<int64_t>(),
                                        rows.data_ptr(), current_stream(x));
     if (rc) fail(rc, "ace_to_experts");
   }
@@ -792,6 +793,7 @@ at::Tensor to_experts(const at::Tensor& x, const at::Tensor& offsets, const at::
                                                    torch::autograd::deleteNode);
     node->set_next_edges(torch::autograd::collect_next_edges(x));
     node->shape.assign(x.sizes().begin(), x.sizes().end());
+    node->source_ = SavedVariable(of, false);
     node->place_ = SavedVariable(at, false);
     torch::autograd::set_history(rows, node);
   }
@@ -806,7 +808,7 @@ struct FromExpertsBackward : public Node {
     const at::Tensor& g = grads[0];
     if (!g.defined()) return out;
     refuse_tangents({g}, "from_experts's gradient");
-    const at::Tensor place = place_.unpack(), offsets = offsets_.unpack(), rows = rows_.unpack(),
+    const at::Tensor place = place_.unpack(), source = source_.unpack(), rows = rows_.unpack(),
                      weights = weights_.unpack();
     {
       const at::NoGradGuard no_grad;
@@ -822,7 +824,7 @@ struct FromExpertsBackward : public Node {
       }
       const int rc = g_from_experts_backward.load()(
           in.defined() ? in.data_ptr() : nullptr, up.data_ptr(), dtype_code(g), slots / top_k,
-          width, top_k, place.data_ptr<int64_t>(), last_offset(offsets),
+          width, top_k, source.data_ptr<int64_t>(), place.data_ptr<int64_t>(),
           w.defined() ? w.data_ptr<float>() : nullptr,
           out[0].defined() ? out[0].data_ptr() : nullptr,
           out[1].defined() ? out[1].data_ptr<float>() : nullptr, current_stream(g));
@@ -835,32 +837,33 @@ struct FromExpertsBackward : public Node {
   void release_variables() override {
     rows_.reset_data();
     weights_.reset_data();
+    source_.reset_data();
     place_.reset_data();
-    offsets_.reset_data();
   }
 
-  SavedVariable rows_, weights_, place_, offsets_;
+  SavedVariable rows_, weights_, source_, place_;
 };
 
 // The tokens' rows of checked arguments.
-at::Tensor from_experts(const at::Tensor& rows, const at::Tensor& offsets, const at::Tensor& place,
+at::Tensor from_experts(const at::Tensor& rows, const at::Tensor& source, const at::Tensor& place,
                         const std::optional<at::Tensor>& weights) {
   if (!g_from_experts.load()) throw std::runtime_error("ace_autograd: entry points not set");
   const at::Tensor factor = weights ? *weights : at::Tensor();
   refuse_tangents({rows, factor}, "from_experts");
   const bool record = torch::autograd::compute_requires_grad(rows, factor);
   const c10::DeviceGuard guard(rows.device());
-  at::Tensor out, at;
+  at::Tensor out, of, at;
   {
     const at::NoGradGuard no_grad;
     const at::Tensor in = plain(rows), w = factor.defined() ? plain(factor) : factor;
+    of = source.contiguous();
     at = place.contiguous();
     const int64_t top_k = at.size(-1), width = rows.size(-1);
     std::vector<int64_t> shape(at.sizes().begin(), at.sizes().end());
     shape.back() = width;
     out = at::empty(shape, rows.options().requires_grad(false));
     const int rc = g_from_experts.load()(in.data_ptr(), dtype_code(rows), at.numel() / top_k, width,
-                                         top_k, at.data_ptr<int64_t>(),
+                                         top_k, of.data_ptr<int64_t>(), at.data_ptr<int64_t>(),
                                          w.defined() ? w.data_ptr<float>() : nullptr,
                                          out.data_ptr(), current_stream(rows));
     if (rc) fail(rc, "ace_from_experts");
@@ -872,8 +875,8 @@ at::Tensor from_experts(const at::Tensor& rows, const at::Tensor& offsets, const
     // the rows only for the weights' gradient
     if (factor.defined() && factor.requires_grad()) node->rows_ = SavedVariable(rows, false);
     if (factor.defined()) node->weights_ = SavedVariable(factor, false);
+    node->source_ = SavedVariable(of, false);
     node->place_ = SavedVariable(at, false);
-    node->offsets_ = SavedVariable(offsets.contiguous(), false);
     torch::autograd::set_history(out, node);
   }
   return out;

@@ -18,10 +18,9 @@ int launched() {
 }
 
 int64_t order_blocks(int64_t slots, int64_t* per_block) {
-  // 1024 slots a block: four rounds of a wave; at most kMaxBlocks
-  int64_t each = 1024;
-  if (slots > each * kMaxBlocks) each = (slots + kMaxBlocks - 1) / kMaxBlocks;
-  *per_block = (each + kBlock - 1) / kBlock * kBlock;
+  // a slot a thread; more from kMaxBlocks on
+  const int64_t each = slots > kOrderBlock * kMaxBlocks ? (slots + kMaxBlocks - 1) / kMaxBlocks : 1;
+  *per_block = (each + kOrderBlock - 1) / kOrderBlock * kOrderBlock;
   const int64_t blocks = (slots + *per_block - 1) / *per_block;
   return blocks < 1 ? 1 : blocks;
 }
@@ -32,10 +31,10 @@ int64_t pieces_of(int64_t width, int dtype, int deep) {
 }
 
 int check(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_k,
-          const int64_t* place) {
+          const int64_t* source, const int64_t* place) {
   if (dtype != ACE_F32 && dtype != ACE_BF16 && dtype != ACE_F16) return ACE_EINVAL;
   if (tokens < 0 || width < 1 || top_k < 1) return ACE_EINVAL;
-  if (tokens > 0 && (!in || !place)) return ACE_EINVAL;
+  if (tokens > 0 && (!in || !source || !place)) return ACE_EINVAL;
   if (width > kMaxWidth || top_k > kMaxSlots || tokens > kMaxSlots || tokens * top_k > kMaxSlots)
     return ACE_EUNSUPPORTED;
   if (tokens * pieces_of(width, dtype, kDeepFrom) >= kMaxWaves || tokens * top_k >= kMaxWaves)
@@ -43,14 +42,15 @@ int check(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_
   return ACE_OK;
 }
 
-RowsParams params(const void* in, int64_t tokens, int64_t width, int64_t top_k, const int64_t* place,
-                  const float* weights) {
+RowsParams params(const void* in, int64_t tokens, int64_t width, int64_t top_k,
+                  const int64_t* source, const int64_t* place, const float* weights) {
   RowsParams p{};
   p.in = in;
   p.tokens = tokens;
   p.slots = tokens * top_k;
   p.width = (int)width;
   p.top_k = (int)top_k;
+  p.source = source;
   p.place = place;
   p.weights = weights;
   return p;
@@ -103,7 +103,7 @@ int ace_expert_order(const int64_t* chosen, int64_t slots, int64_t experts, int6
   p.offsets = offsets;
   p.source = source;
   p.place = place;
-  const dim3 grid((unsigned)p.blocks), block(kBlock);
+  const dim3 grid((unsigned)p.blocks), block(kOrderBlock);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   if (p.blocks > 1) {
     hipLaunchKernelGGL(count_kernel, grid, block, 0, s, p);
@@ -115,13 +115,12 @@ int ace_expert_order(const int64_t* chosen, int64_t slots, int64_t experts, int6
 }
 
 int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width, int64_t top_k,
-                   const int64_t* place, const int64_t* routed, void* rows, void* stream) {
-  const int bad = check(x, dtype, tokens, width, top_k, place);
+                   const int64_t* source, const int64_t* place, void* rows, void* stream) {
+  const int bad = check(x, dtype, tokens, width, top_k, source, place);
   if (bad) return bad;
   if (tokens == 0) return ACE_OK;
-  if (!routed || !rows) return ACE_EINVAL;
-  RowsParams p = params(x, tokens, width, top_k, place, nullptr);
-  p.offsets = routed;
+  if (!rows) return ACE_EINVAL;
+  RowsParams p = params(x, tokens, width, top_k, source, place, nullptr);
   p.out = rows;
   p.pieces = (int)pieces_of(width, dtype, kDeepTo);
   const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
@@ -135,12 +134,13 @@ int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width, int6
 }
 
 int ace_from_experts(const void* rows, int dtype, int64_t tokens, int64_t width, int64_t top_k,
-                     const int64_t* place, const float* weights, void* out, void* stream) {
-  const int bad = check(rows, dtype, tokens, width, top_k, place);
+                     const int64_t* source, const int64_t* place, const float* weights, void* out,
+                     void* stream) {
+  const int bad = check(rows, dtype, tokens, width, top_k, source, place);
   if (bad) return bad;
   if (tokens == 0) return ACE_OK;
   if (!out) return ACE_EINVAL;
-  RowsParams p = params(rows, tokens, width, top_k, place, weights);
+  RowsParams p = params(rows, tokens, width, top_k, source, place, weights);
   p.out = out;
   p.pieces = (int)pieces_of(width, dtype, kDeepFrom);
   const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
@@ -154,17 +154,16 @@ int ace_from_experts(const void* rows, int dtype, int64_t tokens, int64_t width,
 }
 
 int ace_from_experts_backward(const void* rows, const void* grad, int dtype, int64_t tokens,
-                              int64_t width, int64_t top_k, const int64_t* place,
-                              const int64_t* routed, const float* weights, void* d_rows,
+                              int64_t width, int64_t top_k, const int64_t* source,
+                              const int64_t* place, const float* weights, void* d_rows,
                               float* d_weights, void* stream) {
   // without the weights' gradient the rows are not read
-  const int bad = check(d_weights ? rows : grad, dtype, tokens, width, top_k, place);
+  const int bad = check(d_weights ? rows : grad, dtype, tokens, width, top_k, source, place);
   if (bad) return bad;
   if (tokens == 0 || (!d_rows && !d_weights)) return ACE_OK;
-  if (!grad || !routed) return ACE_EINVAL;
-  RowsParams p = params(rows, tokens, width, top_k, place, weights);
+  if (!grad) return ACE_EINVAL;
+  RowsParams p = params(rows, tokens, width, top_k, source, place, weights);
   p.grad = grad;
-  p.offsets = routed;
   p.out = d_rows;
   p.d_weights = d_weights;
   const hipStream_t s = static_cast<hipStream_t>(stream);

@@ -9,7 +9,7 @@ namespace route {
 namespace {
 
 constexpr int64_t kMaxTokens = (int64_t)1 << 30;
-constexpr int64_t kTarget = 2048;  // blocks to aim at: eight on each CU
+constexpr int64_t kTarget = 4096;  // blocks to aim at: sixteen on each CU
 
 int check(const void* logits, int dtype, int64_t tokens, int64_t experts, int top_k) {
   if (dtype != ACE_F32 && dtype != ACE_BF16 && dtype != ACE_F16) return ACE_EINVAL;

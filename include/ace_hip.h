@@ -433,32 +433,33 @@ int ace_expert_order(const int64_t* chosen, int64_t slots, int64_t experts,
 
 /*
  * Rows of tokens in expert order, and back.  No counterpart in the reference.  Tokens
- * have `width` elements (ACE_F32, ACE_BF16 or ACE_F16) and top_k slots each; place
- * [tokens, top_k] is ace_expert_order's, `routed` its last offset (device memory).  A
- * place outside [0, tokens top_k) is none.  All tensors are contiguous; outputs may not
- * overlap inputs.
+ * have `width` elements (ACE_F32, ACE_BF16 or ACE_F16) and top_k slots each; source
+ * [tokens top_k] and place [tokens, top_k] are ace_expert_order's.  Slot s is at row r
+ * where place[s] = r and source[r] = s: a caller drops a choice by a place of -1, and
+ * numbers outside [0, tokens top_k) are none.  All tensors are contiguous; outputs may
+ * not overlap inputs.
  *
- * ace_to_experts: rows [tokens top_k, width], rows[place[t, j]] = x[t]; rows from
- * `routed` on are 0.
- * ace_from_experts: out[t] = sum_j weights[t, j] rows[place[t, j]] over its placed
- * slots, summed in float32 and rounded once; weights [tokens, top_k] float32 or NULL,
- * for 1 (the gradient of ace_to_experts).  Rows that nothing is placed at are not read.
- * ace_from_experts_backward: from the gradient of out, d_rows (0 from `routed` on) and
- * d_weights (0 without a place), either skipped if NULL; `rows` may be NULL without
+ * ace_to_experts: rows [tokens top_k, width], each the token's whose slot is there, or 0.
+ * ace_from_experts: out[t] = sum_j weights[t, j] rows[place[t, j]] over its slots that are
+ * at a row, summed in float32 and rounded once; weights [tokens, top_k] float32 or NULL,
+ * for 1 (the gradient of ace_to_experts).  Rows without a slot are not read.
+ * ace_from_experts_backward: from the gradient of out, d_rows (0 without a slot) and
+ * d_weights (0 without a row), either skipped if NULL; `rows` may be NULL without
  * d_weights.
  * One launch each on `stream`, no allocation, can be captured; results do not vary
  * from run to run.  Returns ACE_EINVAL, ACE_EUNSUPPORTED (width above 2^20, 2^26 slots or
  * pieces of 2048 bytes of tokens or more) or a HIP error.
  */
 int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width,
-                   int64_t top_k, const int64_t* place, const int64_t* routed,
+                   int64_t top_k, const int64_t* source, const int64_t* place,
                    void* rows, void* stream);
 int ace_from_experts(const void* rows, int dtype, int64_t tokens,
-                     int64_t width, int64_t top_k, const int64_t* place,
-                     const float* weights, void* out, void* stream);
+                     int64_t width, int64_t top_k, const int64_t* source,
+                     const int64_t* place, const float* weights, void* out,
+                     void* stream);
 int ace_from_experts_backward(const void* rows, const void* grad, int dtype,
                               int64_t tokens, int64_t width, int64_t top_k,
-                              const int64_t* place, const int64_t* routed,
+                              const int64_t* source, const int64_t* place,
                               const float* weights, void* d_rows,
                               float* d_weights, void* stream);
 

@@ -83,11 +83,10 @@ def test_rows_refusals() -> None:
     with pytest.raises(TypeError, match="weights must be"):
         from_experts(Claims(rows), order, Claims(torch.randn(5, 2).double()))
     with pytest.raises(TypeError, match="must be int64"):
-        to_experts(Claims(x), order._replace(offsets=Claims(torch.zeros(9))))
+        to_experts(Claims(x), order._replace(source=Claims(torch.zeros(10))))
     with pytest.raises(ValueError, match="the order on"):
-        to_experts(Claims(x), order._replace(offsets=torch.zeros(9, dtype=I64)))
-    for bad in (dict(offsets=Claims(torch.zeros(1, dtype=I64))), dict(offsets=Claims(torch.zeros(3, 3, dtype=I64))),
-                dict(source=Claims(torch.zeros(9, dtype=I64)))):
+        to_experts(Claims(x), order._replace(source=torch.zeros(10, dtype=I64)))
+    for bad in (dict(source=Claims(torch.zeros(9, dtype=I64))), dict(source=Claims(torch.zeros(5, 2, dtype=I64)))):
         with pytest.raises(ValueError, match="expert_order's"):
             to_experts(Claims(x), order._replace(**bad))
 
@@ -145,40 +144,40 @@ def test_order_limits() -> None:
 
 
 def _to(**changed):
-    a = dict(x=FAKE, dtype=_lib.BF16, tokens=10, width=64, top_k=2, place=FAKE, routed=FAKE, rows=FAKE)
+    a = dict(x=FAKE, dtype=_lib.BF16, tokens=10, width=64, top_k=2, source=FAKE, place=FAKE, rows=FAKE)
     a.update(changed)
     return _lib.lib().ace_to_experts(*a.values(), None)
 
 
 def _from(**changed):
-    a = dict(x=FAKE, dtype=_lib.BF16, tokens=10, width=64, top_k=2, place=FAKE, weights=FAKE, out=FAKE)
+    a = dict(x=FAKE, dtype=_lib.BF16, tokens=10, width=64, top_k=2, source=FAKE, place=FAKE, weights=FAKE, out=FAKE)
     a.update(changed)
     return _lib.lib().ace_from_experts(*a.values(), None)
 
 
 def _from_back(**changed):
-    a = dict(x=FAKE, grad=FAKE, dtype=_lib.BF16, tokens=10, width=64, top_k=2, place=FAKE, routed=FAKE, weights=FAKE,
+    a = dict(x=FAKE, grad=FAKE, dtype=_lib.BF16, tokens=10, width=64, top_k=2, source=FAKE, place=FAKE, weights=FAKE,
              d_rows=FAKE, d_weights=FAKE)
     a.update(changed)
     return _lib.lib().ace_from_experts_backward(*a.values(), None)
 
 
 @pytest.mark.parametrize("changed", [dict(x=None), dict(dtype=_lib.F64), dict(tokens=-1), dict(width=0), dict(top_k=0),
-                                     dict(place=None)])
+                                     dict(source=None), dict(place=None)])
 def test_rows_refuse_before_launch(changed) -> None:
     for call in (_to, _from, _from_back):
         assert call(**changed) == _lib.EINVAL
 
 
 def test_rows_limits() -> None:
-    assert _to(routed=None) == _lib.EINVAL and _to(rows=None) == _lib.EINVAL and _from(out=None) == _lib.EINVAL
-    assert _from_back(grad=None) == _lib.EINVAL and _from_back(routed=None) == _lib.EINVAL
+    assert _to(rows=None) == _lib.EINVAL and _from(out=None) == _lib.EINVAL
+    assert _from_back(grad=None) == _lib.EINVAL
     for call in (_to, _from, _from_back):
         assert call(width=(1 << 20) + 1) == _lib.EUNSUPPORTED
         assert call(tokens=1 << 25) == _lib.EUNSUPPORTED  # 2^26 slots
         assert call(tokens=1 << 20, width=1 << 20) == _lib.EUNSUPPORTED
         assert call(tokens=1 << 40, top_k=1 << 40) == _lib.EUNSUPPORTED
-        assert call(tokens=0, x=None, place=None) == 0  # nothing to do
+        assert call(tokens=0, x=None, source=None, place=None) == 0  # nothing to do
     assert _from_back(d_rows=None, d_weights=None) == 0
 
 
@@ -186,14 +185,14 @@ def test_tangents_are_refused() -> None:
     import torch.autograd.forward_ad as fwd
 
     mod, x = _lib.autograd(), torch.randn(5, 8)
-    ends, place = torch.zeros(3, dtype=I64), torch.zeros(5, 1, dtype=I64)
+    source, place = torch.zeros(5, dtype=I64), torch.zeros(5, 1, dtype=I64)
     with fwd.dual_level():
         dual = fwd.make_dual(x, torch.ones_like(x))
         with pytest.raises(NotImplementedError, match="route_tokens has no forward-mode derivative"):
             mod.route_tokens(dual, None, 2, True)
         with pytest.raises(NotImplementedError, match="to_experts has no forward-mode derivative"):
-            mod.to_experts(dual, ends, place)
+            mod.to_experts(dual, source, place)
         with pytest.raises(NotImplementedError, match="from_experts has no forward-mode derivative"):
-            mod.from_experts(dual, ends, place, None)
+            mod.from_experts(dual, source, place, None)
         with pytest.raises(NotImplementedError, match="from_experts has no forward-mode derivative"):
-            mod.from_experts(x, ends, place, fwd.make_dual(x[:, :1], torch.ones(5, 1)))
+            mod.from_experts(x, source, place, fwd.make_dual(x[:, :1], torch.ones(5, 1)))

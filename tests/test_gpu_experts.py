@@ -12,7 +12,7 @@ import math
 import pytest
 import torch
 
-from ace_kernels import (BalanceConfig, ExpertOrder, RouteConfig, balance_loss, expert_order, from_experts, route_tokens,
+from ace_kernels import (BalanceConfig, RouteConfig, balance_loss, expert_order, from_experts, route_tokens,
                          to_experts)
 from gpu_helpers import say
 
@@ -368,10 +368,10 @@ def test_rows_strides_offsets_and_shapes(dtype) -> None:
     turned = x.permute(2, 0, 1).contiguous().permute(1, 2, 0)
     wide = torch.stack([x, x], -1)[..., 0]
     place = order.place.permute(2, 0, 1).contiguous().permute(1, 2, 0)
-    ends = torch.stack([order.offsets, order.offsets], -1)[:, 0]
+    source = torch.stack([order.source, order.source], -1)[:, 0]
     for y in (flat[1:].view(2, 3, 40), turned, wide):
         leaf = y.detach().requires_grad_(True)
-        rows = to_experts(leaf, order._replace(place=place, offsets=ends))
+        rows = to_experts(leaf, order._replace(place=place, source=source))
         assert torch.equal(rows, want)
         g = _normal(1, 40, 12).to(dtype).t()
         (dx,) = torch.autograd.grad(rows, leaf, g)
@@ -391,31 +391,66 @@ def test_rows_strides_offsets_and_shapes(dtype) -> None:
     assert torch.autograd.grad(y.sum(), half)[0].dtype == BF16
 
 
-def test_places_that_do_not_exist_are_left_out() -> None:
-    """An order that is not expert_order's: places and offsets outside the rows move
-    nothing."""
-    order = expert_order(_choices(8, 2, 4), 4)
-    x = _normal(0, 8, 64)
-    place = order.place.clone()
-    place[2, 0], place[3, 1], place[4, 0] = 16, -5, 1 << 40
-    away = [int(order.place[2, 0]), int(order.place[3, 1]), int(order.place[4, 0])]
-    stay = [r for r in range(16) if r not in away]
-    forged = order._replace(place=place)
-    assert torch.equal(to_experts(x, forged)[stay], to_experts(x, order)[stay])
-    w = torch.rand(8, 2, generator=_gen(1), device="cuda")
-    rows = _normal(1, 16, 64).requires_grad_(True)
-    zeroed = w.clone()
-    zeroed[2, 0] = zeroed[3, 1] = zeroed[4, 0] = 0.0
-    leaf = w.clone().requires_grad_(True)
-    out = from_experts(rows, forged, leaf)
-    assert torch.equal(out, from_experts(rows, order, zeroed))
-    d_rows, d_w = torch.autograd.grad(out, (rows, leaf), _normal(2, 8, 64))
-    assert d_w[2, 0] == 0 and d_w[3, 1] == 0 and d_w[4, 0] == 0
-    for end in (-3, 1 << 40):  # none behind the last, or all
-        ends = order.offsets.clone()
-        ends[-1] = end
-        got = to_experts(x, order._replace(offsets=ends))
-        assert got.shape == (16, 64)
+def _consistent(order):
+    """The slots that are at a row, and their rows, of any order."""
+    place, source = order.place.flatten(), order.source
+    n = len(source)
+    at = torch.where((place >= 0) & (place < n), place, 0)
+    there = (place >= 0) & (place < n) & (source[at] == torch.arange(n, device="cuda"))
+    slots = there.nonzero()[:, 0]
+    return slots, place[slots]
+
+
+@TYPES
+@pytest.mark.parametrize("kind", ["dropped", "capacity", "strays", "twice", "source"])
+def test_orders_that_a_caller_has_changed(kind, dtype) -> None:
+    """Places of -1, places outside the rows, the same place twice, sources that do not
+    fit: a slot is at a row where both agree, every row that none is at is 0 and gets a
+    gradient of 0, and nothing else is read."""
+    tokens, k, count, width = 40, 3, 6, 72
+    experts = _choices(tokens, k, count)
+    order = expert_order(experts, count)
+    place, source = order.place.clone(), order.source.clone()
+    pick = torch.rand(tokens, k, generator=_gen(9), device="cuda") < 0.3
+    if kind == "dropped":
+        place[pick] = -1
+    elif kind == "capacity":
+        late = place - order.offsets[experts] >= 10
+        assert late.any()
+        place[late] = -1
+    elif kind == "strays":
+        place[pick] = torch.randint(-(1 << 40), 1 << 40, (int(pick.sum()),), generator=_gen(1), device="cuda")
+    elif kind == "twice":
+        place[pick] = 5
+    else:
+        source[::4] = torch.randint(-200, 200, (len(source[::4]),), generator=_gen(2), device="cuda")
+    order = order._replace(place=place, source=source)
+    slots, at = _consistent(order)
+    assert 0 < len(slots) < tokens * k
+    empty = torch.ones(tokens * k, dtype=torch.bool, device="cuda").index_fill(0, at, False)
+    x = _normal(0, tokens, width).to(dtype).requires_grad_(True)
+    rows = to_experts(x, order)
+    assert torch.equal(rows[at], x[slots // k]) and not rows[empty].any()
+    g = _normal(1, tokens * k, width).to(dtype)
+    g[empty] = math.nan
+    (dx,) = torch.autograd.grad(rows, x, g)
+    zero = torch.zeros(tokens, width, dtype=torch.float64, device="cuda")
+    want, size = zero.index_add(0, slots // k, g[at].double()), zero.index_add(0, slots // k, g[at].double().abs())
+    assert ((dx.double() - want).abs() <= (k + 1) * U * size + _half(dtype, want)).all()
+    rows = rows.detach().masked_fill(empty[:, None], math.nan).requires_grad_(True)
+    w = torch.rand(tokens, k, generator=_gen(3), device="cuda").requires_grad_(True)
+    out = from_experts(rows, order, w)
+    each = rows.detach()[at].double() * w.detach().flatten()[slots].double()[:, None]
+    want, size = zero.index_add(0, slots // k, each), zero.index_add(0, slots // k, each.abs())
+    assert ((out.double() - want).abs() <= (k + 1) * U * size + _half(dtype, want)).all()
+    g = _normal(4, tokens, width).to(dtype)
+    d_rows, d_w = torch.autograd.grad(out, (rows, w), g)
+    want = g[slots // k].double() * w.detach().flatten()[slots].double()[:, None]
+    assert ((d_rows[at].double() - want).abs() <= U * want.abs() + _half(dtype, want)).all() and not d_rows[empty].any()
+    each = rows.detach()[at].double() * g[slots // k].double()
+    want, size = torch.zeros(2, tokens * k, dtype=torch.float64, device="cuda")
+    want, size = want.index_copy(0, slots, each.sum(1)), size.index_copy(0, slots, each.abs().sum(1))
+    assert ((d_w.flatten().double() - want).abs() <= (width / 64 + 8) * U * size).all()
 
 
 def test_one_gradient_alone() -> None:
