@@ -42,7 +42,12 @@ int check(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_
   return ACE_OK;
 }
 
-RowsParams params(const void* in, int64_t tokens, int64_t width, int64_t top_k,
+// Whether so many rows read and written exceed the last-level cache.
+bool streams(int64_t rows, int64_t width, int dtype) {
+  return (size_t)(rows * width) * (dtype == ACE_F32 ? 4 : 2) > kStreamBytes;
+}
+
+RowsParams params(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_k,
                   const int64_t* source, const int64_t* place, const float* weights) {
   RowsParams p{};
   p.in = in;
@@ -59,14 +64,36 @@ RowsParams params(const void* in, int64_t tokens, int64_t width, int64_t top_k,
 dim3 grid_of(int64_t waves) { return dim3((unsigned)((waves + kWaves - 1) / kWaves)); }
 
 template <typename T>
+void launch_to(const RowsParams& p, bool stream, hipStream_t s) {
+  const dim3 grid = grid_of(p.tokens * p.pieces), block(kBlock);
+  if (stream)
+    hipLaunchKernelGGL((to_kernel<T, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((to_kernel<T, false>), grid, block, 0, s, p);
+}
+
+template <typename T>
+void launch_from(const RowsParams& p, bool stream, hipStream_t s) {
+  const dim3 grid = grid_of(p.tokens * p.pieces), block(kBlock);
+  if (stream)
+    hipLaunchKernelGGL((from_kernel<T, true>), grid, block, 0, s, p);
+  else
+    hipLaunchKernelGGL((from_kernel<T, false>), grid, block, 0, s, p);
+}
+
+template <typename T, bool STREAM>
 void launch_backward(const RowsParams& p, hipStream_t s) {
   const dim3 grid = grid_of(p.slots), block(kBlock);
   if (p.out && p.d_weights)
-    hipLaunchKernelGGL((from_backward_kernel<T, true, true>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((from_backward_kernel<T, true, true, STREAM>), grid, block, 0, s, p);
   else if (p.out)
-    hipLaunchKernelGGL((from_backward_kernel<T, true, false>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((from_backward_kernel<T, true, false, STREAM>), grid, block, 0, s, p);
   else
-    hipLaunchKernelGGL((from_backward_kernel<T, false, true>), grid, block, 0, s, p);
+    hipLaunchKernelGGL((from_backward_kernel<T, false, true, false>), grid, block, 0, s, p);
+}
+template <typename T>
+void launch_backward(const RowsParams& p, bool stream, hipStream_t s) {
+  stream ? launch_backward<T, true>(p, s) : launch_backward<T, false>(p, s);
 }
 
 }  // namespace
@@ -120,15 +147,15 @@ int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width, int6
   if (bad) return bad;
   if (tokens == 0) return ACE_OK;
   if (!rows) return ACE_EINVAL;
-  RowsParams p = params(x, tokens, width, top_k, source, place, nullptr);
+  RowsParams p = params(x, dtype, tokens, width, top_k, source, place, nullptr);
   p.out = rows;
   p.pieces = (int)pieces_of(width, dtype, kDeepTo);
-  const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
+  const bool past = streams(p.slots + tokens, width, dtype);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case ACE_F32: hipLaunchKernelGGL((to_kernel<float>), grid, block, 0, s, p); break;
-    case ACE_BF16: hipLaunchKernelGGL((to_kernel<__bf16>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((to_kernel<_Float16>), grid, block, 0, s, p);
+    case ACE_F32: launch_to<float>(p, past, s); break;
+    case ACE_BF16: launch_to<__bf16>(p, past, s); break;
+    default: launch_to<_Float16>(p, past, s);
   }
   return launched();
 }
@@ -140,15 +167,15 @@ int ace_from_experts(const void* rows, int dtype, int64_t tokens, int64_t width,
   if (bad) return bad;
   if (tokens == 0) return ACE_OK;
   if (!out) return ACE_EINVAL;
-  RowsParams p = params(rows, tokens, width, top_k, source, place, weights);
+  RowsParams p = params(rows, dtype, tokens, width, top_k, source, place, weights);
   p.out = out;
   p.pieces = (int)pieces_of(width, dtype, kDeepFrom);
-  const dim3 grid = grid_of(tokens * p.pieces), block(kBlock);
+  const bool past = streams(p.slots + tokens, width, dtype);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case ACE_F32: hipLaunchKernelGGL((from_kernel<float>), grid, block, 0, s, p); break;
-    case ACE_BF16: hipLaunchKernelGGL((from_kernel<__bf16>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((from_kernel<_Float16>), grid, block, 0, s, p);
+    case ACE_F32: launch_from<float>(p, past, s); break;
+    case ACE_BF16: launch_from<__bf16>(p, past, s); break;
+    default: launch_from<_Float16>(p, past, s);
   }
   return launched();
 }
@@ -162,15 +189,16 @@ int ace_from_experts_backward(const void* rows, const void* grad, int dtype, int
   if (bad) return bad;
   if (tokens == 0 || (!d_rows && !d_weights)) return ACE_OK;
   if (!grad) return ACE_EINVAL;
-  RowsParams p = params(rows, tokens, width, top_k, source, place, weights);
+  RowsParams p = params(rows, dtype, tokens, width, top_k, source, place, weights);
   p.grad = grad;
   p.out = d_rows;
   p.d_weights = d_weights;
+  const bool past = streams((d_weights ? 2 : 1) * p.slots + tokens, width, dtype);
   const hipStream_t s = static_cast<hipStream_t>(stream);
   switch (dtype) {
-    case ACE_F32: launch_backward<float>(p, s); break;
-    case ACE_BF16: launch_backward<__bf16>(p, s); break;
-    default: launch_backward<_Float16>(p, s);
+    case ACE_F32: launch_backward<float>(p, past, s); break;
+    case ACE_BF16: launch_backward<__bf16>(p, past, s); break;
+    default: launch_backward<_Float16>(p, past, s);
   }
   return launched();
 }

@@ -100,6 +100,7 @@ int launched() {
 }  // namespace ace
 
 using namespace ace::logprob;
+using ace::kStreamBytes;
 
 extern "C" {
 
@@ -174,10 +175,14 @@ int ace_logprob_backward(const void* logits, int dtype, int64_t stride, int64_t 
   p.tiles = (int)groups_of(vocab, dtype);
   const dim3 grid((unsigned)((rows * p.tiles + kBlock / 64 - 1) / (kBlock / 64))), block(kBlock);
   const hipStream_t s = static_cast<hipStream_t>(stream);
+  const bool stream_stores = (size_t)(2 * rows * vocab) * (dtype == ACE_F32 ? 4 : 2) > kStreamBytes;
+  const auto launch = [&](auto plain, auto streamed) {
+    hipLaunchKernelGGL(stream_stores ? streamed : plain, grid, block, 0, s, p);
+  };
   switch (dtype) {
-    case ACE_F32: hipLaunchKernelGGL((backward_kernel<float>), grid, block, 0, s, p); break;
-    case ACE_BF16: hipLaunchKernelGGL((backward_kernel<__bf16>), grid, block, 0, s, p); break;
-    default: hipLaunchKernelGGL((backward_kernel<_Float16>), grid, block, 0, s, p);
+    case ACE_F32: launch(backward_kernel<float, false>, backward_kernel<float, true>); break;
+    case ACE_BF16: launch(backward_kernel<__bf16, false>, backward_kernel<__bf16, true>); break;
+    default: launch(backward_kernel<_Float16, false>, backward_kernel<_Float16, true>);
   }
   return launched();
 }

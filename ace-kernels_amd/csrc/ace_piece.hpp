@@ -45,7 +45,16 @@ struct Piece {
     words = __builtin_bit_cast(Words, all);
   }
   __device__ void load(const T* at) { __builtin_memcpy(&words, at, 16); }
-  __device__ void store(T* at) const { __builtin_memcpy(at, &words, 16); }
+  // STREAM: past the caches, where what a launch reads and writes would not fit the
+  // last-level one anyway and drives out what is read.
+  template <bool STREAM>
+  __device__ void store(T* at) const {
+    typedef uint32_t Unaligned __attribute__((ext_vector_type(4), aligned(2)));
+    if constexpr (STREAM)
+      __builtin_nontemporal_store(words, reinterpret_cast<Unaligned*>(at));
+    else
+      *reinterpret_cast<Unaligned*>(at) = words;
+  }
   // The first n elements; the others are `rest`, or not stored.
   __device__ void load_some(const T* at, int64_t n, T rest) {
     typedef T All __attribute__((ext_vector_type(V)));

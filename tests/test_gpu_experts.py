@@ -356,6 +356,14 @@ def test_rows_tokens(tokens, k, count, dtype) -> None:
 
 
 @TYPES
+def test_rows_beyond_the_caches(dtype) -> None:
+    """More than 224 MB of rows, whose stores go past the caches; a row no whole number
+    of pieces."""
+    _rows_step(dtype, 45000, 1001, 2, 30, 0.1)
+    _rows_step(dtype, 45000, 1001, 2, 30, 0.1, weighted=False)
+
+
+@TYPES
 def test_rows_strides_offsets_and_shapes(dtype) -> None:
     e = _choices(6, 2, 5, 0.2).view(2, 3, 2)
     order = expert_order(e, 5)

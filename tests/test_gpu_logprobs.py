@@ -139,6 +139,14 @@ def test_rows(rows, vocab, dtype) -> None:
 
 
 @TYPES
+def test_gradients_beyond_the_caches(dtype) -> None:
+    """More than 224 MB of logits and gradients, whose stores go past the caches; rows
+    no whole number of pieces."""
+    x = _logits((1300,), 50257, dtype)
+    _compare(x, _tokens(x, ignored=0.2))
+
+
+@TYPES
 @pytest.mark.parametrize("t", [0.001, 0.05, 1.0, 30.0, 1000.0])
 def test_temperatures(t, dtype) -> None:
     x = _logits((2, 3), 5003, dtype)
