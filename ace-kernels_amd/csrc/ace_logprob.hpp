@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
   Sums sums;
   sums.clear();
   Candidates best{s_keys + (TOP ? wave * kHeld : 0), s_pieces + (TOP ? wave * kHeld : 0), 0, 0};
-  float reach = 0.f;  // what a logit has to reach to be a candidate; NaN: nothing
+  float reach = 0.f;  // pieces with a smaller maximum are no candidates; NaN: all are
   bool first = true;
   for (int64_t v = v0; v < v1; v += W * kGroup<T>) {
     Piece<T> x[kPieces];

@@ -8,8 +8,14 @@
 // As in the balance loss (ace_balance.hpp), whose choice this is: L lanes share a
 // token, each holds C of its scores in registers, and the k largest are a sorted
 // list that lanes merge by exchanges.  A 16-bit score's key holds its expert, so the
-// list is the answer; in float32 each entry's expert is looked up among the scores.
-// Normalised weights need the chosen scores only, and their gradient no score at all.
+// list is the answer; in float32 the lanes that hold the taken scores say which they
+// are.  Normalised weights need the chosen scores only, and their gradient no score.
+//
+// What bounds it: the forward of many experts its instructions (131072 x 256, top 8, in
+// float32: 55 us for 134 MB, the vector units busy throughout; 32 us in bfloat16), most
+// of them the lists; the backward memory (62 us for 268 MB, 4.3 TB/s; normalised 37 us
+// for 134).  Where a token has at least as many lanes as choices, each lane writes one of
+// them: with every lane writing its share of all, the forward took 60 us.
 #pragma once
 
 #include "ace_balance.hpp"
@@ -56,8 +62,9 @@ __device__ inline float key_score(uint32_t key) {
 }
 
 template <typename T, int C, int K>
-__global__ __launch_bounds__(kThreads, 4) void forward_kernel(Params p) {
+__global__ __launch_bounds__(kThreads, K <= 8 ? 5 : 4) void forward_kernel(Params p) {
   constexpr bool numbered = sizeof(T) == 2;
+  __shared__ int s_expert[numbered ? 1 : kThreads];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int lanes = 1 << p.lanes_log2, j = lane & (lanes - 1);
   const int E = p.experts;
@@ -77,50 +84,92 @@ __global__ __launch_bounds__(kThreads, 4) void forward_kernel(Params p) {
     bool nan = false;
 #pragma unroll
     for (int i = 0; i < C; ++i) nan |= x[i] != x[i];
-    uint32_t key[C], list[K];
-    balance::largest<T, C, K>(row, x, lanes, __ballot(nan) != 0, key, list);
-    int expert[K];
-#pragma unroll
-    for (int r = 0; r < K; ++r) {
-      expert[r] = (int)(0xffffu ^ (list[r] & 0xffffu));
-      if (!numbered && r < p.top_k) {
-        int found = balance::kMaxExperts;
-#pragma unroll
-        for (int i = C - 1; i >= 0; --i) found = key[i] == list[r] ? row.expert(i) : found;
-        const bool again = r > 0 && list[r] == list[r > 0 ? r - 1 : 0];
-        if (__ballot(again && counted)) {  // equal scores: the lowest number above the last
-          const int last = again ? expert[r > 0 ? r - 1 : 0] : -1;
-          found = balance::kMaxExperts;
-#pragma unroll
-          for (int i = C - 1; i >= 0; --i)
-            if (key[i] == list[r] && row.expert(i) > last) found = row.expert(i);
-        }
-        expert[r] = over_lanes(found, lanes, kMin);
-      }
-    }
-    const float top = key_score<T>(list[0]);
-    const bool dead = top == -INFINITY;  // every expert is closed
-    float weight[K], total = 0.f;
-#pragma unroll
-    for (int r = 0; r < K; ++r) {
-      weight[r] = r >= p.top_k || dead
-                      ? 0.f
-                      : __builtin_amdgcn_exp2f((key_score<T>(list[r]) - top) * kLog2e);
-      total += weight[r];
-    }
-    float by = 1.f / total;
+    float by = 0.f;
     if (!p.normalize) {
       float e[C];
       by = balance::exponentials<T, C>(row, x, lanes, e);
     }
-    if (dead) by = 0.f;
-    if (in) {
+    uint32_t key[C], list[K];
+    balance::largest<T, C, K>(row, x, lanes, __ballot(nan) != 0, key, list);
+    const float top = key_score<T>(list[0]);
+    const bool dead = top == -INFINITY;  // every expert is closed
+    const auto raw = [&](uint32_t k) {
+      return __builtin_amdgcn_exp2f((key_score<T>(k) - top) * kLog2e);
+    };
+    int64_t* chosen = p.chosen + mine * p.top_k;
+    float* weights = p.weights + mine * p.top_k;
+    // float32's keys have no numbers: the place of each score that is taken.  Equal
+    // scores among them, or beyond the last, are seldom, and looked for one by one.
+    bool tied = false;
+    uint32_t taken = 0;
+    if constexpr (!numbered) {
+      uint32_t least = list[0];
 #pragma unroll
-      for (int r = 0; r < K; ++r)
-        if (r < p.top_k && (r & (lanes - 1)) == j) {
-          p.chosen[mine * p.top_k + r] = counted ? expert[r] : -1;
-          p.weights[mine * p.top_k + r] = counted ? weight[r] * by : 0.f;
+      for (int r = 1; r < K; ++r) {
+        tied |= r < p.top_k && list[r] == list[r - 1];
+        least = r < p.top_k ? list[r] : least;
+      }
+#pragma unroll
+      for (int i = 0; i < C; ++i) taken |= key[i] >= least ? 1u << i : 0u;
+      if (!counted) taken = 0;
+      tied |= over_lanes(__popc(taken), lanes, kAdd) > p.top_k;
+    }
+    if (lanes >= K && !__ballot(tied && counted)) {  // lane r writes the r-th
+      uint32_t own = list[0];
+#pragma unroll
+      for (int r = 1; r < K; ++r) own = j == r ? list[r] : own;
+      int expert = (int)(0xffffu ^ (own & 0xffffu));
+      if constexpr (!numbered) {
+        int* place_of = s_expert + wave * 64 + (lane & ~(lanes - 1));
+        wave_sync();
+        while (__ballot(taken != 0)) {
+          const int at = __builtin_ctz(taken | 1u << (C - 1));
+          uint32_t k = key[0];
+          int e = row.expert(0), place = 0;
+#pragma unroll
+          for (int i = 1; i < C; ++i) {
+            k = at == i ? key[i] : k;
+            e = at == i ? row.expert(i) : e;
+          }
+#pragma unroll
+          for (int r = 0; r < K; ++r) place += list[r] > k;
+          if (taken) place_of[place] = e;
+          taken &= taken - 1;
         }
+        wave_sync();
+        expert = place_of[j];
+      }
+      float weight = j < p.top_k && !dead ? raw(own) : 0.f;
+      if (p.normalize) by = 1.f / over_lanes(weight, lanes, kAdd);
+      if (in && j < p.top_k) {
+        chosen[j] = counted ? expert : -1;
+        weights[j] = counted && !dead ? weight * by : 0.f;
+      }
+      continue;
+    }
+    float weight[K], total = 0.f;
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+      weight[r] = r < p.top_k && !dead ? raw(list[r]) : 0.f;
+      total += weight[r];
+    }
+    if (p.normalize) by = 1.f / total;
+    int last = -1;
+#pragma unroll
+    for (int r = 0; r < K; ++r) {
+      int expert = (int)(0xffffu ^ (list[r] & 0xffffu));
+      if (!numbered && r < p.top_k) {  // the lowest that no place before has
+        if (r > 0 && list[r] != list[r > 0 ? r - 1 : 0]) last = -1;
+        int next = balance::kMaxExperts;
+#pragma unroll
+        for (int i = C - 1; i >= 0; --i)
+          if (key[i] == list[r] && row.expert(i) > last) next = row.expert(i);
+        expert = last = over_lanes(next, lanes, kMin);
+      }
+      if (in && r < p.top_k && (r & (lanes - 1)) == j) {
+        chosen[r] = counted ? expert : -1;
+        weights[r] = counted && !dead ? weight[r] * by : 0.f;
+      }
     }
   }
 }

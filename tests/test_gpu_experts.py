@@ -356,6 +356,18 @@ def test_rows_tokens(tokens, k, count, dtype) -> None:
 
 
 @TYPES
+@pytest.mark.parametrize("k", [63, 64, 65, 130])
+def test_rows_of_many_choices(k, dtype) -> None:
+    """More choices than a wave has lanes, the same expert many times among them."""
+    _rows_step(dtype, 9, 200, k, 5, 0.2)
+    _rows_step(dtype, 9, 200, k, 5, 0.2, weighted=False)
+
+
+def test_a_wide_row() -> None:
+    _rows_step(BF16, 3, 1 << 20, 2, 4)
+
+
+@TYPES
 def test_rows_beyond_the_caches(dtype) -> None:
     """More than 224 MB of rows, whose stores go past the caches; a row no whole number
     of pieces."""

@@ -302,6 +302,18 @@ def test_strides_and_offsets(vocab, dtype) -> None:
                 assert torch.equal(a, b)
 
 
+def test_inference_mode_and_leading_dimensions() -> None:
+    x = _logits((2, 5), 700, BF16)
+    y = _tokens(x)
+    want = token_logprobs(x, y, LogprobConfig(top=3))
+    with torch.inference_mode():
+        got = token_logprobs(x.clone(), y, LogprobConfig(top=3))
+        flat = token_logprobs(x.view(10, 700), y.view(10), LogprobConfig(top=3))
+    for a, b, c in zip(want, got, flat):
+        assert torch.equal(a, b) and torch.equal(a.view(c.shape), c)
+    assert not want.top_logprobs.requires_grad and want.logprob.grad_fn is None
+
+
 def test_one_gradient_alone() -> None:
     x = _logits((4,), 900, F32)
     y = _tokens(x)
