@@ -23,8 +23,10 @@ struct Geometry {
 Geometry geometry(int64_t rows, int64_t vocab, int dtype) {
   const int64_t group = words_of(dtype), whole = 4 * group;
   Geometry g{4, 1, vocab};
-  // Many rows that four waves would take in one go or less: a wave each.
-  if (rows >= 2 * kTarget && vocab <= whole) {
+  // Rows that four waves would take in one go or less, and enough of them: a wave each.
+  // Forward in us with four waves and with one: 30000 x 1000 top 5 124 / 34, 8000 x 8000
+  // 48 / 37, 2000 x 8000 18 / 14; 8000 x 16000 65 / 70.
+  if (rows >= kTarget && vocab <= whole) {
     g.waves = 1;
     return g;
   }

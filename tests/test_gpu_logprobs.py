@@ -128,7 +128,7 @@ def test_sizes(vocab, dtype) -> None:
 
 # few rows are cut into parts, many are not, and many short ones share a block
 @TYPES
-@pytest.mark.parametrize("rows,vocab", [(1, 300000), (3, 40000), (130, 20000), (1100, 17000), (2500, 9001), (2047, 8000),
+@pytest.mark.parametrize("rows,vocab", [(1, 300000), (3, 40000), (130, 20000), (1100, 17000), (2500, 9001), (1023, 8000), (1024, 8000), (1024, 8193), (2047, 8000),
                                         (2048, 8000), (4099, 4000), (2500, 1000), (20001, 70), (300, 70)])
 def test_rows(rows, vocab, dtype) -> None:
     say(f"logprobs {rows} x {vocab} {dtype}")
