@@ -2,6 +2,8 @@
 // include/ace_hip.h): argument checks, launch geometry, instantiations.
 #include "ace_experts.hpp"
 
+#include <type_traits>
+
 #include "ace_hip.h"
 
 namespace ace {
@@ -58,42 +60,71 @@ RowsParams params(const void* in, int dtype, int64_t tokens, int64_t width, int6
   p.source = source;
   p.place = place;
   p.weights = weights;
+  const int vector = dtype == ACE_F32 ? kV<float> : kV<__bf16>;
+  while (p.lanes_log2 < 6 && (vector << p.lanes_log2) < width) ++p.lanes_log2;
   return p;
 }
 
 dim3 grid_of(int64_t waves) { return dim3((unsigned)((waves + kWaves - 1) / kWaves)); }
 
+// Rows of at most a piece a lane are narrow: several of them share a wave.
 template <typename T>
-void launch_to(const RowsParams& p, bool stream, hipStream_t s) {
-  const dim3 grid = grid_of(p.tokens * p.pieces), block(kBlock);
-  if (stream)
-    hipLaunchKernelGGL((to_kernel<T, true>), grid, block, 0, s, p);
-  else
-    hipLaunchKernelGGL((to_kernel<T, false>), grid, block, 0, s, p);
-}
-
-template <typename T>
-void launch_from(const RowsParams& p, bool stream, hipStream_t s) {
-  const dim3 grid = grid_of(p.tokens * p.pieces), block(kBlock);
-  if (stream)
-    hipLaunchKernelGGL((from_kernel<T, true>), grid, block, 0, s, p);
-  else
-    hipLaunchKernelGGL((from_kernel<T, false>), grid, block, 0, s, p);
+bool narrow(const RowsParams& p) {
+  return p.width <= 64 * kV<T>;
 }
 
 template <typename T, bool STREAM>
-void launch_backward(const RowsParams& p, hipStream_t s) {
-  const dim3 grid = grid_of(p.slots), block(kBlock);
-  if (p.out && p.d_weights)
-    hipLaunchKernelGGL((from_backward_kernel<T, true, true, STREAM>), grid, block, 0, s, p);
-  else if (p.out)
-    hipLaunchKernelGGL((from_backward_kernel<T, true, false, STREAM>), grid, block, 0, s, p);
-  else
-    hipLaunchKernelGGL((from_backward_kernel<T, false, true, false>), grid, block, 0, s, p);
+void launch_to(RowsParams p, hipStream_t s) {
+  const dim3 block(kBlock);
+  if (narrow<T>(p)) {
+    const int64_t waves = (p.slots + (64 >> p.lanes_log2) * kMany - 1) / ((64 >> p.lanes_log2) * kMany);
+    hipLaunchKernelGGL((to_narrow_kernel<T, STREAM>), grid_of(waves), block, 0, s, p);
+  } else {
+    hipLaunchKernelGGL((to_kernel<T, STREAM>), grid_of(p.tokens * p.pieces), block, 0, s, p);
+  }
 }
-template <typename T>
-void launch_backward(const RowsParams& p, bool stream, hipStream_t s) {
-  stream ? launch_backward<T, true>(p, s) : launch_backward<T, false>(p, s);
+
+template <typename T, bool STREAM>
+void launch_from(RowsParams p, hipStream_t s) {
+  const dim3 block(kBlock);
+  if (narrow<T>(p)) {
+    const int64_t waves = (p.tokens + (64 >> p.lanes_log2) - 1) / (64 >> p.lanes_log2);
+    hipLaunchKernelGGL((from_narrow_kernel<T, STREAM>), grid_of(waves), block, 0, s, p);
+  } else {
+    hipLaunchKernelGGL((from_kernel<T, STREAM>), grid_of(p.tokens * p.pieces), block, 0, s, p);
+  }
+}
+
+template <typename T, bool ROWS, bool WEIGHTS, bool STREAM>
+void launch_back(RowsParams p, hipStream_t s) {
+  const dim3 block(kBlock);
+  if (narrow<T>(p)) {
+    const int64_t waves = (p.slots + (64 >> p.lanes_log2) * kMany - 1) / ((64 >> p.lanes_log2) * kMany);
+    hipLaunchKernelGGL((from_backward_narrow_kernel<T, ROWS, WEIGHTS, STREAM>), grid_of(waves), block, 0,
+                       s, p);
+  } else {
+    hipLaunchKernelGGL((from_backward_kernel<T, ROWS, WEIGHTS, STREAM>), grid_of(p.slots), block, 0, s, p);
+  }
+}
+template <typename T, bool STREAM>
+void launch_back(const RowsParams& p, hipStream_t s) {
+  if (p.out && p.d_weights)
+    launch_back<T, true, true, STREAM>(p, s);
+  else if (p.out)
+    launch_back<T, true, false, STREAM>(p, s);
+  else
+    launch_back<T, false, true, false>(p, s);
+}
+
+// `launch` with the rows' type and whether stores go past the caches.
+template <typename Launch>
+int by_type(int dtype, bool past, Launch launch) {
+  switch (dtype) {
+    case ACE_F32: past ? launch(float{}, std::true_type{}) : launch(float{}, std::false_type{}); break;
+    case ACE_BF16: past ? launch(__bf16{}, std::true_type{}) : launch(__bf16{}, std::false_type{}); break;
+    default: past ? launch(_Float16{}, std::true_type{}) : launch(_Float16{}, std::false_type{});
+  }
+  return launched();
 }
 
 }  // namespace
@@ -152,12 +183,9 @@ int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width, int6
   p.pieces = (int)pieces_of(width, dtype, kDeepTo);
   const bool past = streams(p.slots + tokens, width, dtype);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case ACE_F32: launch_to<float>(p, past, s); break;
-    case ACE_BF16: launch_to<__bf16>(p, past, s); break;
-    default: launch_to<_Float16>(p, past, s);
-  }
-  return launched();
+  return by_type(dtype, past, [&](auto t, auto past_caches) {
+    launch_to<decltype(t), decltype(past_caches)::value>(p, s);
+  });
 }
 
 int ace_from_experts(const void* rows, int dtype, int64_t tokens, int64_t width, int64_t top_k,
@@ -172,12 +200,9 @@ int ace_from_experts(const void* rows, int dtype, int64_t tokens, int64_t width,
   p.pieces = (int)pieces_of(width, dtype, kDeepFrom);
   const bool past = streams(p.slots + tokens, width, dtype);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case ACE_F32: launch_from<float>(p, past, s); break;
-    case ACE_BF16: launch_from<__bf16>(p, past, s); break;
-    default: launch_from<_Float16>(p, past, s);
-  }
-  return launched();
+  return by_type(dtype, past, [&](auto t, auto past_caches) {
+    launch_from<decltype(t), decltype(past_caches)::value>(p, s);
+  });
 }
 
 int ace_from_experts_backward(const void* rows, const void* grad, int dtype, int64_t tokens,
@@ -195,12 +220,9 @@ int ace_from_experts_backward(const void* rows, const void* grad, int dtype, int
   p.d_weights = d_weights;
   const bool past = streams((d_weights ? 2 : 1) * p.slots + tokens, width, dtype);
   const hipStream_t s = static_cast<hipStream_t>(stream);
-  switch (dtype) {
-    case ACE_F32: launch_backward<float>(p, past, s); break;
-    case ACE_BF16: launch_backward<__bf16>(p, past, s); break;
-    default: launch_backward<_Float16>(p, past, s);
-  }
-  return launched();
+  return by_type(dtype, past, [&](auto t, auto past_caches) {
+    launch_back<decltype(t), decltype(past_caches)::value>(p, s);
+  });
 }
 
 }  // extern "C"
