@@ -20,9 +20,14 @@ int launched() {
 }
 
 int64_t order_blocks(int64_t slots, int64_t* per_block) {
-  // a slot a thread; more from kMaxBlocks on
-  const int64_t each = slots > kOrderBlock * kMaxBlocks ? (slots + kMaxBlocks - 1) / kMaxBlocks : 1;
+  // A slot a thread, more where that would be too many blocks.  One block alone needs one
+  // launch instead of two: up to eight slots a thread (8000 slots 9.5 us instead of 10.4, 2000
+  // 7.3 instead of 10.2; 16000 17 instead of 10).
+  int64_t each = 1;
+  if (slots <= 8 * kOrderBlock) each = slots;
+  if (slots > kOrderBlock * kMaxBlocks) each = (slots + kMaxBlocks - 1) / kMaxBlocks;
   *per_block = (each + kOrderBlock - 1) / kOrderBlock * kOrderBlock;
+  if (*per_block < 1) *per_block = kOrderBlock;
   const int64_t blocks = (slots + *per_block - 1) / *per_block;
   return blocks < 1 ? 1 : blocks;
 }

@@ -255,7 +255,7 @@ def _choices(tokens, k, count, share=0.0, seed=0):
 
 @pytest.mark.parametrize("count", [1, 2, 3, 8, 64, 100, 511, 512])
 @pytest.mark.parametrize("tokens,k", [(0, 2), (1, 1), (1, 7), (31, 2), (33, 2), (64, 1), (257, 4), (2047, 2), (2048, 2),
-                                      (2049, 2), (5000, 3), (70001, 2)])
+                                      (2049, 2), (4096, 2), (4097, 2), (5000, 3), (70001, 2)])
 def test_order(tokens, k, count) -> None:
     for share in (0.0, 0.3, 1.0):
         e = _choices(tokens, k, count, share)
