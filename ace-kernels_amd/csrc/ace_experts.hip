@@ -12,7 +12,8 @@ namespace {
 
 constexpr int64_t kMaxSlots = (int64_t)1 << 30;
 constexpr int64_t kMaxWidth = (int64_t)1 << 20;
-constexpr int64_t kMaxWaves = (int64_t)1 << 26;  // a launch has fewer than 2^32 threads
+// A launch has fewer than 2^32 threads, in whole blocks.
+constexpr int64_t kMaxWaves = ((int64_t)1 << 26) - kWaves;
 
 int launched() {
   const hipError_t e = hipGetLastError();
@@ -44,7 +45,7 @@ int check(const void* in, int dtype, int64_t tokens, int64_t width, int64_t top_
   if (tokens > 0 && (!in || !source || !place)) return ACE_EINVAL;
   if (width > kMaxWidth || top_k > kMaxSlots || tokens > kMaxSlots || tokens * top_k > kMaxSlots)
     return ACE_EUNSUPPORTED;
-  if (tokens * pieces_of(width, dtype, kDeepFrom) >= kMaxWaves || tokens * top_k >= kMaxWaves)
+  if (tokens * pieces_of(width, dtype, kDeepFrom) > kMaxWaves || tokens * top_k > kMaxWaves)
     return ACE_EUNSUPPORTED;
   return ACE_OK;
 }
@@ -72,6 +73,12 @@ RowsParams params(const void* in, int dtype, int64_t tokens, int64_t width, int6
 
 dim3 grid_of(int64_t waves) { return dim3((unsigned)((waves + kWaves - 1) / kWaves)); }
 
+// Waves of narrow rows that take `each` of n units a lane.
+int64_t narrow_waves(const RowsParams& p, int64_t n, int each) {
+  const int64_t units = (int64_t)(64 >> p.lanes_log2) * each;
+  return (n + units - 1) / units;
+}
+
 // Rows of at most a piece a lane are narrow: several of them share a wave.
 template <typename T>
 bool narrow(const RowsParams& p) {
@@ -82,7 +89,7 @@ template <typename T, bool STREAM>
 void launch_to(RowsParams p, hipStream_t s) {
   const dim3 block(kBlock);
   if (narrow<T>(p)) {
-    const int64_t waves = (p.slots + (64 >> p.lanes_log2) * kMany - 1) / ((64 >> p.lanes_log2) * kMany);
+    const int64_t waves = narrow_waves(p, p.slots, kMany);
     hipLaunchKernelGGL((to_narrow_kernel<T, STREAM>), grid_of(waves), block, 0, s, p);
   } else {
     hipLaunchKernelGGL((to_kernel<T, STREAM>), grid_of(p.tokens * p.pieces), block, 0, s, p);
@@ -93,7 +100,7 @@ template <typename T, bool STREAM>
 void launch_from(RowsParams p, hipStream_t s) {
   const dim3 block(kBlock);
   if (narrow<T>(p)) {
-    const int64_t waves = (p.tokens + (64 >> p.lanes_log2) - 1) / (64 >> p.lanes_log2);
+    const int64_t waves = narrow_waves(p, p.tokens, 1);
     hipLaunchKernelGGL((from_narrow_kernel<T, STREAM>), grid_of(waves), block, 0, s, p);
   } else {
     hipLaunchKernelGGL((from_kernel<T, STREAM>), grid_of(p.tokens * p.pieces), block, 0, s, p);
@@ -104,7 +111,7 @@ template <typename T, bool ROWS, bool WEIGHTS, bool STREAM>
 void launch_back(RowsParams p, hipStream_t s) {
   const dim3 block(kBlock);
   if (narrow<T>(p)) {
-    const int64_t waves = (p.slots + (64 >> p.lanes_log2) * kMany - 1) / ((64 >> p.lanes_log2) * kMany);
+    const int64_t waves = narrow_waves(p, p.slots, kMany);
     hipLaunchKernelGGL((from_backward_narrow_kernel<T, ROWS, WEIGHTS, STREAM>), grid_of(waves), block, 0,
                        s, p);
   } else {

@@ -10,7 +10,8 @@ namespace {
 
 constexpr int64_t kMaxSize = (int64_t)1 << 30;
 constexpr int64_t kMaxRows = (int64_t)1 << 24;   // a launch has less than 2^32 threads
-constexpr int64_t kMaxGroups = (int64_t)1 << 26;
+// A wave each, and whole blocks of four of them: below 2^32 threads too.
+constexpr int64_t kMaxGroups = ((int64_t)1 << 26) - kBlock / 64;
 constexpr int64_t kTarget = 1024;  // blocks to aim at: four on each CU
 
 int words_of(int dtype) { return dtype == ACE_F32 ? kGroup<float> : kGroup<__bf16>; }
@@ -49,7 +50,7 @@ int64_t groups_of(int64_t vocab, int dtype) {
   return (vocab + words_of(dtype) - 1) / words_of(dtype);
 }
 bool fits(int64_t rows, int64_t vocab, int dtype) {
-  return rows < kMaxRows && vocab <= kMaxSize && rows * groups_of(vocab, dtype) < kMaxGroups;
+  return rows < kMaxRows && vocab <= kMaxSize && rows * groups_of(vocab, dtype) <= kMaxGroups;
 }
 bool sizes(int64_t rows, int64_t vocab, int dtype) {
   return (dtype == ACE_F32 || dtype == ACE_BF16 || dtype == ACE_F16) && rows >= 0 && vocab >= 1 &&

@@ -368,7 +368,7 @@ int ace_balance_backward(const void* logits, int dtype, const uint8_t* mask,
  * Both calls are one launch on `stream`, allocate nothing and can be captured; results
  * do not vary from run to run.  Returns ACE_EINVAL (temperature outside [1e-3, 1e3]
  * among others), ACE_EUNSUPPORTED (top above 32, vocab above 2^30, 2^24 rows or more,
- * 2^26 pieces of 4096 bytes of rows or more), ACE_EWORKSPACE or a HIP error.
+ * more than 2^26 - 4 pieces of 4096 bytes of rows), ACE_EWORKSPACE or a HIP error.
  */
 size_t ace_logprob_saved_bytes(int64_t rows);
 size_t ace_logprob_workspace_bytes(int dtype, int64_t rows, int64_t vocab,
@@ -447,8 +447,8 @@ int ace_expert_order(const int64_t* chosen, int64_t slots, int64_t experts,
  * d_weights (0 without a row), either skipped if NULL; `rows` may be NULL without
  * d_weights.
  * One launch each on `stream`, no allocation, can be captured; results do not vary
- * from run to run.  Returns ACE_EINVAL, ACE_EUNSUPPORTED (width above 2^20, 2^26 slots or
- * pieces of 2048 bytes of tokens or more) or a HIP error.
+ * from run to run.  Returns ACE_EINVAL, ACE_EUNSUPPORTED (width above 2^20, more than
+ * 2^26 - 4 slots or pieces of 2048 bytes of tokens) or a HIP error.
  */
 int ace_to_experts(const void* x, int dtype, int64_t tokens, int64_t width,
                    int64_t top_k, const int64_t* source, const int64_t* place,

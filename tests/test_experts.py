@@ -169,6 +169,13 @@ def test_rows_refuse_before_launch(changed) -> None:
         assert call(**changed) == _lib.EINVAL
 
 
+def test_last_block_stays_below_the_grid_limit() -> None:
+    # four waves a block: 2^26 - 1 of them would round up to 2^32 threads
+    for call in (_to, _from, _from_back):
+        assert call(tokens=(1 << 26) - 1, top_k=1, width=1024) == _lib.EUNSUPPORTED
+        assert call(tokens=(1 << 26) - 3, top_k=1, width=1024) == _lib.EUNSUPPORTED
+
+
 def test_rows_limits() -> None:
     assert _to(rows=None) == _lib.EINVAL and _from(out=None) == _lib.EINVAL
     assert _from_back(grad=None) == _lib.EINVAL

@@ -89,6 +89,13 @@ def test_backward_refuses_before_launch(changed) -> None:
     assert _backward(**changed) == _lib.EINVAL
 
 
+def test_last_block_stays_below_the_grid_limit() -> None:
+    # four groups a block: 2^26 - 1 of them would round up to 2^32 threads
+    call = dict(rows=8191, vocab=8193 * 2048, stride=8193 * 2048)
+    assert call["rows"] * 8193 == (1 << 26) - 1
+    assert _forward(**call) == _lib.EUNSUPPORTED and _backward(**call) == _lib.EUNSUPPORTED
+
+
 def test_limits_and_workspace() -> None:
     lib = _lib.lib()
     for call in (_forward, _backward):
