@@ -21,7 +21,7 @@
 // each piece before a word's own has a word before it.  The maxima are there anyway, so
 // pieces are what is looked for.  The k-th largest of the lanes' maxima over the
 // team's first words bounds the k-th largest from below; pieces that reach it are
-// kept as candidates, in LDS, a few dozen in a usual row.  At the end every
+// kept as candidates, in LDS.  At the end every
 // candidate counts those above it, which is its place; then the same for the words
 // of the k best.  A wave whose candidates outgrow its LDS (logits in ascending
 // order, say) keeps its k best and raises the bound.

@@ -12,10 +12,10 @@
 // are.  Normalised weights need the chosen scores only, and their gradient no score.
 //
 // What bounds it: the forward of many experts its instructions (131072 x 256, top 8, in
-// float32: 55 us for 134 MB, the vector units busy throughout; 32 us in bfloat16), most
-// of them the lists; the backward memory (62 us for 268 MB, 4.3 TB/s; normalised 37 us
+// float32: 58 us for 134 MB, the vector units busy throughout; 32 us in bfloat16), most
+// of them the lists; the backward memory (63 us for 268 MB, 4.2 TB/s; normalised 37 us
 // for 134).  Where a token has at least as many lanes as choices, each lane writes one of
-// them: with every lane writing its share of all, the forward took 60 us.
+// them: with every lane writing its share of all, the forward took 65 us.
 #pragma once
 
 #include "ace_balance.hpp"
