@@ -12,8 +12,13 @@
 // Forward: a team of one wave (short rows) or four reads a row, or a part of one
 // where there are few rows.  Each lane keeps a running maximum, sum of exp z and sum
 // of z exp z; these are joined across lanes, waves and, through the workspace, the
-// row's parts, by the part that ends last.  Sums are float32 over at most V / 64
-// words a lane.
+// row's parts, by the part that ends last.  The largest word's e^0 is in the sum, and
+// where it is most of it (a word that is all but certain) l is what the others add to that
+// 1.  So groups, lanes and parts are added in float64, and where a wave's sum is below 2,
+// so that one word has its 1 alone, the words that its lane had added to it in float32 are
+// read once more, by a lane each, and added up without it.  (With float32 throughout, what
+// words below 2^-25 of the largest add was lost in its lane: log probabilities near 0 of a
+// row of 131072 were off by 6e-6 of themselves, now 2e-7.)
 //
 // Alternatives: a key is a logit's bits in their order above the complement of its
 // number, so keys differ and equal logits rank by number, lowest first.  The k
@@ -89,19 +94,25 @@ struct Params {
 __device__ inline float max_of(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 __device__ inline float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+__device__ inline float exponent(float x, float top, float scale) {
+  return fmaxf((x - top) * scale, -kFar);
+}
+
 // Running maximum of x, sum of e = 2^((x - top) scale), sum of e (x - top) scale.
 struct Sums {
-  float top, sum, pull;
+  double sum;
+  float top, pull;
 
   __device__ void clear() {
     top = -FLT_MAX;  // not -inf: e of a logit of -inf is then 0
-    sum = pull = 0.f;
+    sum = 0.0;
+    pull = 0.f;
   }
   // moved to another, larger maximum
   __device__ void raise(float to, float scale) {
     const float d = fminf((to - top) * scale, kFar), f = exp2_of(-d);
-    pull = f * (pull - d * sum);
-    sum *= f;
+    pull = f * (pull - d * (float)sum);
+    sum *= (double)f;
     top = to;
   }
   __device__ void over_wave(float scale);
@@ -115,7 +126,8 @@ __device__ inline float over_lanes(float x, Op op) {
 }
 __device__ inline void Sums::over_wave(float scale) {
   raise(over_lanes(top, [](float a, float b) { return max_of(a, b); }), scale);
-  sum = over_lanes(sum, balance::kAdd);
+#pragma unroll
+  for (int d = 1; d < 64; d *= 2) sum += __shfl_xor(sum, d);
   pull = over_lanes(pull, balance::kAdd);
 }
 
@@ -268,6 +280,8 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
   Sums sums;
   sums.clear();
   Candidates best{s_keys + (TOP ? wave * kHeld : 0), s_pieces + (TOP ? wave * kHeld : 0), 0, 0};
+  int highest = 0;      // the group of the lane's largest word, from v0
+  float beside = 0.f;   // what the lane added there
   float reach = 0.f;  // pieces with a smaller maximum are no candidates; NaN: all are
   bool first = true;
   for (int64_t v = v0; v < v1; v += W * kGroup<T>) {
@@ -286,19 +300,23 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
       // four waves fit a SIMD instead of seven (4096 x 32000, top 20: 68 us instead of 61)
       if constexpr (TOP) asm volatile("" : "+v"(x[u].words));
     }
+    const bool raised = t > sums.top;
     sums.raise(max_of(sums.top, t), p.scale);
     float sum = 0.f, pull = 0.f;
 #pragma unroll
     for (int u = 0; u < kPieces; ++u)
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float z = fmaxf((x[u][e] - sums.top) * p.scale, -kFar);
-        const float ex = exp2_of(z);
+        const float z = exponent(x[u][e], sums.top, p.scale), ex = exp2_of(z);
         sum += ex;
         pull = fmaf(ex, z, pull);
       }
-    sums.sum += sum;
+    sums.sum += (double)sum;
     sums.pull += pull;
+    if (raised) {
+      highest = (int)(v - v0);
+      beside = sum;
+    }
     if constexpr (TOP) {
       if (first) {
         const uint32_t order = order_of(t);
@@ -331,7 +349,22 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
     }
     first = false;
   }
+  const float own = sums.top;
   sums.over_wave(p.scale);
+  if (sums.sum >= 1.0 && sums.sum < 2.0) {  // one word's 1, and less than 1 of all others
+    static_assert(kPieces * V <= 64, "the holder's words have a lane each");
+    const int holder = __builtin_ctzll(__ballot(own == sums.top));
+    const int64_t at = v0 + __builtin_amdgcn_readlane(highest, holder) + mate * kGroup<T> +
+                       lane / V * kTile<T> + holder * V + lane % V;
+    float rest = 0.f;
+    if (lane < kPieces * V && at < v1) {
+      const float ex = exp2_of(exponent((float)logits[at], sums.top, p.scale));
+      rest = ex == 1.f ? 0.f : ex;
+    }
+    rest = over_lanes(rest, balance::kAdd);
+    const float added = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(beside), holder));
+    sums.sum += 1.0 + (double)rest - (double)added;
+  }
   if constexpr (W > 1) {
     if (lane == 0) s_sums[mate] = sums;
   }
@@ -343,7 +376,8 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
     float t = s_sums[0].top;
 #pragma unroll
     for (int i = 1; i < W; ++i) t = max_of(t, s_sums[i].top);
-    sums.sum = sums.pull = 0.f;
+    sums.sum = 0.0;
+    sums.pull = 0.f;
     sums.top = t;
 #pragma unroll
     for (int i = 0; i < W; ++i) {
@@ -401,9 +435,9 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
       unsigned long long* all = p.part + row * p.parts * (2 + p.top);
       unsigned long long* own = all + part * (2 + p.top);
       if (thread == 0) {
-        ace::store_dev(own, (unsigned long long)__float_as_uint(sums.top) << 32 |
-                                __float_as_uint(sums.sum));
-        ace::store_dev(own + 1, (unsigned long long)__float_as_uint(sums.pull));
+        ace::store_dev(own, (unsigned long long)__double_as_longlong(sums.sum));
+        ace::store_dev(own + 1, (unsigned long long)__float_as_uint(sums.top) << 32 |
+                                    __float_as_uint(sums.pull));
       }
       if constexpr (TOP) {
         int held = 0;
@@ -422,7 +456,7 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
       const uint64_t key = TOP ? ace::load_dev(at + 1 + d) : 0ull;
       sums.clear();
       if (lane < p.parts)
-        sums = Sums{__uint_as_float((uint32_t)(a >> 32)), __uint_as_float((uint32_t)a),
+        sums = Sums{__longlong_as_double((long long)a), __uint_as_float((uint32_t)(b >> 32)),
                     __uint_as_float((uint32_t)b)};
       if constexpr (TOP) {
         const int m = (p.top + d - 1) / d, n = p.parts * p.top;
@@ -449,13 +483,15 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
   }
 
   const bool defined = sums.top < INFINITY;  // not NaN, not +inf
-  const bool dead = sums.sum == 0.f;         // every logit is -inf
-  const float log_sum = logf(sums.sum);
+  const bool dead = sums.sum == 0.0;         // every logit is -inf
+  // log(hi + lo) = log hi + lo / hi, lo being less than a step of hi
+  const float hi = (float)sums.sum, lo = (float)(sums.sum - (double)hi);
+  const float log_sum = logf(hi) + lo * __builtin_amdgcn_rcpf(hi);
   const auto logprob_of = [&](float x) {
     return !defined ? NAN : dead ? -INFINITY : (x - sums.top) * p.inv_t - log_sum;
   };
   if (thread == 0) {
-    const float entropy = !defined ? NAN : dead ? 0.f : log_sum - kLn2 * (sums.pull / sums.sum);
+    const float entropy = !defined ? NAN : dead ? 0.f : log_sum - kLn2 * (sums.pull / (float)sums.sum);
     p.logprob[row] = logprob_of(x_y);
     p.entropy[row] = entropy;
     p.saved[row] = Saved{defined ? sums.top : NAN, log_sum, entropy, dead && defined ? -1 : (int)y};

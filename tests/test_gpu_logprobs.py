@@ -278,6 +278,24 @@ def test_many_nans(dtype) -> None:
 
 
 @TYPES
+@pytest.mark.parametrize("rows,vocab", [(1024, 4096), (1, 1 << 20), (1024, 65536)])
+def test_words_that_are_all_but_certain(rows, vocab, dtype) -> None:
+    """The others' sum s is what the log probability of the largest word consists of, and
+    each of them is far below a step of 1.  s is off by (3 |z| + 2) u s from its exponentials
+    and by at most 32 u s, u for each word that a lane adds of a group; it meets the 1, and
+    other lanes and waves, in float64; the logarithm adds 4 u of the result."""
+    x = torch.full((rows, vocab), -18.0, dtype=dtype, device="cuda")  # each e^-18 = 2^-25.97
+    y = (torch.arange(rows, device="cuda") * 7919 + vocab // 2) % vocab
+    x[torch.arange(rows, device="cuda"), y] = 0.0
+    out = token_logprobs(x, y, LogprobConfig(top=1))
+    s = (vocab - 1) * math.exp(-18.0)
+    tol = (3 * 18 / math.log(2.0) + 2 + 32) * U * s + 4 * U * math.log1p(s)
+    for got in (out.logprob, out.top_logprobs[:, 0]):
+        assert float((got.double() + math.log1p(s)).abs().max()) <= tol
+    assert torch.equal(out.top_tokens[:, 0], y)
+
+
+@TYPES
 @pytest.mark.parametrize("vocab", [501, 504, 9000])
 def test_strides_and_offsets(vocab, dtype) -> None:
     """Rows that lie apart are read where they are; any other order is copied."""
