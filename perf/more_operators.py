@@ -14,7 +14,6 @@ from __future__ import annotations
 
 import math
 import sys
-from functools import lru_cache
 from pathlib import Path
 
 import torch
@@ -213,7 +212,6 @@ def run(state):
 # ------------------------------------------------------------ the package's
 
 
-@lru_cache(maxsize=1)  # a program imports it once, not on every call
 def _package():
     path = str(Path(__file__).resolve().parent.parent / "ace-kernels_amd")
     if path not in sys.path:
