@@ -351,7 +351,9 @@ __global__ __launch_bounds__(kBlock) void forward_kernel(Params p) {
   }
   const float own = sums.top;
   sums.over_wave(p.scale);
-  if (sums.sum >= 1.0 && sums.sum < 2.0) {  // one word's 1, and less than 1 of all others
+  // one word's 1, and less than 1 of all others; at -FLT_MAX all others are -inf, and
+  // lanes that have no word have that maximum too
+  if (sums.sum >= 1.0 && sums.sum < 2.0 && sums.top > -FLT_MAX) {
     static_assert(kPieces * V <= 64, "the holder's words have a lane each");
     const int holder = __builtin_ctzll(__ballot(own == sums.top));
     const int64_t at = v0 + __builtin_amdgcn_readlane(highest, holder) + mate * kGroup<T> +

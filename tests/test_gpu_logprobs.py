@@ -296,6 +296,25 @@ def test_words_that_are_all_but_certain(rows, vocab, dtype) -> None:
 
 
 @TYPES
+@pytest.mark.parametrize("rows", [1, 5, 1100])
+@pytest.mark.parametrize("vocab", [1, 2, 257, 1025, 2049, 4097, 40001])
+def test_rows_whose_largest_word_is_the_lowest_value(vocab, rows, dtype) -> None:
+    """A type's lowest value is a word like any other where nothing else is open: all of a
+    row at it, of which some sizes leave a wave one word, and one such word alone, in any lane."""
+    low = torch.finfo(dtype).min
+    x = torch.full((rows, vocab), low, dtype=dtype, device="cuda")
+    y = (torch.arange(rows, device="cuda") * 7919 + vocab // 2) % vocab
+    top = min(vocab, 5)
+    out, _ = _compare(x, y, top)
+    assert torch.equal(out.top_tokens, torch.arange(top, device="cuda").expand(rows, top))
+    x = torch.full((rows, vocab), -math.inf, dtype=dtype, device="cuda")
+    x[torch.arange(rows, device="cuda"), y] = low
+    out, grad = _compare(x, y, top)
+    assert not out.logprob.any() and not out.entropy.any() and not grad.any()
+    assert torch.equal(out.top_tokens[:, 0], y) and not out.top_logprobs[:, 0].any()
+
+
+@TYPES
 @pytest.mark.parametrize("vocab", [501, 504, 9000])
 def test_strides_and_offsets(vocab, dtype) -> None:
     """Rows that lie apart are read where they are; any other order is copied."""
