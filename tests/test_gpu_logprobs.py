@@ -296,6 +296,39 @@ def test_words_that_are_all_but_certain(rows, vocab, dtype) -> None:
 
 
 @TYPES
+@pytest.mark.parametrize("t", [1.0, 0.5])
+@pytest.mark.parametrize("rows,vocab,low", [(1024, 4096, -18.0), (1, 1 << 20, -18.0), (64, 32000, -26.0), (1300, 50257, -30.0),
+                                            (5, 2, -9.0)])
+def test_gradients_of_words_that_are_all_but_certain(rows, vocab, low, t, dtype) -> None:
+    """g (1 - p) of the given word is what the others' p g add up to, s / (1 + s) of g, also
+    where p rounds to 1.  The log probability is off relatively by the bound above over s,
+    expm1 and the product by 4 u, an other word's p by (3 |z| + 6) u and what the sum is off; the
+    entropy's term p (lp + H) = p |z| s / (1 + s) by twice that, lp and H each being small.  s
+    meets the 1 in float64, in at most 16 steps across lanes, waves and parts."""
+    z = low / t
+    x = torch.full((rows, vocab), low, dtype=dtype, device="cuda")
+    y = (torch.arange(rows, device="cuda") * 7919 + vocab // 2) % vocab
+    here = torch.arange(rows, device="cuda")
+    x[here, y] = 0.0
+    s = (vocab - 1) * math.exp(z)
+    rel = (3 * abs(z) / math.log(2.0) + 2 + 32 + 8) * U
+    half = torch.finfo(dtype).eps / 2
+    tiny = torch.finfo(dtype).tiny * half * 1.01 + 2.0 ** -125 + 3.0 / t * 16 * 2.0 ** -53
+    g = torch.full((rows,), 3.0, device="cuda")
+    for ups in ([g, torch.zeros_like(g)], [torch.zeros_like(g), g]):
+        leaf = x.detach().requires_grad_(True)
+        out = token_logprobs(leaf, y, LogprobConfig(temperature=t))
+        (grad,) = torch.autograd.grad((out.logprob, out.entropy), leaf, ups)
+        p, q = 1 / (1 + s), math.exp(z) / (1 + s)  # the given word's and each other's
+        lp, lq = -math.log1p(s), z - math.log1p(s)
+        h = math.log1p(s) - (vocab - 1) * q * z
+        want = (3.0 * s * p / t, -3.0 * q / t) if ups[0] is g else (-3.0 * p * (lp + h) / t, -3.0 * q * (lq + h) / t)
+        for got, value in ((grad[here, y], want[0]), (grad[here, (y + 1) % vocab], want[1])):
+            err = float((got.double() - value).abs().max())
+            assert err <= (3 * rel + half) * abs(value) + tiny, f"{err / abs(value):.3g} of {value:.3g}"
+
+
+@TYPES
 @pytest.mark.parametrize("rows", [1, 5, 1100])
 @pytest.mark.parametrize("vocab", [1, 2, 257, 1025, 2049, 4097, 40001])
 def test_rows_whose_largest_word_is_the_lowest_value(vocab, rows, dtype) -> None:
