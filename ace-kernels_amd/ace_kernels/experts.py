@@ -104,7 +104,8 @@ def _check_route(logits: torch.Tensor, config: RouteConfig, mask: Optional[torch
 def route_tokens(logits: torch.Tensor, config: RouteConfig, mask: Optional[torch.Tensor] = None) -> Routes:
     """The ``top_k`` experts of each token and their weights, from router scores ``[...,
     E]`` (float32, bfloat16 or float16).  ``mask`` ``[...]`` (bool): tokens that are
-    routed.  Differentiable once in ``logits``, through ``weights``."""
+    routed.  Differentiable once in ``logits``, through ``weights``; for that the scores
+    are kept, as they were, only with ``normalize=False``."""
     _check_route(logits, config, mask)
     return Routes(*_lib.autograd().route_tokens(logits, mask, config.top_k, config.normalize))
 

@@ -321,13 +321,17 @@ at::Tensor float32(const at::Tensor& g) {
 
 // Gradients of a backward that is itself recorded (create_graph) refuse to be
 // differentiated again, rather than pass as constants.
-void refuse_second_derivative(variable_list& out, const variable_list& inputs, const char* what) {
+void refuse_second_derivative(variable_list& out, torch::autograd::edge_list inputs,
+                              const char* what) {
   if (!at::GradMode::is_enabled()) return;
   auto node = std::make_shared<torch::autograd::Error>(
-      std::string(what) + " can be differentiated only once",
-      torch::autograd::collect_next_edges(inputs));
+      std::string(what) + " can be differentiated only once", std::move(inputs));
   for (at::Tensor& t : out)
     if (t.defined()) torch::autograd::set_history(t, node);
+}
+void refuse_second_derivative(variable_list& out, const variable_list& inputs, const char* what) {
+  if (!at::GradMode::is_enabled()) return;
+  refuse_second_derivative(out, torch::autograd::collect_next_edges(inputs), what);
 }
 
 // The nodes know no forward-mode derivative: a tensor that carries a tangent is
@@ -647,17 +651,19 @@ struct RouteTokensBackward : public Node {
                      weights = weights_.unpack();
     {
       const at::NoGradGuard no_grad;
-      const c10::DeviceGuard guard(logits.device());
-      // normalised weights' gradient reads no score
-      const at::Tensor x = normalize ? logits : plain(logits), g = float32(grads[0]);
-      out[0] = at::empty(logits.sizes(), logits.options().requires_grad(false));
+      const c10::DeviceGuard guard(chosen.device());
+      const at::Tensor g = float32(grads[0]);
+      out[0] = at::empty(sizes, options);
+      // without kept scores any address will do
+      const at::Tensor x = logits.defined() ? plain(logits) : out[0];
       const int rc = g_route_backward.load()(
-          x.data_ptr(), dtype_code(logits), tokens, logits.size(-1), top_k, normalize,
+          x.data_ptr(), dtype_code(out[0]), tokens, sizes.back(), top_k, normalize,
           chosen.data_ptr<int64_t>(), weights.data_ptr<float>(), g.data_ptr<float>(),
-          out[0].data_ptr(), current_stream(logits));
+          out[0].data_ptr(), current_stream(out[0]));
       if (rc) fail(rc, "ace_route_backward");
     }
-    refuse_second_derivative(out, {logits, grads[0]}, "route_tokens");
+    refuse_second_derivative(out, {next_edge(0), torch::autograd::impl::gradient_edge(grads[0])},
+                             "route_tokens");
     return out;
   }
 
@@ -669,6 +675,8 @@ struct RouteTokensBackward : public Node {
 
   int64_t tokens = 0;
   int top_k = 0, normalize = 0;
+  std::vector<int64_t> sizes;
+  at::TensorOptions options;
   SavedVariable logits_, chosen_, weights_;
 };
 
@@ -705,7 +713,10 @@ std::vector<at::Tensor> route_tokens(const at::Tensor& logits, const std::option
     node->tokens = tokens;
     node->top_k = top_k;
     node->normalize = normalize;
-    node->logits_ = SavedVariable(logits, false);
+    node->sizes.assign(logits.sizes().begin(), logits.sizes().end());
+    node->options = logits.options().requires_grad(false);
+    // the gradient of normalised weights reads no score
+    if (!normalize) node->logits_ = SavedVariable(logits, false);
     node->chosen_ = SavedVariable(chosen, false);
     // not the result itself, which will hold the node; it shares the version that
     // tells of changes in place

@@ -397,7 +397,8 @@ int ace_logprob_backward(const void* logits, int dtype, int64_t stride,
  * token has -1 and 0, and its logits are not read.  An expert at -inf has weight 0,
  * also where all of a token's are.
  * ace_route_backward: the gradient of logits for an upstream gradient of weights, from
- * the forward's chosen and weights; the choice is a constant.
+ * the forward's chosen and weights; the choice is a constant.  With `normalize` the
+ * logits are not read (any address but NULL).
  * Both calls are one launch on `stream`, allocate nothing and can be captured.
  * Returns ACE_EINVAL, ACE_EUNSUPPORTED (experts above 512, top_k above 16, tokens above
  * 2^30) or a HIP error.

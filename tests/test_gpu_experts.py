@@ -230,6 +230,40 @@ def test_route_keeps_nothing_alive() -> None:
     assert torch.cuda.memory_allocated() == before
 
 
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_keeps_scores_only_where_they_are_read(normalize) -> None:
+    """Normalised weights' gradient needs the weights alone: the scores' memory is free,
+    and they may be changed, before the backward."""
+    leaf = _scores((4000,), 256, F32).requires_grad_(True)
+    cfg, up = RouteConfig(top_k=8, normalize=normalize), _normal(7, 4000, 8)
+    (want,) = torch.autograd.grad(route_tokens(leaf, cfg).weights, leaf, up)
+    scores = leaf * 1.0
+    out = route_tokens(scores, cfg)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    del scores
+    assert before - torch.cuda.memory_allocated() == (4000 * 256 * 4 if normalize else 0)
+    assert torch.equal(torch.autograd.grad(out.weights, leaf, up)[0], want)
+    scores = leaf * 1.0
+    out = route_tokens(scores, cfg)
+    scores.fill_(-math.inf)
+    if normalize:
+        assert torch.equal(torch.autograd.grad(out.weights, leaf, up)[0], want)
+    else:
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(out.weights, leaf, up)
+
+
+@pytest.mark.parametrize("normalize", [True, False])
+def test_route_has_no_second_derivative_in_the_scores(normalize) -> None:
+    leaf = _scores((20,), 8, F32).requires_grad_(True)
+    for scores in (leaf, leaf * 1.0):
+        out = route_tokens(scores, RouteConfig(top_k=2, normalize=normalize))
+        (g,) = torch.autograd.grad(out.weights, leaf, torch.ones_like(out.weights), create_graph=True)
+        with pytest.raises(RuntimeError, match="only once"):
+            torch.autograd.grad(g.sum(), leaf)
+
+
 # -------------------------------------------------------------------- order
 
 
