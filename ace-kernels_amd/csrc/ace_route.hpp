@@ -11,10 +11,12 @@
 // list is the answer; in float32 the lanes that hold the taken scores say which they
 // are.  Normalised weights need the chosen scores only, and their gradient no score.
 //
-// What bounds it: the forward of many experts its instructions (131072 x 256, top 8, in
-// float32: 58 us for 134 MB, the vector units busy throughout; 32 us in bfloat16), most
-// of them the lists; the backward memory (63 us for 268 MB, 4.2 TB/s; normalised 37 us
-// for 134).  Where a token has at least as many lanes as choices, each lane writes one of
+// What bounds it (131072 x 256, top 8, in a trace): the forward of many experts its
+// instructions, 59 us for 147 MB in float32 and 41 for 80 in bfloat16 (normalised 54 and
+// 35).  A float32 token's lists are about 275 vector instructions; some 370 stand before
+// the loop, for two trips of it, 142 of them spills of scalars that say which score a lane
+// has, which the trips read back.  The backward memory: 53 us for 285 MB, 5.4 TB/s
+// (normalised 37 us for 151).  Where a token has at least as many lanes as choices, each lane writes one of
 // them: with every lane writing its share of all, the forward took 65 us.
 #pragma once
 
